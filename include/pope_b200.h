@@ -69,8 +69,13 @@ typedef enum PopeStatus {
 typedef enum PopeDtype { POPE_F32 = 0, POPE_BF16 = 1, POPE_F16 = 2 } PopeDtype;
 
 typedef enum PopeOp {
-  POPE_OP_SIM_FWD = 0, POPE_OP_SIM_BWD = 1, POPE_OP_ATTN_FWD = 2, POPE_OP_ATTN_BWD = 3, POPE_OP_DECODE_PAGED = 4
+  POPE_OP_SIM_FWD = 0, POPE_OP_SIM_BWD = 1, POPE_OP_ATTN_FWD = 2, POPE_OP_ATTN_BWD = 3, POPE_OP_DECODE_PAGED = 4,
+  POPE_OP_ATTN_PAGED = 5
 } PopeOp;
+
+/* What the pages of a cache hold: values of the 16-bit type, or 8-bit codes with one fp32 scale per row (a token's k or v
+ * of one key head). */
+typedef enum PopeStore { POPE_STORE_16 = 0, POPE_STORE_INT8 = 1, POPE_STORE_E4M3 = 2 } PopeStore;
 
 /* Element strides of the batch, head and row axes (innermost axis is contiguous). */
 typedef struct PopeStride3 { int64_t b, h, n; } PopeStride3;
@@ -287,6 +292,63 @@ typedef struct PopePagedDecodeArgs {
   void* workspace; size_t workspace_bytes;
 } PopePagedDecodeArgs;
 
+/* ---- a cache that holds 8 bits ------------------------------------------------------------------------
+ * The cache of PopePagedKV with `store`: the pages hold one byte per value and every row of d values (a token's k, or its
+ * v, of one key head) has an fp32 scale, k_scales / v_scales = [num_pages][Hk][page_size].  With A = the row's largest
+ * magnitude and M = 127 (int8) or 448 (e4m3):
+ *   scale = A / M, code = x * (M / A) rounded to the nearest code (ties to even), value = code * scale.
+ * A row with A < 2^-119 holds zeros (scale 0); a row with an infinity or a NaN has the scale NaN, so that it reads back
+ * as NaN.  With POPE_STORE_16 the scales are NULL and the pages are those of PopePagedKV. */
+typedef struct PopePagedStore {
+  PopePagedKV kv;
+  float* k_scales;
+  float* v_scales;
+  int32_t store;               /* PopeStore */
+  int32_t reserved0;
+} PopePagedStore;
+
+/* Append to a cache that holds 8 bits: as PopeKvAppendArgs, the rows are quantised as they are written. */
+typedef struct PopeKvWriteArgs {
+  uint32_t struct_bytes;
+  int32_t dtype;               /* PopeDtype of k and v: POPE_BF16 or POPE_F16 */
+  int32_t B, Hk, d, n_new;
+  int32_t advance, reserved0;
+  PopePagedStore cache;
+  const void* k; PopeStride3 sk;
+  const void* v; PopeStride3 sv;
+} PopeKvWriteArgs;
+
+/* Read the rows [first, first + n) of sequence 0 of `cache` (page_table and seq_lens start at the sequence that is wanted)
+ * into k, v: (Hk, n, d) of `dtype`, strides of (head, row), rows on 16-byte boundaries.  Positions without a page read as zeros
+ * and set bit 1 of the status word. */
+typedef struct PopeKvReadArgs {
+  uint32_t struct_bytes;
+  int32_t dtype;
+  int32_t Hk, d, first, n;
+  PopePagedStore cache;
+  void* k; int64_t sk_h, sk_n;
+  void* v; int64_t sv_h, sv_n;
+} PopeKvReadArgs;
+
+/* Attention of the newest tokens of every sequence over everything the cache holds for it.  Row i < counts[b] of q (B, H, Nq, d)
+ * is the query of position seq_lens[b] - counts[b] + i and sees the keys up to that position; counts (device, may be NULL = Nq
+ * everywhere) is clamped to [0, Nq].  Rows behind the count, and rows whose position is negative, give out = 0, lse = -inf.
+ * shape.Nk = an upper bound of every seq_lens[b], as for PopePagedDecodeArgs; shape.Nq may exceed it.  dtype is that of q and
+ * out and, with POPE_STORE_16, of the pages.  lse (B, H, Nq) fp32 may be NULL.  Workspace: pope_b200_workspace_bytes(
+ * POPE_OP_ATTN_PAGED, &args). */
+typedef struct PopePagedAttnArgs {
+  uint32_t struct_bytes;
+  float softmax_scale;
+  PopeShape shape;
+  PopeEmbed embed;
+  PopePagedStore cache;
+  const int32_t* counts;
+  const void* q; PopeStride3 sq;
+  void* out;     PopeStride3 so;
+  float* lse;
+  void* workspace; size_t workspace_bytes;
+} PopePagedAttnArgs;
+
 /* ---- the embedding tables --------------------------------------------------------------------------
  * Replaces the elementwise chains of PoPE.forward and AxialPoPE.forward, PoPE_pytorch/pope.py:125-147 and
  * pope_nd.py:66-106, for integer lengths: positions of a sequence (axes = 1, dims[0] = its length) or of a
@@ -359,6 +421,9 @@ POPE_API int pope_b200_apply_qk_bwd(const PopeApplyBwdArgs* args, void* stream);
 POPE_API int pope_b200_kv_append(const PopeKvAppendArgs* args, void* stream);
 POPE_API int pope_b200_kv_map(const PopeKvMapArgs* args, void* stream);
 POPE_API int pope_b200_attn_decode_paged(const PopePagedDecodeArgs* args, void* stream);
+POPE_API int pope_b200_kv_write(const PopeKvWriteArgs* args, void* stream);
+POPE_API int pope_b200_kv_read(const PopeKvReadArgs* args, void* stream);
+POPE_API int pope_b200_attn_paged(const PopePagedAttnArgs* args, void* stream);
 POPE_API int pope_b200_table(const PopeTableArgs* args, void* stream);
 POPE_API int pope_b200_clamp_bwd(const PopeClampBwdArgs* args, void* stream);
 

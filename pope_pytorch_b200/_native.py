@@ -20,7 +20,7 @@ import torch
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG_DIR, "libpope_b200.so")
 
-OP_SIM_FWD, OP_SIM_BWD, OP_ATTN_FWD, OP_ATTN_BWD, OP_DECODE_PAGED = 0, 1, 2, 3, 4
+OP_SIM_FWD, OP_SIM_BWD, OP_ATTN_FWD, OP_ATTN_BWD, OP_DECODE_PAGED, OP_ATTN_PAGED = 0, 1, 2, 3, 4, 5
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -108,10 +108,36 @@ class PagedDecodeArgs(C.Structure):
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+STORE_16, STORE_INT8, STORE_E4M3 = 0, 1, 2
+
+
+class PagedStore(C.Structure):
+    _fields_ = [("kv", PagedKV), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p), ("store", C.c_int32), ("reserved0", C.c_int32)]
+
+
+class KvWriteArgs(C.Structure):
+    _fields_ = [("struct_bytes", C.c_uint32), ("dtype", C.c_int32), ("B", C.c_int32), ("Hk", C.c_int32), ("d", C.c_int32),
+                ("n_new", C.c_int32), ("advance", C.c_int32), ("reserved0", C.c_int32), ("cache", PagedStore),
+                ("k", C.c_void_p), ("sk", Stride3), ("v", C.c_void_p), ("sv", Stride3)]
+
+
+class KvReadArgs(C.Structure):
+    _fields_ = [("struct_bytes", C.c_uint32), ("dtype", C.c_int32), ("Hk", C.c_int32), ("d", C.c_int32), ("first", C.c_int32),
+                ("n", C.c_int32), ("cache", PagedStore), ("k", C.c_void_p), ("sk_h", C.c_int64), ("sk_n", C.c_int64),
+                ("v", C.c_void_p), ("sv_h", C.c_int64), ("sv_n", C.c_int64)]
+
+
+class PagedAttnArgs(C.Structure):
+    _fields_ = [("struct_bytes", C.c_uint32), ("softmax_scale", C.c_float), ("shape", Shape), ("embed", Embed), ("cache", PagedStore),
+                ("counts", C.c_void_p), ("q", C.c_void_p), ("sq", Stride3), ("out", C.c_void_p), ("so", Stride3), ("lse", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 EXPORTS = ("pope_b200_abi_version", "pope_b200_apply_qk_fwd", "pope_b200_apply_qk_bwd", "pope_b200_status_str", "pope_b200_last_path", "pope_b200_device_status",
            "pope_b200_clear_device_status", "pope_b200_selftest_bounded_wait",
            "pope_b200_workspace_bytes", "pope_b200_attn_fwd_noalloc", "pope_b200_kv_append", "pope_b200_attn_decode_paged",
            "pope_b200_table", "pope_b200_clamp_bwd", "pope_b200_kv_map",
+           "pope_b200_kv_write", "pope_b200_kv_read", "pope_b200_attn_paged",
            "pope_b200_sim_fwd", "pope_b200_sim_bwd", "pope_b200_attn_fwd", "pope_b200_attn_bwd")
 
 _lib = None
@@ -128,7 +154,8 @@ def _bind(lib):
     lib.pope_b200_workspace_bytes.argtypes = [C.c_int, C.c_void_p]
     for name in ("pope_b200_sim_fwd", "pope_b200_sim_bwd", "pope_b200_attn_fwd", "pope_b200_attn_bwd",
                  "pope_b200_apply_qk_fwd", "pope_b200_apply_qk_bwd", "pope_b200_kv_append", "pope_b200_attn_decode_paged",
-                 "pope_b200_table", "pope_b200_clamp_bwd", "pope_b200_kv_map"):
+                 "pope_b200_table", "pope_b200_clamp_bwd", "pope_b200_kv_map",
+                 "pope_b200_kv_write", "pope_b200_kv_read", "pope_b200_attn_paged"):
         fn = getattr(lib, name)
         fn.restype = C.c_int
         fn.argtypes = [C.c_void_p, C.c_void_p]

@@ -29,6 +29,13 @@ int check_shape(const PopeShape& s) {
   return POPE_OK;
 }
 
+// (new tokens of a sequence may outnumber the bound of its keys: their rows are then empty)
+int check_paged_shape(const PopeShape& s) {
+  PopeShape t = s;
+  t.Nk = t.Nk < t.Nq ? t.Nq : t.Nk;
+  return s.Nk <= 0 ? POPE_ERR_BAD_ARG : check_shape(t);
+}
+
 // POPE_B200_FORCE_SIMT=1 routes every call to the exact-arithmetic family (for A/B comparisons)
 bool force_simt() {
   const char* e = std::getenv("POPE_B200_FORCE_SIMT");
@@ -106,6 +113,11 @@ size_t pope_b200_workspace_bytes(int op, const void* args) {
       const PopePagedDecodeArgs& a = *static_cast<const PopePagedDecodeArgs*>(args);
       if (a.struct_bytes != sizeof(PopePagedDecodeArgs) || check_shape(a.shape) != POPE_OK) return 0;
       return pope::decode_paged_supported(a) ? pope::decode_paged_workspace(a) : 0;
+    }
+    case POPE_OP_ATTN_PAGED: {
+      const PopePagedAttnArgs& a = *static_cast<const PopePagedAttnArgs*>(args);
+      if (a.struct_bytes != sizeof(PopePagedAttnArgs) || check_paged_shape(a.shape) != POPE_OK || a.cache.kv.page_size <= 0) return 0;
+      return pope::attn_paged_supported(a) ? pope::attn_paged_workspace(a) : 0;
     }
     default: return 0;
   }
@@ -274,6 +286,67 @@ int pope_b200_attn_decode_paged(const PopePagedDecodeArgs* a, void* stream) {
   if ((rc = check_device()) != POPE_OK) return rc;
   if (pope::decode_paged(*a, static_cast<cudaStream_t>(stream)) != cudaSuccess) return POPE_ERR_CUDA;
   g_last_path = "decode_stream_paged";
+  return POPE_OK;
+}
+
+static int check_store(const PopePagedStore& c, int B) {
+  if (c.store < POPE_STORE_16 || c.store > POPE_STORE_E4M3) return POPE_ERR_BAD_ARG;
+  const int rc = check_paged(c.kv, B);
+  if (rc != POPE_OK || c.store == POPE_STORE_16) return rc;
+  if (!c.k_scales || !c.v_scales) return POPE_ERR_BAD_ARG;
+  if ((reinterpret_cast<uintptr_t>(c.k_scales) & 15) != 0 || (reinterpret_cast<uintptr_t>(c.v_scales) & 15) != 0) return POPE_ERR_MISALIGNED;
+  return POPE_OK;
+}
+
+static bool rows_on_16_bytes(const void* ptr, const PopeStride3& st) {
+  return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && st.b % 8 == 0 && st.h % 8 == 0 && st.n % 8 == 0;
+}
+
+int pope_b200_kv_write(const PopeKvWriteArgs* a, void* stream) {
+  if (!a || a->struct_bytes != sizeof(PopeKvWriteArgs)) return POPE_ERR_BAD_ARG;
+  if (a->B <= 0 || a->Hk <= 0 || a->d <= 0 || a->n_new < 0 || !a->k || !a->v) return POPE_ERR_BAD_ARG;
+  if (a->dtype != POPE_BF16 && a->dtype != POPE_F16) return POPE_ERR_UNSUPPORTED;
+  if ((a->d != 64 && a->d != 96 && a->d != 128) || a->Hk > 65535 || a->B > 65535) return POPE_ERR_UNSUPPORTED;
+  int rc = check_store(a->cache, a->B);
+  if (rc == POPE_OK && a->cache.store == POPE_STORE_16) rc = POPE_ERR_UNSUPPORTED;   // (pope_b200_kv_append)
+  if (rc != POPE_OK) return rc;
+  if (!rows_on_16_bytes(a->k, a->sk) || !rows_on_16_bytes(a->v, a->sv)) return POPE_ERR_MISALIGNED;
+  if (a->n_new == 0) return POPE_OK;
+  if ((rc = check_device()) != POPE_OK) return rc;
+  if (pope::kv_write(*a, static_cast<cudaStream_t>(stream)) != cudaSuccess) return POPE_ERR_CUDA;
+  g_last_path = "kv_write";
+  return POPE_OK;
+}
+
+int pope_b200_kv_read(const PopeKvReadArgs* a, void* stream) {
+  if (!a || a->struct_bytes != sizeof(PopeKvReadArgs)) return POPE_ERR_BAD_ARG;
+  if (a->Hk <= 0 || a->d <= 0 || a->n < 0 || a->first < 0 || a->first > INT32_MAX - a->n || !a->k || !a->v) return POPE_ERR_BAD_ARG;
+  if (a->dtype != POPE_BF16 && a->dtype != POPE_F16) return POPE_ERR_UNSUPPORTED;
+  if ((a->d != 64 && a->d != 96 && a->d != 128) || a->Hk > 65535) return POPE_ERR_UNSUPPORTED;
+  int rc = check_store(a->cache, 1);
+  if (rc != POPE_OK) return rc;
+  if (!rows_on_16_bytes(a->k, {0, a->sk_h, a->sk_n}) || !rows_on_16_bytes(a->v, {0, a->sv_h, a->sv_n})) return POPE_ERR_MISALIGNED;
+  if (a->n == 0) return POPE_OK;
+  if ((rc = check_device()) != POPE_OK) return rc;
+  if (pope::kv_read(*a, static_cast<cudaStream_t>(stream)) != cudaSuccess) return POPE_ERR_CUDA;
+  g_last_path = "kv_read";
+  return POPE_OK;
+}
+
+int pope_b200_attn_paged(const PopePagedAttnArgs* a, void* stream) {
+  if (!a || a->struct_bytes != sizeof(PopePagedAttnArgs)) return POPE_ERR_BAD_ARG;
+  int rc = check_paged_shape(a->shape);
+  if (rc == POPE_OK) rc = check_embed(a->shape, a->embed);
+  if (rc == POPE_OK) rc = check_store(a->cache, a->shape.B);
+  if (rc != POPE_OK) return rc;
+  if (!a->q || !a->out) return POPE_ERR_BAD_ARG;
+  if (!pope::attn_paged_supported(*a)) return POPE_ERR_UNSUPPORTED;
+  const size_t need = pope::attn_paged_workspace(*a);
+  if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return POPE_ERR_WORKSPACE;
+  if (need > 0 && (reinterpret_cast<uintptr_t>(a->workspace) & 255) != 0) return POPE_ERR_MISALIGNED;
+  if ((rc = check_device()) != POPE_OK) return rc;
+  if (pope::attn_paged(*a, static_cast<cudaStream_t>(stream)) != cudaSuccess) return POPE_ERR_CUDA;
+  g_last_path = "attn_paged";
   return POPE_OK;
 }
 

@@ -39,6 +39,12 @@ size_t decode_paged_workspace(const PopePagedDecodeArgs& a);
 cudaError_t decode_paged(const PopePagedDecodeArgs& a, cudaStream_t st);
 cudaError_t kv_append(const PopeKvAppendArgs& a, cudaStream_t st);
 cudaError_t kv_map(const PopeKvMapArgs& a, cudaStream_t st);
+// a cache that holds 8 bits: rows quantised as they are written, rows read back; attention of the newest tokens over a cache
+cudaError_t kv_write(const PopeKvWriteArgs& a, cudaStream_t st);
+cudaError_t kv_read(const PopeKvReadArgs& a, cudaStream_t st);
+bool attn_paged_supported(const PopePagedAttnArgs& a);
+size_t attn_paged_workspace(const PopePagedAttnArgs& a);
+cudaError_t attn_paged(const PopePagedAttnArgs& a, cudaStream_t st);
 // phase table, clamped bias and the clamp's gradient
 cudaError_t pope_table(const PopeTableArgs& a, cudaStream_t st);
 cudaError_t pope_clamp_bwd(const PopeClampBwdArgs& a, cudaStream_t st);

@@ -1,0 +1,215 @@
+// Rows of a paged cache that holds 8 bits: quantised as they are appended, and read back (sm_100a).
+//
+// A row x of d values (a token's k, or its v, of one key head) with A = max |x| is stored as codes x * (M / A), rounded to
+// the nearest code, and the scale A / M (M = 127 for int8, 448 for e4m3): the value of a code is code * scale.  Both kernels move
+// their bytes once and are bound by memory: a lane holds 8 values of a row (one 16-byte access on the 16-bit side, 8 bytes on
+// the other), 8 or 16 lanes share a row, and a warp has several rows in flight.
+#include "kernels.h"
+#include "paged.cuh"
+
+namespace pope {
+
+struct KvWriteP {
+  PagedPtrs c;
+  int n_new, advance;
+  const void *k, *v;
+  Strides sk, sv;
+};
+
+// The largest magnitude over the lanes of a row, as bits: ordered like the values, with infinities and NaNs above all of them.
+template <int LPR> __device__ __forceinline__ uint32_t row_max_bits(uint32_t m) {
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
+}
+
+// Eight values of a row (raw words), the row's maximum over its LPR lanes -> eight codes and the scale.
+template <typename T, int STORE, int LPR>
+__device__ __forceinline__ uint2 quantise8(const uint4& raw, float* scale) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = max(m, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+  m = row_max_bits<LPR>(m);
+  const bool finite = m < (sizeof(T) == 2 && TcFmt<T>::fmt == FMT_BF16 ? 0x7f80u : 0x7c00u);
+  const float top = unpack2<T>(m).x;
+  if (!finite || top < ROW_LEAST) {
+    *scale = finite ? 0.f : __int_as_float(0x7fffffff);
+    return make_uint2(0, 0);
+  }
+  *scale = __fdiv_rn(top, kCodeTop<STORE>);
+  const float inv = __fdiv_rn(kCodeTop<STORE>, top);
+  uint32_t out[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float2 a = unpack2<T>(w[2 * i]), b = unpack2<T>(w[2 * i + 1]);
+    const float y[4] = {__fmul_rn(a.x, inv), __fmul_rn(a.y, inv), __fmul_rn(b.x, inv), __fmul_rn(b.y, inv)};
+    if constexpr (STORE == POPE_STORE_INT8) {
+      // |y| <= 127 + 2^-16: y + 1.5 * 2^23 rounds it to an integer, ties to even, whose low byte is the code
+      uint32_t c[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c[e] = __float_as_uint(__fadd_rn(y[e], 12582912.f));
+      out[i] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+    } else {
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+      out[i] = lo | hi << 16;
+    }
+  }
+  return make_uint2(out[0], out[1]);
+}
+
+// Row `tensor` (0 = k, 1 = v) of token i, head hk: every lane of the warp calls this; `on` = the lane has a row at all.
+template <typename T, int STORE, int D, int LPR>
+__device__ __forceinline__ void write_row(const KvWriteP& p, int b, int hk, int i, int tensor, int len, int lane, bool on) {
+  on = on && lane * 8 < D;
+  const Strides& s = tensor ? p.sv : p.sk;
+  const T* src = static_cast<const T*>(tensor ? p.v : p.k) + b * s.b + hk * s.h + (int64_t)i * s.n + lane * 8;
+  uint4 raw = make_uint4(0, 0, 0, 0);
+  if (on) raw = *reinterpret_cast<const uint4*>(src);
+  float scale;
+  const uint2 codes = quantise8<T, STORE, LPR>(raw, &scale);
+  if (!on) return;
+  const int64_t row = paged_row(p.c, b, hk, len + i);
+  if (row < 0) return;
+  *reinterpret_cast<uint2*>((tensor ? p.c.v : p.c.k) + row * D + lane * 8) = codes;
+  if (lane == 0) (tensor ? p.c.v_scales : p.c.k_scales)[row] = scale;
+}
+
+constexpr int KW_ROWS = 4;   // rows of each of k and v that a group of lanes takes
+template <typename T, int STORE, int D>
+__global__ void __launch_bounds__(256) kv_write_kernel(KvWriteP p) {
+  constexpr int LPR = D == 64 ? 8 : 16;
+  const int group = threadIdx.x / LPR, lane = threadIdx.x % LPR, b = blockIdx.z;
+  pdl_wait();
+  const int len = p.c.seq_lens[b];
+#pragma unroll
+  for (int j = 0; j < KW_ROWS; ++j) {
+    const int i = (blockIdx.x * KW_ROWS + j) * (256 / LPR) + group;
+    write_row<T, STORE, D, LPR>(p, b, blockIdx.y, i, 0, len, lane, i < p.n_new);
+    write_row<T, STORE, D, LPR>(p, b, blockIdx.y, i, 1, len, lane, i < p.n_new);
+  }
+}
+
+// A few tokens (a decode step): one CTA per sequence, which advances the length itself once all of its threads have read it.
+constexpr int KW_STEP_ROWS = 512;
+template <typename T, int STORE, int D>
+__global__ void __launch_bounds__(256) kv_write_step_kernel(KvWriteP p) {
+  constexpr int LPR = D == 64 ? 8 : 16;
+  const int group = threadIdx.x / LPR, lane = threadIdx.x % LPR, b = blockIdx.x;
+  pdl_wait();
+  const int len = p.c.seq_lens[b], rows = p.c.Hk * p.n_new;
+  for (int first = 0; first < 2 * rows; first += 256 / LPR) {   // (whole warps stay in the loop: the maxima are warp operations)
+    const int at = first + group, row = at >> 1;
+    write_row<T, STORE, D, LPR>(p, b, min(row, rows - 1) / p.n_new, row % p.n_new, at & 1, len, lane, row < rows);
+  }
+  __syncthreads();
+  if (p.advance && threadIdx.x == 0) p.c.seq_lens[b] = len + p.n_new;
+}
+
+__global__ void kv_write_advance_kernel(int32_t* seq_lens, int B, int n_new) {
+  pdl_wait();
+  const int b = blockIdx.x * blockDim.x + threadIdx.x;
+  if (b < B) seq_lens[b] += n_new;
+}
+
+template <typename T, int STORE, int D> static cudaError_t kv_write_t(const PopeKvWriteArgs& a, cudaStream_t st) {
+  KvWriteP p;
+  p.c = paged_ptrs(a.cache, a.Hk, a.d);
+  if (!p.c.status) return cudaErrorInvalidSymbol;
+  p.n_new = a.n_new, p.advance = a.advance;
+  p.k = a.k, p.v = a.v, p.sk = Strides(a.sk), p.sv = Strides(a.sv);
+  if ((int64_t)a.Hk * a.n_new * 2 <= KW_STEP_ROWS) return launch_dependent(kv_write_step_kernel<T, STORE, D>, dim3(a.B), dim3(256), 0, st, p);
+  constexpr int rows = KW_ROWS * 256 / (D == 64 ? 8 : 16);
+  const dim3 grid((unsigned)((a.n_new + rows - 1) / rows), (unsigned)a.Hk, (unsigned)a.B);
+  cudaError_t e = launch_dependent(kv_write_kernel<T, STORE, D>, grid, dim3(256), 0, st, p);
+  if (e != cudaSuccess || !a.advance) return e;
+  return launch_dependent(kv_write_advance_kernel, dim3((a.B + 255) / 256), dim3(256), 0, st, p.c.seq_lens, (int)a.B, (int)a.n_new);
+}
+template <typename T, int STORE> static cudaError_t kv_write_d(const PopeKvWriteArgs& a, cudaStream_t st) {
+  return a.d == 64 ? kv_write_t<T, STORE, 64>(a, st) : a.d == 96 ? kv_write_t<T, STORE, 96>(a, st) : kv_write_t<T, STORE, 128>(a, st);
+}
+template <typename T> static cudaError_t kv_write_s(const PopeKvWriteArgs& a, cudaStream_t st) {
+  return a.cache.store == POPE_STORE_INT8 ? kv_write_d<T, POPE_STORE_INT8>(a, st) : kv_write_d<T, POPE_STORE_E4M3>(a, st);
+}
+cudaError_t kv_write(const PopeKvWriteArgs& a, cudaStream_t st) {
+  return a.dtype == POPE_BF16 ? kv_write_s<__nv_bfloat16>(a, st) : kv_write_s<__half>(a, st);
+}
+
+// ---- reading back ----------------------------------------------------------------------------------
+struct KvReadP {
+  PagedPtrs c;
+  int first, n;
+  void *k, *v;
+  int64_t sk_h, sk_n, sv_h, sv_n;
+};
+
+constexpr int KR_ROWS = 4;   // rows of each of k and v that a group of lanes takes: all their loads are issued before the first store
+template <typename T, int STORE, int D>
+__global__ void __launch_bounds__(256) kv_read_kernel(KvReadP p) {
+  constexpr int LPR = D == 64 ? 8 : 16, CB = STORE == POPE_STORE_16 ? 16 : 8;   // bytes of a lane's eight values in the page
+  const int group = threadIdx.x / LPR, lane = threadIdx.x % LPR, hk = blockIdx.y;
+  pdl_wait();
+  if (lane * 8 >= D) return;
+  uint4 held[KR_ROWS][2];
+  float scale[KR_ROWS][2];
+#pragma unroll
+  for (int j = 0; j < KR_ROWS; ++j) {
+    const int i = (blockIdx.x * KR_ROWS + j) * (256 / LPR) + group;
+    const int64_t row = i < p.n ? paged_row(p.c, 0, hk, p.first + i) : -1;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      held[j][t] = make_uint4(0, 0, 0, 0), scale[j][t] = 0.f;
+      if (row < 0) continue;
+      const uint8_t* src = (t ? p.c.v : p.c.k) + row * p.c.row_bytes + lane * CB;
+      if constexpr (STORE == POPE_STORE_16) {
+        held[j][t] = *reinterpret_cast<const uint4*>(src);
+      } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(src);
+        held[j][t].x = w.x, held[j][t].y = w.y;
+        scale[j][t] = (t ? p.c.v_scales : p.c.k_scales)[row];
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < KR_ROWS; ++j) {
+    const int i = (blockIdx.x * KR_ROWS + j) * (256 / LPR) + group;
+    if (i >= p.n) continue;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      uint4 o = held[j][t];
+      if constexpr (STORE != POPE_STORE_16) {
+        float x[8], *lo = x, *hi = x + 4;
+        codes_to_f32<STORE>(o.x, *reinterpret_cast<float(*)[4]>(lo)), codes_to_f32<STORE>(o.y, *reinterpret_cast<float(*)[4]>(hi));
+        const float s = scale[j][t];
+        o = make_uint4(pack2<T>(x[0] * s, x[1] * s), pack2<T>(x[2] * s, x[3] * s), pack2<T>(x[4] * s, x[5] * s), pack2<T>(x[6] * s, x[7] * s));
+      }
+      T* dst = static_cast<T*>(t ? p.v : p.k) + hk * (t ? p.sv_h : p.sk_h) + (int64_t)i * (t ? p.sv_n : p.sk_n) + lane * 8;
+      *reinterpret_cast<uint4*>(dst) = o;
+    }
+  }
+}
+
+template <typename T, int STORE, int D> static cudaError_t kv_read_t(const PopeKvReadArgs& a, cudaStream_t st) {
+  KvReadP p;
+  p.c = paged_ptrs(a.cache, a.Hk, a.d);
+  if (!p.c.status) return cudaErrorInvalidSymbol;
+  p.first = a.first, p.n = a.n, p.k = a.k, p.v = a.v, p.sk_h = a.sk_h, p.sk_n = a.sk_n, p.sv_h = a.sv_h, p.sv_n = a.sv_n;
+  constexpr int rows = KR_ROWS * 256 / (D == 64 ? 8 : 16);
+  return launch_dependent(kv_read_kernel<T, STORE, D>, dim3((unsigned)((a.n + rows - 1) / rows), (unsigned)a.Hk), dim3(256), 0, st, p);
+}
+template <typename T, int STORE> static cudaError_t kv_read_d(const PopeKvReadArgs& a, cudaStream_t st) {
+  return a.d == 64 ? kv_read_t<T, STORE, 64>(a, st) : a.d == 96 ? kv_read_t<T, STORE, 96>(a, st) : kv_read_t<T, STORE, 128>(a, st);
+}
+template <typename T> static cudaError_t kv_read_s(const PopeKvReadArgs& a, cudaStream_t st) {
+  switch (a.cache.store) {
+    case POPE_STORE_INT8: return kv_read_d<T, POPE_STORE_INT8>(a, st);
+    case POPE_STORE_E4M3: return kv_read_d<T, POPE_STORE_E4M3>(a, st);
+    default: return kv_read_d<T, POPE_STORE_16>(a, st);
+  }
+}
+cudaError_t kv_read(const PopeKvReadArgs& a, cudaStream_t st) {
+  return a.dtype == POPE_BF16 ? kv_read_s<__nv_bfloat16>(a, st) : kv_read_s<__half>(a, st);
+}
+
+}  // namespace pope

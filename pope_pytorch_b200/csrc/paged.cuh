@@ -1,0 +1,61 @@
+// Helpers of the kernels that read and write a paged cache (sm_100a): where a row sits, and what its codes stand for.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "tc_common.cuh"
+
+namespace pope {
+
+// The cache as a kernel sees it; a row of d values is `row_bytes` long.
+struct PagedPtrs {
+  uint8_t *k, *v;                 // [num_pages][Hk][page_size][row_bytes]
+  float *k_scales, *v_scales;     // [num_pages][Hk][page_size], 8-bit stores
+  const int32_t* page_table;
+  int32_t* seq_lens;
+  int Hk, page_size, max_pages, num_pages, row_bytes;
+  unsigned int* status;
+};
+inline PagedPtrs paged_ptrs(const PopePagedStore& c, int Hk, int d) {
+  PagedPtrs p;
+  p.k = static_cast<uint8_t*>(c.kv.k_pages), p.v = static_cast<uint8_t*>(c.kv.v_pages);
+  p.k_scales = c.k_scales, p.v_scales = c.v_scales;
+  p.page_table = c.kv.page_table, p.seq_lens = c.kv.seq_lens;
+  p.Hk = Hk, p.page_size = c.kv.page_size, p.max_pages = c.kv.max_pages_per_seq, p.num_pages = c.kv.num_pages;
+  p.row_bytes = c.store == POPE_STORE_16 ? 2 * d : d;
+  p.status = tc_status_ptr();
+  return p;
+}
+
+// Row number, in the pool, of token `pos` of sequence b and key head hk; -1 (and status bit 1) where the cache has no such row.
+__device__ __forceinline__ int64_t paged_row(const PagedPtrs& p, int b, int hk, int pos) {
+  const int lp = pos / p.page_size;
+  const int pg = pos >= 0 && lp < p.max_pages ? p.page_table[(int64_t)b * p.max_pages + lp] : -1;
+  if (pg < 0 || pg >= p.num_pages) {
+    atomicOr(p.status, 2u);
+    return -1;
+  }
+  return ((int64_t)pg * p.Hk + hk) * p.page_size + (pos - lp * p.page_size);
+}
+
+// ---- 8-bit codes -----------------------------------------------------------------------------------
+constexpr float ROW_LEAST = 1.5046327690525280e-36f;   // 2^-119: M / A of a smaller A would leave the range
+template <int STORE> constexpr float kCodeTop = STORE == POPE_STORE_INT8 ? 127.f : 448.f;
+
+// four codes of a word as fp32.  int8: the byte with its top bit flipped is code + 128, placed into the low mantissa bits of
+// 2^23 it makes 2^23 + code + 128, exactly.
+template <int STORE> __device__ __forceinline__ void codes_to_f32(uint32_t w, float (&x)[4]) {
+  if constexpr (STORE == POPE_STORE_INT8) {
+    w ^= 0x80808080u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + i)) - 8388736.f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * i)), __NV_E4M3);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    }
+  }
+}
+
+}  // namespace pope

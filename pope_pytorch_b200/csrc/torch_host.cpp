@@ -466,7 +466,20 @@ optional<std::vector<Tensor>> table(const Tensor& bias, const std::vector<Tensor
 // ---- paged key / value cache ---------------------------------------------------------------------------------------
 // The cache's tensors; `row` > 0 = the view that starts at sequence `row` (a batch of one)
 struct Pages {
-  Tensor k, v, table, lens;
+  Tensor k, v, table, lens, k_scales, v_scales;   // the scales of a cache that holds 8 bits
+  int store() const {
+    switch (k.scalar_type()) {
+      case at::kChar: return POPE_STORE_INT8;
+      case at::kFloat8_e4m3fn: return POPE_STORE_E4M3;
+      default: return POPE_STORE_16;
+    }
+  }
+  PopePagedStore held(int64_t row = 0) const {
+    PopePagedStore c = {};
+    c.kv = view(row), c.store = store();
+    if (c.store != POPE_STORE_16) c.k_scales = k_scales.mutable_data_ptr<float>(), c.v_scales = v_scales.mutable_data_ptr<float>();
+    return c;
+  }
   PopePagedKV view(int64_t row = 0) const {
     PopePagedKV kv = {};
     kv.k_pages = k.mutable_data_ptr(), kv.v_pages = v.mutable_data_ptr();
@@ -495,11 +508,21 @@ void kv_append(const Pages& p, const Tensor& k_, const Tensor& v_, int64_t row) 
   const bool one = k.dim() == 3;
   const int64_t h = one ? 0 : 1;
   TORCH_CHECK_INDEX(row >= 0 && row + (one ? 1 : k.size(0)) <= p.lens.size(0), "sequence ", row, " is not in the cache");
+  // (the two structs share their fields but for the cache)
+  const auto fill = [&](auto& a) {
+    a.struct_bytes = sizeof(a), a.dtype = dtype_of(k), a.B = one ? 1 : (int32_t)k.size(0), a.Hk = (int32_t)k.size(h), a.d = (int32_t)k.size(h + 2);
+    a.n_new = (int32_t)k.size(h + 1), a.advance = 1;
+    a.k = k.const_data_ptr(), a.sk = {one ? 0 : k.stride(0), k.stride(h), k.stride(h + 1)};
+    a.v = v.const_data_ptr(), a.sv = {one ? 0 : v.stride(0), v.stride(h), v.stride(h + 1)};
+  };
+  if (p.store() != POPE_STORE_16) {
+    PopeKvWriteArgs a = {};
+    fill(a), a.cache = p.held(row);
+    check(pope_b200_kv_write(&a, stream_of(k)), "pope_b200_kv_write");
+    return;
+  }
   PopeKvAppendArgs a = {};
-  a.struct_bytes = sizeof(a), a.dtype = dtype_of(k), a.B = one ? 1 : (int32_t)k.size(0), a.Hk = (int32_t)k.size(h), a.d = (int32_t)k.size(h + 2);
-  a.n_new = (int32_t)k.size(h + 1), a.advance = 1, a.kv = p.view(row);
-  a.k = k.const_data_ptr(), a.sk = {one ? 0 : k.stride(0), k.stride(h), k.stride(h + 1)};
-  a.v = v.const_data_ptr(), a.sv = {one ? 0 : v.stride(0), v.stride(h), v.stride(h + 1)};
+  fill(a), a.kv = p.view(row);
   check(pope_b200_kv_append(&a, stream_of(k)), "pope_b200_kv_append");
 }
 
@@ -521,6 +544,45 @@ std::tuple<Tensor, Tensor> kv_decode(const Pages& p, const Tensor& q_, const Ten
   return {out, lse};
 }
 
+// rows [first, first + n) of sequence `row` -> (k, v), (hk, n, d) each, in `dtype`
+std::tuple<Tensor, Tensor> kv_read(const Pages& p, int64_t row, int64_t first, int64_t n, at::ScalarType dtype) {
+  py::gil_scoped_release nogil;
+  c10::cuda::OptionalCUDAGuard guard(p.k.device());
+  at::NoGradGuard off;
+  TORCH_CHECK_INDEX(row >= 0 && row < p.lens.size(0) && first >= 0 && n >= 0 && first + n <= INT32_MAX, "rows ", first, " to ", first + n, " of sequence ", row);
+  const auto opt = p.k.options().dtype(dtype);
+  Tensor k = at::empty({p.k.size(1), n, p.k.size(3)}, opt), v = at::empty({p.k.size(1), n, p.k.size(3)}, opt);
+  if (n == 0) return {k, v};
+  PopeKvReadArgs a = {};
+  a.struct_bytes = sizeof(a), a.dtype = dtype_of(k), a.Hk = (int32_t)k.size(0), a.d = (int32_t)k.size(2), a.first = (int32_t)first, a.n = (int32_t)n;
+  a.cache = p.held(row);
+  a.k = k.mutable_data_ptr(), a.sk_h = k.stride(0), a.sk_n = k.stride(1), a.v = v.mutable_data_ptr(), a.sv_h = v.stride(0), a.sv_n = v.stride(1);
+  check(pope_b200_kv_read(&a, stream_of(k)), "pope_b200_kv_read");
+  return {k, v};
+}
+
+// q (b, h, n, d): the newest tokens of every sequence, counts (b) of them where given -> (out, lse (b, h, n))
+std::tuple<Tensor, Tensor> kv_attend(const Pages& p, const Tensor& q_, const Tensor& freqs_, const Tensor& bias_, const optional<Tensor>& counts,
+                                     double scale, int64_t nk) {
+  validate_embed(q_, q_.size(0), q_.size(1), p.k.size(1), freqs_, bias_);
+  py::gil_scoped_release nogil;
+  c10::cuda::OptionalCUDAGuard guard(p.k.device());
+  at::NoGradGuard off;
+  const Tensor q = inner_contig(q_), freqs = fp32_rows(freqs_), bias = fp32_rows(bias_);
+  const int r = (int)freqs.size(-1);
+  Tensor out = at::empty_like(q), lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+  if (q.size(2) == 0) return {out, lse};
+  PopePagedAttnArgs a = {};
+  a.struct_bytes = sizeof(a), a.softmax_scale = (float)scale;
+  a.shape = {(int32_t)q.size(0), (int32_t)q.size(1), (int32_t)p.k.size(1), (int32_t)q.size(2), (int32_t)nk, (int32_t)q.size(3), r, dtype_of(q)};
+  a.embed = embed_of(freqs, bias, r), a.cache = p.held();
+  if (counts) a.counts = counts->const_data_ptr<int32_t>();
+  a.q = q.const_data_ptr(), a.sq = s3(q), a.out = out.mutable_data_ptr(), a.so = s3(out), a.lse = lse.mutable_data_ptr<float>();
+  const Tensor ws = workspace(POPE_OP_ATTN_PAGED, a, q);
+  check(pope_b200_attn_paged(&a, stream_of(q)), "pope_b200_attn_paged");
+  return {out, lse};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -530,10 +592,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("apply_qk", &apply_qk);
   m.def("apply_qk_takes", &apply_qk_takes);
   m.def("table", &table);
-  py::class_<Pages>(m, "Pages").def(py::init([](Tensor k, Tensor v, Tensor table, Tensor lens) { return Pages{k, v, table, lens}; }));
+  py::class_<Pages>(m, "Pages").def(py::init([](Tensor k, Tensor v, Tensor table, Tensor lens, optional<Tensor> k_scales, optional<Tensor> v_scales) {
+    return Pages{k, v, table, lens, k_scales.value_or(Tensor()), v_scales.value_or(Tensor())};
+  }), py::arg("k"), py::arg("v"), py::arg("table"), py::arg("lens"), py::arg("k_scales") = py::none(), py::arg("v_scales") = py::none());
   m.def("kv_map", &kv_map);
   m.def("kv_append", &kv_append);
   m.def("kv_decode", &kv_decode);
+  m.def("kv_read", [](const Pages& p, int64_t row, int64_t first, int64_t n, bool bf16) { return kv_read(p, row, first, n, bf16 ? at::kBFloat16 : at::kHalf); });
+  m.def("kv_attend", &kv_attend);
   m.def("attn_forward", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& freqs, const Tensor& bias, const optional<Tensor>& mask,
                            bool causal, double scale, const Factors& factors) {
     validate_attn(q, k, v, freqs, bias, mask, false);

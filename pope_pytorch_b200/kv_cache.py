@@ -1,19 +1,25 @@
-"""Paged key / value cache for single-token decode with PoPE attention.
+"""Paged key / value cache for decode and chunked prefill with PoPE attention.
 
 The reference has no cache: every decode step calls ``flash_attn_with_pope`` with the full K and V
 (PoPE_pytorch/attention.py:75-145; the query then sits at the last position, PoPE_pytorch/pope.py:64).
 This is the serving-side step either side of that call: ``append`` writes the new rows of k and v into
 fixed-size pages, ``decode`` attends one new query row per (batch, head) over everything a sequence holds.
+``attend`` does the same for a chunk of new tokens at a time, ``read`` gives stored rows back and ``rollback`` forgets the newest.
 Raw k is cached; the polar transform is applied inside the decode kernel as the keys stream through
 shared memory, so cached entries do not depend on the phase bias.
 
+With ``store`` the cache holds 8 bits per value and one fp32 scale per row (a token's k, or its v, of one key head): half the
+memory, and half of what a decode step reads.  Rows are quantised as they are appended and every call on the cache works as on
+a 16-bit cache of the values that the codes stand for.
+
 Page bookkeeping (free list, page table, lengths) is host policy and lives here; the library only reads the
-table (``pope_b200_kv_append`` / ``pope_b200_attn_decode_paged`` in include/pope_b200.h).  All arithmetic is
+table (``pope_b200_kv_append``, ``pope_b200_kv_write``, ``pope_b200_attn_decode_paged``, ``pope_b200_attn_paged``, ``pope_b200_kv_read``
+in include/pope_b200.h).  All arithmetic is
 in the CUDA library; there is no fallback.
 """
 from __future__ import annotations
 
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Union
 
 import torch
 
@@ -62,6 +68,15 @@ class PageAllocator:
         for b in (range(self.batch) if rows is None else rows):
             self.lens[b] += n_new
 
+    def rollback(self, counts: Sequence[int]) -> None:
+        """Take the newest ``counts[b]`` keys off every sequence; pages that then hold none go back to the pool, the newest
+        first, so that they are handed out again in the same order."""
+        for b, n in enumerate(counts):
+            self.lens[b] -= n
+            keep = -(-self.lens[b] // self.page_size)
+            self.free.extend(reversed(self.table[b][keep:]))
+            del self.table[b][keep:]
+
     def release(self, b: int) -> None:
         """Return every page of sequence ``b`` to the pool."""
         self.free.extend(reversed(self.table[b]))
@@ -72,24 +87,41 @@ class PageAllocator:
 class PagedKVCache:
     """K and V pages ``(num_pages, kv_heads, page_size, head_dim)`` on one GPU plus their page table.
 
+    ``dtype`` is the type of k, v, q and the results.  ``store`` is what the pages hold: ``None`` that type itself,
+    ``torch.int8`` or ``torch.float8_e4m3fn`` codes with the scales ``k_scales`` / ``v_scales`` ``(num_pages, kv_heads, page_size)``.
+    With A the largest magnitude of a row and M = 127 or 448 its scale is A / M, its codes are x * (M / A) rounded to the nearest
+    (ties to even), and a code stands for code * scale.  (A row with A < 2^-119 is held as zeros; one with an infinity or a NaN reads
+    back as NaN.)
+
     >>> cache = PagedKVCache(batch, kv_heads, head_dim, num_pages=..., page_size=256, max_seq_len=32768)
     >>> cache.append(k_prompt, v_prompt)            # (b, hk, n, d)
     >>> out = cache.decode(q, pope(cache.max_len))  # q (b, h, 1, d) at the last cached position
+    >>> cache.append(k_next, v_next)                # a chunk of the prompt: (b, hk, m, d)
+    >>> out = cache.attend(q_next, pope(cache.max_len))   # q (b, h, m, d) at the last m positions
     """
 
+    store: Optional[torch.dtype] = None      # (also of caches that were pickled before there was a choice)
+    k_scales = v_scales = None
+
     def __init__(self, batch: int, kv_heads: int, head_dim: int, *, num_pages: int, page_size: int = 256,
-                 max_seq_len: Optional[int] = None, dtype: torch.dtype = torch.bfloat16, device="cuda"):
+                 max_seq_len: Optional[int] = None, dtype: torch.dtype = torch.bfloat16, device="cuda",
+                 store: Optional[torch.dtype] = None):
         if dtype not in (torch.bfloat16, torch.float16):
             raise TypeError("the paged cache holds bf16 or fp16")
         if head_dim not in (64, 96, 128):
             raise ValueError("head_dim must be 64, 96 or 128")
+        if store not in (None, dtype, torch.int8, torch.float8_e4m3fn):
+            raise TypeError("the pages hold the cache's dtype, int8 or float8_e4m3fn")
+        self.store = None if store == dtype else store
         self.device = torch.device(device)
         max_pages = num_pages if max_seq_len is None else -(-max_seq_len // page_size)
         self.alloc = PageAllocator(batch, num_pages, page_size, max_pages)
         self.batch, self.kv_heads, self.head_dim, self.dtype = batch, kv_heads, head_dim, dtype
-        self.k_pages = torch.zeros(num_pages, kv_heads, page_size, head_dim, dtype=dtype, device=self.device)
+        self.k_pages = torch.zeros(num_pages, kv_heads, page_size, head_dim, dtype=self.store or dtype, device=self.device)
         self.v_pages = torch.zeros_like(self.k_pages)
         self.device = self.k_pages.device   # with its index
+        if self.store is not None:
+            self.k_scales, self.v_scales = (torch.zeros(num_pages, kv_heads, page_size, device=self.device) for _ in range(2))
         self.page_table = torch.zeros(batch, max_pages, dtype=torch.int32, device=self.device)
         self.seq_lens = torch.zeros(batch, dtype=torch.int32, device=self.device)
         self._held = None
@@ -110,10 +142,12 @@ class PagedKVCache:
     def _pages(self):
         """The cache's tensors as the binding takes them (they are fixed for the life of the cache)."""
         held = self._held
-        if held is None or held[0] is not self.k_pages or held[1] is not self.v_pages or held[2] is not self.page_table or held[3] is not self.seq_lens:
-            tensors = (self.k_pages, self.v_pages, self.page_table, self.seq_lens)
+        tensors = (self.k_pages, self.v_pages, self.page_table, self.seq_lens)
+        if self.store is not None:
+            tensors += (self.k_scales, self.v_scales)
+        if held is None or any(a is not b for a, b in zip(held, tensors)):
             self._held = held = (*tensors, N._ops().Pages(*tensors))
-        return held[4]
+        return held[-1]
 
     def __getstate__(self):
         return {**self.__dict__, "_held": None}   # (the binding's object is made again; copies have tensors of their own)
@@ -135,7 +169,20 @@ class PagedKVCache:
         self.alloc.release(b)
         N._ops().kv_map(self._pages(), [-1 - b], [0])
 
-    # ---- the two operators -------------------------------------------------------------------------
+    def rollback(self, counts: Union[int, Sequence[int]]) -> None:
+        """Forget the newest ``counts[b]`` tokens of every sequence (one number: of each); what remains stays as it is.  Drafted
+        tokens that were not accepted, for one."""
+        counts = [counts] * self.batch if isinstance(counts, int) else [int(n) for n in counts]
+        if len(counts) != self.batch:
+            raise ValueError("one count per sequence")
+        if any(not 0 <= n <= held for n, held in zip(counts, self.alloc.lens)):
+            raise ValueError("a sequence does not hold that many tokens")
+        rows = [b for b, n in enumerate(counts) if n]
+        if rows:
+            self.alloc.rollback(counts)
+            N._ops().kv_map(self._pages(), [-1 - b for b in rows], [self.alloc.lens[b] for b in rows])
+
+    # ---- the operators -------------------------------------------------------------------------
     def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
         """k, v: (batch, kv_heads, n_new, head_dim) views with contiguous features; every sequence grows by n_new."""
         if k.shape != v.shape or k.ndim != 4 or k.shape[0] != self.batch or k.shape[1] != self.kv_heads or k.shape[3] != self.head_dim:
@@ -177,12 +224,55 @@ class PagedKVCache:
         if r > 0 and freqs.shape[0] < nk:
             raise ValueError("freqs must cover every cached position")
         scale = self.head_dim ** -0.5 if softmax_scale is None else softmax_scale
-        out, lse = N._ops().kv_decode(self._pages(), q, freqs, bias, scale, nk)
+        if self.store is None:
+            out, lse = N._ops().kv_decode(self._pages(), q, freqs, bias, scale, nk)
+        else:
+            out, lse = N._ops().kv_attend(self._pages(), q, freqs, bias, None, scale, nk)
+            lse = lse[..., 0]
         return (out, lse) if return_lse else out
+
+    def attend(self, q: torch.Tensor, pos_emb, counts: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None,
+               return_lse: bool = False):
+        """q: (batch, heads, n, head_dim), the queries of the newest tokens of every sequence, whose k and v have been appended:
+        row i stands at position ``len - n + i`` and sees the keys up to its own.  ``counts``, an int32 tensor (batch,) on the
+        cache's device, gives sequences fewer new tokens than n: row i < counts[b] then stands at ``len - counts[b] + i`` and the
+        rows behind are padding (counts outside [0, n] are clamped).  Padding, and rows at negative positions, give zeros (lse -inf).
+        pos_emb: (freqs, bias) with at least ``max_len`` rows of freqs.  Returns out (batch, heads, n, head_dim) in q's dtype and
+        layout (and lse (batch, heads, n) on request)."""
+        freqs, bias = pos_emb
+        if q.ndim != 4 or q.shape[0] != self.batch or q.shape[3] != self.head_dim or q.shape[1] == 0 or q.shape[1] % self.kv_heads != 0:
+            raise ValueError("q must be (batch, heads, n, head_dim) with heads a multiple of kv_heads")
+        if q.dtype != self.dtype or q.device != self.device:
+            raise TypeError("q must have the cache's dtype and device")
+        r, nk = freqs.shape[-1], max(self.max_len, 1)
+        if freqs.ndim != 2:
+            raise ValueError("the paged attention takes a (positions, rotate_dim) table")
+        if r > 0 and freqs.shape[0] < nk:
+            raise ValueError("freqs must cover every cached position")
+        if counts is not None:
+            if counts.dtype != torch.int32 or counts.device != self.device:
+                raise TypeError("counts must be int32 on the cache's device")
+            if counts.shape != (self.batch,):
+                raise ValueError("counts must be (batch,)")
+            counts = counts.contiguous()
+        scale = self.head_dim ** -0.5 if softmax_scale is None else softmax_scale
+        out, lse = N._ops().kv_attend(self._pages(), q, freqs, bias, counts, scale, nk)
+        return (out, lse) if return_lse else out
+
+    def read(self, b: int, start: int = 0, stop: Optional[int] = None):
+        """Keys and values [start, stop) of sequence ``b``, contiguous (kv_heads, stop - start, head_dim) each, in the cache's
+        dtype: of an 8-bit cache the values that the codes stand for."""
+        b = self._row(b)
+        stop = self.alloc.lens[b] if stop is None else stop
+        if not 0 <= start <= stop <= self.alloc.lens[b]:
+            raise IndexError(f"rows {start} to {stop} of a sequence of {self.alloc.lens[b]}")
+        return N._ops().kv_read(self._pages(), b, start, stop - start, self.dtype == torch.bfloat16)
 
     # ---- for tests and debugging -------------------------------------------------------------------
     def gather(self, b: int):
         """Contiguous (kv_heads, len, head_dim) copies of sequence ``b``'s keys and values (torch indexing)."""
+        if self.store is not None:
+            return self.read(b)
         n = self.alloc.lens[b]
         pages = torch.tensor(self.alloc.table[b], dtype=torch.long, device=self.device)
         k = self.k_pages[pages].permute(1, 0, 2, 3).reshape(self.kv_heads, -1, self.head_dim)[:, :n]
