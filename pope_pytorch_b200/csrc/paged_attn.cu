@@ -107,7 +107,10 @@ bool attn_paged_supported(const PopePagedAttnArgs& a) {
   return a.cache.kv.page_size % 64 == 0;
 }
 
-size_t attn_paged_workspace(const PopePagedAttnArgs&) { return 0; }
+// Rows that share a key head, up to which one pass over the keys per block of 32 is taken
+static bool few_rows(const PopeShape& s) { return (int64_t)s.Nq * (s.H / s.Hk) <= 64; }
+
+size_t attn_paged_workspace(const PopePagedAttnArgs& a) { return few_rows(a.shape) ? paged_rows_workspace(a) : 0; }
 
 template <typename T, int STORE, int D> static cudaError_t paged_attn_t(const PopePagedAttnArgs& a, cudaStream_t st) {
   PagedAttnP p;
@@ -130,6 +133,7 @@ template <typename T> static cudaError_t paged_attn_s(const PopePagedAttnArgs& a
   }
 }
 cudaError_t attn_paged(const PopePagedAttnArgs& a, cudaStream_t st) {
+  if (few_rows(a.shape)) return paged_rows(a, st);
   return a.shape.dtype == POPE_BF16 ? paged_attn_s<__nv_bfloat16>(a, st) : paged_attn_s<__half>(a, st);
 }
 

@@ -100,6 +100,11 @@ bool make_wide_tmap(CUtensorMap* out, const void* base, bool is_bf16, int d, int
                  batch, sn, sh, sb, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// rows of one-byte codes cut into boxes of 128 bytes x box_rows rows, 128-byte swizzled
+bool make_code_tmap(CUtensorMap* out, const void* base, int d, int rows, int heads, int batch, int64_t sn, int64_t sh, int64_t sb, int box_rows) {
+  return tmap_4d(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, d, rows, heads, batch, sn, sh, sb, 128, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 // An operand image ([tile][chunk][64 rows x 16 B]) seen as (1 KB run, tile, chunk): a box of (1 KB, 2 tiles, all chunks)
 // lands in shared memory as [chunk][128 rows][16 B], i.e. a resident 128-row operand arrives by ONE copy.
 bool make_image_tmap(CUtensorMap* out, const void* img, int64_t ntiles, int chunks) {
