@@ -2,27 +2,30 @@
 // tokens, the last short piece of a prompt.
 //
 // The query rows that share a key head -- the newest tokens of a sequence times the heads of the group -- are packed into blocks of
-// 16 or 32 (row = token * group + head).  A call then is one pass over K and V, each key transformed once for all rows of the block:
+// 8, 16 or 32 (row = token * group + head).  A call then is one pass over K and V, each key transformed once for all rows of the block:
 //
-//   loader warp    : tiles of 64 keys (K rows, V rows, fp16 cos / sin rows, row scales) through a ring of shared-memory stages, by
-//                    tensor-map copies in 128-byte-swizzled rows; the page of a tile comes from the page table
-//   8 worker warps : two groups of four take turns with the tiles, a warp owns 16 keys of a tile.  K' never exists in memory: a lane
-//                    reads 16 bytes of a key and turns them into the B fragments of mma.sync m16n8k16 in its registers.  (The order of the
-//                    features inside a product is free as long as Q' uses the same one, so a lane's fragment is made of the
-//                    features that sit next to each other in its key.)  The scores' accumulator fragments are, as they are, the A
-//                    fragments of P V.  Every warp keeps its own running (max, sum, output); they meet at the end.
+//   copies  : tiles of 32 keys (K rows and V rows of one or two key heads, fp16 cos / sin rows, row scales) by tensor-map copies in
+//             128-byte-swizzled rows; the page of a tile comes from the page table.  There is no loading warp: of the warps that share a
+//             tile the last one to be done with it issues the copies that refill its stage.
+//   compute : pairs of warps take the tiles of a key head in turn, a warp owns 16 keys of a tile.  K' never exists in memory: a lane
+//             reads 16 bytes of a key and turns them into the A fragments of mma.sync m16n8k16 in its registers, S^T = K' Q'^T.  (The
+//             order of the features inside a product is free as long as Q' uses the same one, so a lane's fragment is made of
+//             features that sit next to each other in its key.)  A transposition inside the warp turns the probabilities into the B
+//             fragment of O^T = V^T P^T.  Every warp keeps its own running (max, sum, output); they meet at the end.
 //
 // The tensor cores are used through mma.sync because the operand is made in registers: writing it to shared memory for tcgen05 would
-// cost as much as the products of a 16-row block, which are a small part of the time either way.
+// cost as much as the products of a few rows, which are a small part of the time either way.
 //
 // With q' = (a_q cos fq, a_q sin fq), k' = (a_k cos(fk + b), a_k sin(fk + b)) a rotated feature adds a_k (Qc cos fk + Qs sin fk),
 // Qc = a_q cos(fq - b), Qs = a_q sin(fq - b): the head's bias sits in the query.
 //
-// 8-bit codes: K' and Q' are fp16 whatever the compute type (11 bits instead of 8).  Rows beyond 2^15 are brought down by a factor that
-// returns with the scores.  V enters the products as its codes, exact in fp16, and its scale s_j goes into the probability:
-// p_j s_j = 2^(score + log2 s_j - m), with m the running maximum of that sum, so that it stays in fp16's range whatever the scales
-// are, while the softmax's own sum adds 2^(score - m) in fp32.
+// 8-bit codes: K' and Q' are fp16 whatever the compute type (11 bits instead of 8).  Plain features enter their products as codes,
+// exact in fp16, and the key's scale is applied to the sum.  Magnitudes of rows beyond 2^15 are brought down by a factor that returns
+// with the scores.  V enters as its codes too, and its scale s_j goes into the probability: p_j s_j = 2^(score + log2 s_j - m), with m the
+// running maximum of that sum, so that it stays in fp16's range whatever the scales are, while the softmax's own sum adds
+// 2^(score - m) in fp32.
 #include <algorithm>
+#include <type_traits>
 
 #include "kernels.h"
 #include "paged.cuh"
@@ -30,8 +33,8 @@
 namespace pope {
 
 struct PagedRowsP {
-  int B, H, Hk, G, Nq, Nk, r, nsplit, nstages, blocks;   // G: query heads per key head; blocks: row blocks per (sequence, key head)
-  int page_size, max_pages, num_pages;
+  int H, Hk, G, Nq, Nk, r, nsplit, stages, blocks, hb;   // G: query heads per key head; stages: of one tile ring; blocks: row blocks per
+  int page_size, max_pages, num_pages, npg_smem;         // (sequence, key head); hb: key heads that a CTA takes
   float scale_log2;
   const int32_t *page_table, *seq_lens, *counts;
   const float *k_scales, *v_scales;
@@ -41,11 +44,14 @@ struct PagedRowsP {
   void* out;
   Strides sq, so;
   float* lse;
-  float *part_o, *part_ml;   // [unit][split][row][D] and [unit][split][row][max (log2 units), sum]
+  float *part_o, *part_ml;   // [unit][split][head][row][D] and [unit][split][head][row][max (log2 units), sum]
   unsigned int *done, *status;
 };
 
-constexpr int PR_TILE = 64, PR_NW = 8, PR_MAX_SPLIT = 64, PR_BLOCK = PR_TILE * 128;   // PR_BLOCK: 64 rows of 128 bytes
+constexpr int PR_TILE = 32;              // keys of a tile
+constexpr int PR_WPT = PR_TILE / 16;     // warps that share a tile of one key head
+constexpr int PR_MAX_SPLIT = 64;
+constexpr int PR_BLOCK = PR_TILE * 128;  // bytes of 128-byte rows of a tile
 
 template <typename TM> __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
 template <> __device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -68,8 +74,54 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   const __half2 v = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+// the transpose of an 8 x 8 matrix of 16-bit values, one row per four lanes
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
 // softplus(x) / ln 2 = max(y, 0) + log2(1 + 2^-|y|), y = x log2(e)
-__device__ __forceinline__ float softplus_log2(float y) { return fmaxf(y, 0.f) + lg2_approx(1.f + ex2_approx(-fabsf(y))); }
+__device__ __forceinline__ float2 softplus_log2(float2 y) {
+  const float2 u = add2(make_float2(ex2_approx(-fabsf(y.x)), ex2_approx(-fabsf(y.y))), make_float2(1.f, 1.f));
+  return add2(make_float2(lg2_approx(u.x), lg2_approx(u.y)), make_float2(fmaxf(y.x, 0.f), fmaxf(y.y, 0.f)));
+}
+
+// Codes of a word -> fp16 pairs (0, 1), (2, 3)
+template <int STORE> __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t (&h)[2]) {
+  if constexpr (STORE == POPE_STORE_INT8) {
+    // 1024 + (code + 128), exact, minus 1152
+    w ^= 0x80808080u;
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));
+    const uint32_t m[2] = {__byte_perm(w, 0x64646464u, 0x4140), __byte_perm(w, 0x64646464u, 0x4342)};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&m[i]), off);
+      h[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const __half2_raw v = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * i)), __NV_E4M3);
+      h[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+  }
+}
+// Codes of a word times c.  int8: the byte u = code + 128 in the mantissa of 2^15 makes 2^15 + u; (2^15 + u) c - (2^15 + 128) c is one fused
+// operation, off by the rounding of the constant (2^-9 of a code step).
+template <int STORE> __device__ __forceinline__ void codes_times(uint32_t w, float c, float2 (&x)[2]) {
+  if constexpr (STORE == POPE_STORE_INT8) {
+    w ^= 0x80808080u;
+    const float2 cc = make_float2(c, c), off = make_float2(-32896.f * c, -32896.f * c);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      x[i] = fma2(make_float2(__uint_as_float(__byte_perm(w, 0x47000000u, 0x7404 + (i << 5))), __uint_as_float(__byte_perm(w, 0x47000000u, 0x7414 + (i << 5)))), cc, off);
+  } else {
+    uint32_t h[2];
+    codes_to_half<STORE>(w, h);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) x[i] = mul2(unpack2<__half>(h[i]), make_float2(c, c));
+  }
+}
 
 // Four codes of each of two keys, first features first -> fp16 pairs (key 0, key 1) of the four features
 template <int STORE> __device__ __forceinline__ void code_pairs(uint32_t a, uint32_t b, uint32_t (&h)[4]) {
@@ -97,43 +149,48 @@ template <int STORE> __device__ __forceinline__ void code_pairs(uint32_t a, uint
 
 constexpr float PR_BIG = 32768.f;   // magnitudes of fp16 operands stay below twice this
 
-template <typename T, int STORE, int D, int MT>
-__global__ void __launch_bounds__(32 * (PR_NW + 1), 1)
+// RQ: groups of eight query rows in a block (1, 2, 4); NW: warps
+template <typename T, int STORE, int D, int RQ, int NW>
+__global__ void __launch_bounds__(32 * NW, 1)
     paged_rows_kernel(PagedRowsP p, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                       const __grid_constant__ CUtensorMap tmap_t) {
   constexpr bool Q8 = STORE != POPE_STORE_16;
   using TM = std::conditional_t<Q8, __half, T>;            // operand type of the products
   constexpr bool HALF = std::is_same_v<TM, __half>;
-  constexpr int RB = 16 * MT;
+  constexpr bool LN2_IN_Q = Q8 || !HALF;                   // the keys' magnitudes come in units of ln 2 (fp16 keeps 16-bit keys in its range)
+  constexpr int RB = 8 * RQ;
   constexpr int VL = Q8 ? 16 : 8;                          // features in a lane's 16 bytes of a key
   constexpr int FPI = 4 * VL;                              // features of a key that its four lanes read together
   constexpr int NI = (D + FPI - 1) / FPI, DP = NI * FPI;
   constexpr int NH = VL / 8;
   constexpr int KBLK = (D * (Q8 ? 1 : 2) + 127) / 128;     // 128-byte blocks of a row
   constexpr int EPB = Q8 ? 128 : 64;                       // elements of one
-  constexpr int NT = D / 8;                                // output column tiles
+  constexpr int NT = D / 16;                               // output feature tiles
   constexpr int FL = D / 8;                                // 8-bit V: neighbouring features of a lane
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  const int r = p.r, tblk = (r + 63) / 64, RP = (r + FPI - 1) / FPI * FPI;
-  const int stage_bytes = (2 * KBLK + 2 * tblk) * PR_BLOCK + (Q8 ? 1024 : 0);
+  const int r = p.r, tblk = (r + 63) / 64, RP = (r + FPI - 1) / FPI * FPI, hb = p.hb;
+  const int rings = NW / (PR_WPT * hb);                                // tiles in work at a time, a ring of stages for each
+  const int head_bytes = 2 * KBLK * PR_BLOCK, trig_at = hb * head_bytes, scale_at = trig_at + 2 * tblk * PR_BLOCK;
+  const int stage_bytes = scale_at + (Q8 ? 1024 : 0);                 // [head][K blocks, V blocks][cos][sin][head][k scales, v scales]
   const int pitch = (DP + RP) * 2 + ((DP + RP) % 64 == 0 ? 64 : 0);   // an odd multiple of 64 bytes: eight rows x 64 bytes on distinct banks
-  const size_t ring = (size_t)p.nstages * stage_bytes, red_bytes = (size_t)PR_NW * RB * D * 4;
-  uint8_t* qsm = smem + (ring > red_bytes ? ring : red_bytes);        // Q': [RB] rows of (cos or plain features, sin features)
-  float* red_ml = reinterpret_cast<float*>(qsm + RB * pitch);         // [PR_NW][RB][2]
-  float* row_scale = red_ml + PR_NW * RB * 2;                         // [RB] what was taken off a row of Q'
-  int* row_pos = reinterpret_cast<int*>(row_scale + RB);              // [RB] position, -1 = no row
-  float* bias_cs = reinterpret_cast<float*>(row_pos + RB);            // [2][r]
-  uint64_t* full = reinterpret_cast<uint64_t*>(bias_cs + 2 * r);
-  uint64_t* empty = full + p.nstages;
-  unsigned int* last_s = reinterpret_cast<unsigned int*>(empty + p.nstages);
+  const size_t ring = (size_t)rings * p.stages * stage_bytes, red_bytes = (size_t)NW * RB * D * 4;
+  uint8_t* qsm = smem + (ring > red_bytes ? ring : red_bytes);        // Q': [hb][RB] rows of (cos or plain features, sin features)
+  float* red_ml = reinterpret_cast<float*>(qsm + hb * RB * pitch);    // [NW][RB][2]
+  float* row_scale = red_ml + NW * RB * 2;                            // [hb][RB] what was taken off a row of Q'
+  int* row_pos = reinterpret_cast<int*>(row_scale + hb * RB);         // [RB] position, -1 = no row
+  float* bias_cs = reinterpret_cast<float*>(row_pos + RB);            // [hb][2][r]
+  uint64_t* full = reinterpret_cast<uint64_t*>(bias_cs + hb * 2 * r);  // [rings][stages] the tile has landed
+  unsigned int* used = reinterpret_cast<unsigned int*>(full + rings * p.stages);   // [rings][stages] warps done with it
+  unsigned int* last_s = used + rings * p.stages;
+  int* pages_s = reinterpret_cast<int*>(last_s + 1);                  // [npg_smem] pages of this CTA's key range
 
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int split = blockIdx.x % p.nsplit, u = blockIdx.x / p.nsplit;
-  const int rb = u % p.blocks, bk = u / p.blocks, hk = bk % p.Hk, b = bk / p.Hk;
+  const int rb = u % p.blocks, bk = u / p.blocks, hk0 = bk % (p.Hk / hb) * hb, b = bk / (p.Hk / hb);
   if (tid == 0) {
-    for (int s = 0; s < p.nstages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], PR_NW / 2);
+    for (int s = 0; s < rings * p.stages; ++s) mbar_init(&full[s], 1), used[s] = 0;
     mbar_init_fence();
   }
   pdl_wait();
@@ -145,64 +202,55 @@ __global__ void __launch_bounds__(32 * (PR_NW + 1), 1)
   const int kb = (int)((int64_t)tiles_all * split / p.nsplit) * PR_TILE;
   const int ke = min(kend, (int)((int64_t)tiles_all * (split + 1) / p.nsplit) * PR_TILE);
   const int T_tiles = ke > kb ? (ke - kb + PR_TILE - 1) / PR_TILE : 0;
-  __syncthreads();
-  bool failed = false;
-
-  if (w == PR_NW) {
-    // =============================== loader =====================================================
-    const uint32_t bytes = (uint32_t)(2 * KBLK + 2 * tblk) * PR_BLOCK + (Q8 ? 512 : 0);
-    int page = 0;
-    for (int jt = 0, s = 0, par = 0; jt < T_tiles; ++jt) {
-      if ((jt & 31) == 0) {   // pages of the next 32 tiles; one outside the pool is never dereferenced (clamped, status bit 1)
-        const int mine = jt + lane, lp = (kb + mine * PR_TILE) / p.page_size;
-        page = 0;
-        if (mine < T_tiles) {
-          page = lp < p.max_pages ? p.page_table[(int64_t)b * p.max_pages + lp] : -1;
-          if (page < 0 || page >= p.num_pages) page = 0, atomicOr(p.status, 2u);
-        }
-      }
-      const int pg = __shfl_sync(0xffffffffu, page, jt & 31);
-      if (lane == 0) {
-        if (jt >= p.nstages) {
-          failed = !mbar_wait(&empty[s], par ^ 1, WAIT_LIMIT);
-          if (failed) drain_copies(full, p.nstages, jt - p.nstages, jt);
-        }
-        if (!failed) {
-          const int key0 = kb + jt * PR_TILE, row = key0 % p.page_size;
-          uint8_t* st = smem + (size_t)s * stage_bytes;
-          mbar_expect_tx(&full[s], bytes);
-#pragma unroll
-          for (int c = 0; c < KBLK; ++c) tma_load_4d(st + c * PR_BLOCK, &tmap_k, &full[s], c * EPB, row, hk, pg);
-          uint8_t* tt = st + 2 * KBLK * PR_BLOCK;
-          for (int c = 0; c < tblk; ++c) {
-            tma_load_4d(tt + c * PR_BLOCK, &tmap_t, &full[s], c * 64, key0, 0, 0);
-            tma_load_4d(tt + (tblk + c) * PR_BLOCK, &tmap_t, &full[s], c * 64, key0, 1, 0);
-          }
-          if constexpr (Q8) {
-            const int64_t at = ((int64_t)pg * p.Hk + hk) * p.page_size + row;
-            uint8_t* sc = tt + 2 * tblk * PR_BLOCK;
-            bulk_load(sc, p.k_scales + at, 256, &full[s]), bulk_load(sc + 256, p.v_scales + at, 256, &full[s]);
-          }
-#pragma unroll
-          for (int c = 0; c < KBLK; ++c) tma_load_4d(st + (KBLK + c) * PR_BLOCK, &tmap_v, &full[s], c * EPB, row, hk, pg);
-        }
-      }
-      failed = __shfl_sync(0xffffffffu, (int)failed, 0) != 0;
-      if (failed) break;
-      if (++s == p.nstages) s = 0, par ^= 1;
+  // pages of [kb, ke); one outside the pool is never dereferenced (clamped, status bit 1)
+  for (int i = tid; i < p.npg_smem; i += 32 * NW) {
+    const int lp = kb / p.page_size + i;
+    int pg = 0;
+    if ((int64_t)lp * p.page_size < ke) {
+      pg = lp < p.max_pages ? p.page_table[(int64_t)b * p.max_pages + lp] : -1;
+      if (pg < 0 || pg >= p.num_pages) pg = 0, atomicOr(p.status, 2u);
     }
-    if (failed && lane == 0) atomicOr(p.status, 1u);
-    return;   // nothing below is a block-wide barrier
+    pages_s[i] = pg;
   }
+  for (int i = tid; i < hb * r; i += 32 * NW) {
+    const int h = i / r, c = i - h * r;
+    sincosf(p.bias[(hk0 + h) * p.bias_sh + c], &bias_cs[(2 * h + 1) * r + c], &bias_cs[2 * h * r + c]);
+  }
+  __syncthreads();
 
-  // =============================== workers ======================================================
-  auto worker_sync = []() { asm volatile("bar.sync 1, %0;" ::"n"(32 * PR_NW) : "memory"); };
-  for (int c = tid; c < r; c += 32 * PR_NW) sincosf(p.bias[hk * p.bias_sh + c], &bias_cs[r + c], &bias_cs[c]);
-  worker_sync();
-  for (int row = w; row < RB; row += PR_NW) {   // a warp per row of Q'
-    const int rho = rb * RB + row, i = rho / p.G, head = hk + (rho - i * p.G) * p.Hk, pos = len - cnt + i;
+  // One thread: the copies of tile jt into stage `at` (ring * stages + stage)
+  auto load_tile = [&](int jt, int at) {
+    const int key0 = kb + jt * PR_TILE, row = key0 % p.page_size, pg = pages_s[key0 / p.page_size - kb / p.page_size];
+    uint8_t* st = smem + (size_t)at * stage_bytes;
+    uint64_t* bar = &full[at];
+    mbar_expect_tx(bar, (uint32_t)(scale_at + (Q8 ? hb * 8 * PR_TILE : 0)));
+    for (int h = 0; h < hb; ++h)
+#pragma unroll
+      for (int c = 0; c < KBLK; ++c) {
+        tma_load_4d(st + h * head_bytes + c * PR_BLOCK, &tmap_k, bar, c * EPB, row, hk0 + h, pg);
+        tma_load_4d(st + h * head_bytes + (KBLK + c) * PR_BLOCK, &tmap_v, bar, c * EPB, row, hk0 + h, pg);
+      }
+    for (int c = 0; c < tblk; ++c) {
+      tma_load_4d(st + trig_at + c * PR_BLOCK, &tmap_t, bar, c * 64, key0, 0, 0);
+      tma_load_4d(st + trig_at + (tblk + c) * PR_BLOCK, &tmap_t, bar, c * 64, key0, 1, 0);
+    }
+    if constexpr (Q8) {
+      for (int h = 0; h < hb; ++h) {
+        const int64_t from = ((int64_t)pg * p.Hk + hk0 + h) * p.page_size + row;
+        uint8_t* sc = st + scale_at + h * 8 * PR_TILE;
+        bulk_load(sc, p.k_scales + from, 4 * PR_TILE, bar), bulk_load(sc + 4 * PR_TILE, p.v_scales + from, 4 * PR_TILE, bar);
+      }
+    }
+  };
+  if (tid == 0)
+    for (int jt = 0; jt < min(T_tiles, rings * p.stages); ++jt) load_tile(jt, jt % rings * p.stages + jt / rings);
+
+  for (int i = w; i < hb * RB; i += NW) {   // a warp per row of Q'
+    const int h = i / RB, row = i - h * RB;
+    const int rho = rb * RB + row, tok = rho / p.G, head = hk0 + h + (rho - tok * p.G) * p.Hk, pos = len - cnt + tok;
     const bool live = row < rows && pos >= 0;
-    const T* qrow = static_cast<const T*>(p.q) + b * p.sq.b + head * p.sq.h + (int64_t)i * p.sq.n;
+    const T* qrow = static_cast<const T*>(p.q) + b * p.sq.b + head * p.sq.h + (int64_t)tok * p.sq.n;
+    const float* bcs = bias_cs + 2 * h * r;
     float qc[DP / 32], qs[DP / 32], mx = 0.f;
 #pragma unroll
     for (int j = 0; j < DP / 32; ++j) {
@@ -211,8 +259,8 @@ __global__ void __launch_bounds__(32 * (PR_NW + 1), 1)
       if (live && c < r) {
         float sn, cs;
         sincosf(p.freqs[(int64_t)pos * p.sfn + c], &sn, &cs);
-        const float a = softplus_f(qc[j]) * (HALF ? 1.f : LN2);   // (the bf16 keys' magnitudes come in units of ln 2)
-        qc[j] = a * (cs * bias_cs[c] + sn * bias_cs[r + c]), qs[j] = a * (sn * bias_cs[c] - cs * bias_cs[r + c]);
+        const float a = softplus_f(qc[j]) * (LN2_IN_Q ? LN2 : 1.f);
+        qc[j] = a * (cs * bcs[c] + sn * bcs[r + c]), qs[j] = a * (sn * bcs[c] - cs * bcs[r + c]);
       }
       mx = fmaxf(mx, fmaxf(fabsf(qc[j]), fabsf(qs[j])));
     }
@@ -221,42 +269,31 @@ __global__ void __launch_bounds__(32 * (PR_NW + 1), 1)
       mx = warp_max(mx);
       if (mx > PR_BIG && mx < CUDART_INF_F) down = PR_BIG / mx;
     }
-    TM* dst = reinterpret_cast<TM*>(qsm + row * pitch);
+    TM* dst = reinterpret_cast<TM*>(qsm + i * pitch);
 #pragma unroll
     for (int j = 0; j < DP / 32; ++j) {
       const int c = lane + 32 * j;
       dst[c] = from_f32<TM>(qc[j] * down);
       if (c < RP) dst[DP + c] = from_f32<TM>(qs[j] * down);
     }
-    if (lane == 0) row_scale[row] = p.scale_log2 / down, row_pos[row] = live ? pos : -1;
+    if (lane == 0) {
+      row_scale[i] = p.scale_log2 / down;
+      if (h == 0) row_pos[row] = live ? pos : -1;
+    }
   }
-  worker_sync();
+  __syncthreads();
 
-  const int g = lane >> 2, t = lane & 3, sub = w & 3;
-  const uint8_t* qlane = qsm + g * pitch + t * (VL * 2);
-  constexpr bool QREG = MT == 1;
-  uint4 qreg_c[QREG ? NI : 1][NH][2], qreg_s[QREG ? NI : 1][NH][2];   // the A fragments, eight features of rows g and g + 8 each
-  if constexpr (QREG) {
+  const int g = lane >> 2, t = lane & 3, sub = w % PR_WPT, hloc = w / PR_WPT % hb, rg = w / PR_WPT / hb;
+  const uint8_t* qlane = qsm + (hloc * RB + g) * pitch + t * (VL * 2);
+  int pos_of[RQ][2];        // queries 2 t, 2 t + 1 of a group of eight
+  float sc_of[RQ][2];
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
+  for (int m = 0; m < RQ; ++m)
 #pragma unroll
-      for (int h = 0; h < NH; ++h)
+    for (int e = 0; e < 2; ++e) pos_of[m][e] = row_pos[m * 8 + 2 * t + e], sc_of[m][e] = row_scale[hloc * RB + m * 8 + 2 * t + e];
+  float m_run[RQ][2], l_run[RQ][2], o[RQ][NT][4];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint8_t* a = qlane + e * 8 * pitch + (i * FPI + h * 8) * 2;
-          qreg_c[i][h][e] = *reinterpret_cast<const uint4*>(a);
-          qreg_s[i][h][e] = i * FPI < r ? *reinterpret_cast<const uint4*>(a + DP * 2) : make_uint4(0, 0, 0, 0);
-        }
-  }
-  int pos_of[MT][2];
-  float sc_of[MT][2];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) pos_of[m][e] = row_pos[m * 16 + e * 8 + g], sc_of[m][e] = row_scale[m * 16 + e * 8 + g];
-  float m_run[MT][2], l_run[MT][2], o[MT][NT][4];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
+  for (int m = 0; m < RQ; ++m) {
     m_run[m][0] = m_run[m][1] = -CUDART_INF_F, l_run[m][0] = l_run[m][1] = 0.f;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
@@ -264,147 +301,170 @@ __global__ void __launch_bounds__(32 * (PR_NW + 1), 1)
       for (int e = 0; e < 4; ++e) o[m][n][e] = 0.f;
   }
 
-  int s = (w >> 2) % p.nstages;
+  bool failed = false;
+  int s = 0;
   uint32_t par = 0;
-  for (int jt = w >> 2; jt < T_tiles; jt += 2) {
+  for (int jt = rg; jt < T_tiles; jt += rings) {
     const int key0 = kb + jt * PR_TILE + sub * 16;   // first key of this warp
-    uint8_t* st = smem + (size_t)s * stage_bytes;
-    const uint8_t* tt = st + 2 * KBLK * PR_BLOCK;
-    const float* scl = reinterpret_cast<const float*>(tt + 2 * tblk * PR_BLOCK);
-    if (!mbar_wait(&full[s], par, WAIT_LIMIT)) {
+    const int at = rg * p.stages + s;
+    uint8_t* st = smem + (size_t)at * stage_bytes;
+    const uint8_t* tt = st + trig_at;
+    const float* scl = reinterpret_cast<const float*>(st + scale_at) + hloc * 2 * PR_TILE;
+    st += hloc * head_bytes;
+    if (!mbar_wait(&full[at], par, WAIT_LIMIT)) {
       failed = true;
       break;
     }
-    // ---- scores: two tiles of eight keys ------------------------------------------------------------
-    float sco[MT][2][4];
+    // ---- scores: keys g and g + 8 of this warp's sixteen ----------------------------------------------
+    float sco[RQ][4], plain[Q8 ? RQ : 1][4];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < RQ; ++m)
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sco[m][n][e] = 0.f;
-    float ks[2] = {1.f, 1.f}, kd[2] = {1.f, 1.f};   // 8-bit: a key's scale, and the factor that brings its operands down
+      for (int e = 0; e < 4; ++e) {
+        sco[m][e] = 0.f;
+        if constexpr (Q8) plain[m][e] = 0.f;
+      }
+    float ks[2] = {1.f, 1.f}, kd[2] = {1.f, 1.f};   // 8-bit: a key's scale, and the factor that brings its magnitudes down
+    bool big = false;
     if constexpr (Q8) {
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         ks[n] = scl[sub * 16 + n * 8 + g];
         const float top = ks[n] * kCodeTop<STORE>;
-        kd[n] = top > PR_BIG ? PR_BIG / top : 1.f;
+        if (top > PR_BIG) kd[n] = PR_BIG / top, big = true;
       }
+      big = __any_sync(0xffffffffu, big);
     }
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int ch = 4 * i + t;
-      const bool rot_i = i * FPI < r;   // (the same for all lanes)
+      const bool rot_i = i * FPI < r, all_i = (i + 1) * FPI <= r;   // any, all features of these lanes rotated (the same for all lanes)
+      uint32_t rw[2][4];
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         const int row = sub * 16 + n * 8 + g;
         const uint4 raw = *reinterpret_cast<const uint4*>(st + (ch >> 3) * PR_BLOCK + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
-        const uint32_t rw[4] = {raw.x, raw.y, raw.z, raw.w};
+        rw[n][0] = raw.x, rw[n][1] = raw.y, rw[n][2] = raw.z, rw[n][3] = raw.w;
+      }
 #pragma unroll
-        for (int h = 0; h < NH; ++h) {
-          const int f0 = ch * VL + h * 8;   // first of the lane's eight features
-          uint32_t kc[4], kn[4];            // fragments: features (f0, f0 + 1), ...
-          if (!rot_i) {
+      for (int h = 0; h < NH; ++h) {
+        const int f0 = ch * VL + h * 8;   // first of the lane's eight features
+        uint32_t kc[2][4], kn[2][4];      // fragments of both keys: features (f0, f0 + 1), ...
+        if (!rot_i) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
             if constexpr (!Q8) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) kc[e] = rw[e];
+              for (int e = 0; e < 4; ++e) kc[n][e] = rw[n][e];
             } else {
-              const float f = ks[n] * kd[n];
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                float x[4];
-                codes_to_f32<STORE>(rw[h * 2 + e], x);
-                kc[2 * e] = pack2<__half>(x[0] * f, x[1] * f), kc[2 * e + 1] = pack2<__half>(x[2] * f, x[3] * f);
+                uint32_t x[2];
+                codes_to_half<STORE>(rw[n][h * 2 + e], x);
+                kc[n][2 * e] = x[0], kc[n][2 * e + 1] = x[1];
               }
             }
-          } else {
-            const bool rot = f0 < r;
+          }
+        } else {
+          const bool rot = all_i || f0 < r;
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const int row = sub * 16 + n * 8 + g;
             const uint8_t* trow = tt + (f0 >> 6) * PR_BLOCK + row * 128 + ((((f0 >> 3) & 7) ^ (row & 7)) << 4);
-            uint4 cr = *reinterpret_cast<const uint4*>(trow);
+            const uint4 cr = *reinterpret_cast<const uint4*>(trow);
             const uint4 sr = *reinterpret_cast<const uint4*>(trow + tblk * PR_BLOCK);   // (zeros where nothing is rotated)
-            if (!rot) cr = make_uint4(0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u);
-            const uint32_t cw[4] = {cr.x, cr.y, cr.z, cr.w}, sw[4] = {sr.x, sr.y, sr.z, sr.w};
-            float x[8];
+            uint32_t cw[4] = {cr.x, cr.y, cr.z, cr.w};
+            const uint32_t sw[4] = {sr.x, sr.y, sr.z, sr.w};
+            float2 x[4];
             if constexpr (!Q8) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 v = unpack2<T>(rw[e]);
-                x[2 * e] = v.x, x[2 * e + 1] = v.y;
-              }
+              for (int e = 0; e < 4; ++e) x[e] = mul2(unpack2<T>(rw[n][e]), make_float2(LOG2E, LOG2E));
             } else {
-              codes_to_f32<STORE>(rw[h * 2], *reinterpret_cast<float(*)[4]>(x));
-              codes_to_f32<STORE>(rw[h * 2 + 1], *reinterpret_cast<float(*)[4]>(x + 4));
-            }
-            const float unit = ks[n] * LOG2E, back = HALF ? LN2 * kd[n] : 1.f, plain = ks[n] * kd[n];
+              float2 y[2];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float a = softplus_log2(x[e] * unit) * back;
-              x[e] = rot ? a : x[e] * plain;
+              for (int e = 0; e < 2; ++e) codes_times<STORE>(rw[n][h * 2 + e], ks[n] * LOG2E, y), x[2 * e] = y[0], x[2 * e + 1] = y[1];
+            }
+            if (all_i) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[e] = softplus_log2(x[e]);
+            } else {   // plain features among them: in the same units, with a cosine of one
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 a = softplus_log2(x[e]);
+                const float f = LN2_IN_Q ? LN2 : 1.f;
+                x[e] = rot ? a : mul2(x[e], make_float2(f, f));
+                if (!rot) cw[e] = 0x3c003c00u;
+              }
+            }
+            if constexpr (!LN2_IN_Q) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[e] = mul2(x[e], make_float2(LN2, LN2));
+            }
+            if (Q8 && big) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[e] = mul2(x[e], make_float2(kd[n], kd[n]));
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               if constexpr (HALF) {
-                const uint32_t a = pack2<__half>(x[2 * e], x[2 * e + 1]);
-                kc[e] = hmul2(a, cw[e]), kn[e] = hmul2(a, sw[e]);
+                const uint32_t a = pack2<__half>(x[e].x, x[e].y);
+                kc[n][e] = hmul2(a, cw[e]), kn[n][e] = hmul2(a, sw[e]);
               } else {
-                const float2 c = unpack2<__half>(cw[e]), v = unpack2<__half>(sw[e]);
-                kc[e] = pack2<TM>(x[2 * e] * c.x, x[2 * e + 1] * c.y), kn[e] = pack2<TM>(x[2 * e] * v.x, x[2 * e + 1] * v.y);
+                const float2 c = mul2(x[e], unpack2<__half>(cw[e])), v = mul2(x[e], unpack2<__half>(sw[e]));
+                kc[n][e] = pack2<TM>(c.x, c.y), kn[n][e] = pack2<TM>(v.x, v.y);
               }
             }
           }
+        }
 #pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            uint4 a0, a1;
-            const uint8_t* qa = qlane + m * 16 * pitch + (i * FPI + h * 8) * 2;
-            if constexpr (QREG) a0 = qreg_c[i][h][0], a1 = qreg_c[i][h][1];
-            else a0 = *reinterpret_cast<const uint4*>(qa), a1 = *reinterpret_cast<const uint4*>(qa + 8 * pitch);
-            mma16816<TM>(sco[m][n], a0.x, a1.x, a0.y, a1.y, kc[0], kc[1]);
-            mma16816<TM>(sco[m][n], a0.z, a1.z, a0.w, a1.w, kc[2], kc[3]);
-            if (rot_i) {
-              if constexpr (QREG) a0 = qreg_s[i][h][0], a1 = qreg_s[i][h][1];
-              else a0 = *reinterpret_cast<const uint4*>(qa + DP * 2), a1 = *reinterpret_cast<const uint4*>(qa + DP * 2 + 8 * pitch);
-              mma16816<TM>(sco[m][n], a0.x, a1.x, a0.y, a1.y, kn[0], kn[1]);
-              mma16816<TM>(sco[m][n], a0.z, a1.z, a0.w, a1.w, kn[2], kn[3]);
-            }
+        for (int m = 0; m < RQ; ++m) {
+          const uint8_t* qa = qlane + m * 8 * pitch + (i * FPI + h * 8) * 2;
+          const uint4 qc = *reinterpret_cast<const uint4*>(qa);
+          if (rot_i) {
+            const uint4 qs = *reinterpret_cast<const uint4*>(qa + DP * 2);
+            mma16816<TM>(sco[m], kc[0][0], kc[1][0], kc[0][1], kc[1][1], qc.x, qc.y);
+            mma16816<TM>(sco[m], kc[0][2], kc[1][2], kc[0][3], kc[1][3], qc.z, qc.w);
+            mma16816<TM>(sco[m], kn[0][0], kn[1][0], kn[0][1], kn[1][1], qs.x, qs.y);
+            mma16816<TM>(sco[m], kn[0][2], kn[1][2], kn[0][3], kn[1][3], qs.z, qs.w);
+          } else {
+            float(&acc)[4] = Q8 ? plain[Q8 ? m : 0] : sco[m];
+            mma16816<TM>(acc, kc[0][0], kc[1][0], kc[0][1], kc[1][1], qc.x, qc.y);
+            mma16816<TM>(acc, kc[0][2], kc[1][2], kc[0][3], kc[1][3], qc.z, qc.w);
           }
         }
       }
     }
-    // ---- softmax: rows g and g + 8, keys 2 t, 2 t + 1 of both tiles -----------------------------------
-    float kup[2][2], vs[2][2], lvs[2][2];
+    // ---- softmax: keys g, g + 8; queries 2 t, 2 t + 1 -------------------------------------------------
+    float vs[2] = {1.f, 1.f}, lvs[2] = {0.f, 0.f};
     if constexpr (Q8) {
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        const float2 k2 = *reinterpret_cast<const float2*>(scl + sub * 16 + n * 8 + 2 * t);
-        const float2 v2 = *reinterpret_cast<const float2*>(scl + 64 + sub * 16 + n * 8 + 2 * t);
-        kup[n][0] = fmaxf(1.f, k2.x * (kCodeTop<STORE> / PR_BIG)), kup[n][1] = fmaxf(1.f, k2.y * (kCodeTop<STORE> / PR_BIG));
-        vs[n][0] = v2.x, vs[n][1] = v2.y;
-        lvs[n][0] = fmaxf(lg2_approx(v2.x), -100.f), lvs[n][1] = fmaxf(lg2_approx(v2.y), -100.f);
+        vs[n] = scl[PR_TILE + sub * 16 + n * 8 + g], lvs[n] = fmaxf(lg2_approx(vs[n]), -100.f);
+        kd[n] = big ? fmaxf(1.f, ks[n] * (kCodeTop<STORE> / PR_BIG)) : 1.f;   // (from here on what returns with the scores)
       }
     }
     const bool clean = key0 + 16 <= min(ke, first_pos + 1);   // every row sees every key of this warp
-    uint32_t pa[MT][4];
+    uint32_t pb[RQ][2];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
+    for (int m = 0; m < RQ; ++m) {
       float mx[2] = {-CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = sco[m][n][e] * sc_of[m][e >> 1];
-          if constexpr (Q8) v *= kup[n][e & 1];
-          if (!clean && key0 + n * 8 + 2 * t + (e & 1) > min(ke - 1, pos_of[m][e >> 1])) v = -CUDART_INF_F;
-          sco[m][n][e] = v;
-          mx[e >> 1] = fmaxf(mx[e >> 1], Q8 ? v + lvs[n][e & 1] : v);
-        }
+      for (int e = 0; e < 4; ++e) {
+        const int n = e >> 1;
+        float v = sco[m][e];
+        if constexpr (Q8) v = fmaf(plain[m][e], ks[n], v * kd[n]);
+        v *= sc_of[m][e & 1];
+        if (!clean && key0 + n * 8 + g > min(ke - 1, pos_of[m][e & 1])) v = -CUDART_INF_F;
+        sco[m][e] = v;
+        mx[e & 1] = fmaxf(mx[e & 1], Q8 ? v + lvs[n] : v);
+      }
       // the maximum may lag by 2^8: most tiles then need neither a reduction nor a rescale
       if (__any_sync(0xffffffffu, mx[0] > m_run[m][0] + 8.f || mx[1] > m_run[m][1] + 8.f)) {
         float alpha[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-          mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
+#pragma unroll
+          for (int off = 4; off < 32; off *= 2) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], off));
           mx[e] = fmaxf(mx[e], m_run[m][e]);
           alpha[e] = mx[e] == -CUDART_INF_F ? 1.f : ex2_approx(m_run[m][e] - mx[e]);
           m_run[m][e] = mx[e], l_run[m][e] *= alpha[e];
@@ -412,23 +472,20 @@ __global__ void __launch_bounds__(32 * (PR_NW + 1), 1)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[m][n][e] *= alpha[e >> 1];
+          for (int e = 0; e < 4; ++e) o[m][n][e] *= alpha[e & 1];
       }
-      float pr[2][4];
+      float pr[4];
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float mu = m_run[m][e >> 1];
-          const float x = ex2_approx(sco[m][n][e] - (mu == -CUDART_INF_F ? 0.f : mu));
-          l_run[m][e >> 1] += x;
-          pr[n][e] = x;
-          if constexpr (Q8) pr[n][e] = sco[m][n][e] == -CUDART_INF_F ? 0.f : x * vs[n][e & 1];   // (unused rows may have any scale)
-        }
-      pa[m][0] = pack2<TM>(pr[0][0], pr[0][1]), pa[m][1] = pack2<TM>(pr[0][2], pr[0][3]);
-      pa[m][2] = pack2<TM>(pr[1][0], pr[1][1]), pa[m][3] = pack2<TM>(pr[1][2], pr[1][3]);
+      for (int e = 0; e < 4; ++e) {
+        const float mu = m_run[m][e & 1];
+        const float x = ex2_approx(sco[m][e] - (mu == -CUDART_INF_F ? 0.f : mu));
+        l_run[m][e & 1] += x;
+        pr[e] = x;
+        if constexpr (Q8) pr[e] = sco[m][e] == -CUDART_INF_F ? 0.f : x * vs[e >> 1];   // (unused rows may have any scale)
+      }
+      pb[m][0] = movmatrix_trans(pack2<TM>(pr[0], pr[1])), pb[m][1] = movmatrix_trans(pack2<TM>(pr[2], pr[3]));
     }
-    // ---- O += P V --------------------------------------------------------------------------------------
+    // ---- O^T += V^T P^T ---------------------------------------------------------------------------------
     uint8_t* vt = st + KBLK * PR_BLOCK;
     if constexpr (!Q8) {
       if (key0 + 16 > ke) {   // rows behind the last key may hold anything, and 0 * NaN is NaN
@@ -437,17 +494,14 @@ __global__ void __launch_bounds__(32 * (PR_NW + 1), 1)
           *reinterpret_cast<uint4*>(vt + (i / 8 / dead) * PR_BLOCK + (sub * 16 + 16 - dead + i / 8 % dead) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
         __syncwarp();
       }
-      const int row = sub * 16 + (lane & 15);
+      const int row = sub * 16 + (lane & 7) + ((lane >> 4) << 3);
 #pragma unroll
-      for (int n = 0; n < NT; n += 2) {
-        uint32_t bf[4];
-        const int ch = n + (lane >> 4);
-        ldmatrix_x4_trans(bf, smem_u32(vt + (ch >> 3) * PR_BLOCK + row * 128 + (((ch & 7) ^ (row & 7)) << 4)));
+      for (int n = 0; n < NT; ++n) {
+        uint32_t af[4];   // features 16 n + g and + 8 of keys 2 t, 2 t + 1, then of keys 2 t + 8, 2 t + 9
+        const int ch = 2 * n + ((lane >> 3) & 1);
+        ldmatrix_x4_trans(af, smem_u32(vt + (ch >> 3) * PR_BLOCK + row * 128 + (((ch & 7) ^ (row & 7)) << 4)));
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          mma16816<TM>(o[m][n], pa[m][0], pa[m][1], pa[m][2], pa[m][3], bf[0], bf[1]);
-          mma16816<TM>(o[m][n + 1], pa[m][0], pa[m][1], pa[m][2], pa[m][3], bf[2], bf[3]);
-        }
+        for (int m = 0; m < RQ; ++m) mma16816<TM>(o[m][n], af[0], af[1], af[2], af[3], pb[m][0], pb[m][1]);
       }
     } else {
       uint32_t vw[4][FL / 4];   // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9: features FL g ...
@@ -474,86 +528,100 @@ __global__ void __launch_bounds__(32 * (PR_NW + 1), 1)
         uint32_t lo[4], hi[4];
         code_pairs<STORE>(vw[0][c], vw[1][c], lo), code_pairs<STORE>(vw[2][c], vw[3][c], hi);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
-          for (int m = 0; m < MT; ++m) mma16816<TM>(o[m][4 * c + e], pa[m][0], pa[m][1], pa[m][2], pa[m][3], lo[e], hi[e]);
+          for (int m = 0; m < RQ; ++m) mma16816<TM>(o[m][2 * c + e], lo[2 * e], lo[2 * e + 1], hi[2 * e], hi[2 * e + 1], pb[m][0], pb[m][1]);
       }
     }
-    fence_async_smem();   // the tile has been read: the loader's next copy may write over it
+    // The tile has been read: the last of its warps refills the stage (each fences its reads before it counts itself).
+    fence_async_smem();
     __syncwarp();
-    if (lane == 0) mbar_arrive(&empty[s]);
-    if ((s += 2) >= p.nstages) s -= p.nstages, par ^= 1;
+    if (lane == 0) {
+      __threadfence_block();
+      const unsigned int n = atomicAdd(&used[at], 1u) + 1u;
+      __threadfence_block();
+      const int next = jt + rings * p.stages;
+      if (n % (unsigned)(PR_WPT * hb) == 0u && next < T_tiles) fence_async_smem(), load_tile(next, at);
+    }
+    if (++s == p.stages) s = 0, par ^= 1;
   }
-  if (failed && lane == 0) atomicOr(p.status, 1u);
+  if (failed) {   // (no copy of this ring is left in flight behind the CTA)
+    if (lane == 0) {
+      atomicOr(p.status, 1u);
+      for (int i = 0; i < p.stages; ++i) mbar_wait(&full[rg * p.stages + i], i < s ? par ^ 1 : par, 1u << 12);
+    }
+    __syncwarp();
+  }
 
   // ---- the warps' results meet ---------------------------------------------------------------------
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int m = 0; m < RQ; ++m)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      l_run[m][e] += __shfl_xor_sync(0xffffffffu, l_run[m][e], 1);
-      l_run[m][e] += __shfl_xor_sync(0xffffffffu, l_run[m][e], 2);
-      // (a lane's maximum is its row's: it changes for all four lanes of the row together)
-      if (t == 0) red_ml[(w * RB + m * 16 + e * 8 + g) * 2] = m_run[m][e], red_ml[(w * RB + m * 16 + e * 8 + g) * 2 + 1] = l_run[m][e];
-    }
-  worker_sync();   // every tile has been read: the ring takes the warps' outputs
-  float* red_o = reinterpret_cast<float*>(smem) + (size_t)w * RB * D;
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+      for (int off = 4; off < 32; off *= 2) l_run[m][e] += __shfl_xor_sync(0xffffffffu, l_run[m][e], off);
+      // (a lane's maximum is its row's: it changes for all lanes of the row together)
+      if (g == 0) red_ml[(w * RB + m * 8 + 2 * t + e) * 2] = m_run[m][e], red_ml[(w * RB + m * 8 + 2 * t + e) * 2 + 1] = l_run[m][e];
+    }
+  __syncthreads();   // every tile has been read: the ring takes the warps' outputs
+  float* red_o = reinterpret_cast<float*>(smem);
+#pragma unroll
+  for (int m = 0; m < RQ; ++m)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int c = Q8 ? (2 * t + (e & 1)) * FL + n : n * 8 + 2 * t + (e & 1);
-        red_o[(m * 16 + (e >> 1) * 8 + g) * D + c] = o[m][n][e];
+        const int c = Q8 ? g * FL + 2 * n + (e >> 1) : n * 16 + g + (e >> 1) * 8;
+        red_o[(w * RB + m * 8 + 2 * t + (e & 1)) * D + c] = o[m][n][e];
       }
-  worker_sync();
-  auto write_out = [&](int row, int c, float x) {
-    const int rho = rb * RB + row, i = rho / p.G, head = hk + (rho - i * p.G) * p.Hk;
-    static_cast<T*>(p.out)[b * p.so.b + head * p.so.h + (int64_t)i * p.so.n + c] = from_f32<T>(x);
+  __syncthreads();
+  auto write_out = [&](int h, int row, int c, float x) {
+    const int rho = rb * RB + row, tok = rho / p.G, head = hk0 + h + (rho - tok * p.G) * p.Hk;
+    static_cast<T*>(p.out)[b * p.so.b + head * p.so.h + (int64_t)tok * p.so.n + c] = from_f32<T>(x);
   };
-  auto write_lse = [&](int row, float M, float L) {
-    const int rho = rb * RB + row, i = rho / p.G, head = hk + (rho - i * p.G) * p.Hk;
-    if (p.lse) p.lse[((int64_t)b * p.H + head) * p.Nq + i] = L != 0.f ? M * LN2 + logf(L) : -CUDART_INF_F;
+  auto write_lse = [&](int h, int row, float M, float L) {
+    const int rho = rb * RB + row, tok = rho / p.G, head = hk0 + h + (rho - tok * p.G) * p.Hk;
+    if (p.lse) p.lse[((int64_t)b * p.H + head) * p.Nq + tok] = L != 0.f ? M * LN2 + logf(L) : -CUDART_INF_F;
   };
   const int out_rows = min(RB, p.Nq * p.G - rb * RB);   // (padding is written too)
-  const int64_t slot = ((int64_t)u * p.nsplit + split) * RB;
-  for (int i = tid; i < out_rows * D; i += 32 * PR_NW) {
-    const int row = i / D, c = i - row * D;
+  const int64_t slot = ((int64_t)u * p.nsplit + split) * hb * RB;
+  for (int i = tid; i < hb * out_rows * D; i += 32 * NW) {
+    const int c = i % D, hr = i / D, h = hr / out_rows, row = hr - h * out_rows;
     float M = -CUDART_INF_F, L = 0.f, acc = 0.f;
-#pragma unroll
-    for (int ww = 0; ww < PR_NW; ++ww) M = fmaxf(M, red_ml[(ww * RB + row) * 2]);
+    auto warp_of = [&](int k) { return ((k / PR_WPT) * hb + h) * PR_WPT + k % PR_WPT; };   // warp k of this head
+    for (int k = 0; k < NW / hb; ++k) M = fmaxf(M, red_ml[(warp_of(k) * RB + row) * 2]);
     const float mu = M == -CUDART_INF_F ? 0.f : M;
-#pragma unroll
-    for (int ww = 0; ww < PR_NW; ++ww) {
-      const float f = ex2_approx(red_ml[(ww * RB + row) * 2] - mu);   // 0 for a warp without visible keys
-      L = fmaf(red_ml[(ww * RB + row) * 2 + 1], f, L), acc = fmaf(reinterpret_cast<const float*>(smem)[(size_t)(ww * RB + row) * D + c], f, acc);
+    for (int k = 0; k < NW / hb; ++k) {
+      const int at = warp_of(k) * RB + row;
+      const float f = ex2_approx(red_ml[at * 2] - mu);   // 0 for a warp without visible keys
+      L = fmaf(red_ml[at * 2 + 1], f, L), acc = fmaf(red_o[(size_t)at * D + c], f, acc);
     }
     if (row_pos[row] < 0) M = -CUDART_INF_F, L = acc = 0.f;   // (where every query sees every key the other rows of the block were not told apart)
     if (p.nsplit == 1) {
-      write_out(row, c, L != 0.f ? acc / L : 0.f);
-      if (c == 0) write_lse(row, M, L);
+      write_out(h, row, c, L != 0.f ? acc / L : 0.f);
+      if (c == 0) write_lse(h, row, M, L);
     } else {
-      p.part_o[(slot + row) * D + c] = acc;
-      if (c == 0) p.part_ml[(slot + row) * 2] = M, p.part_ml[(slot + row) * 2 + 1] = L;
+      p.part_o[(slot + h * RB + row) * D + c] = acc;
+      if (c == 0) p.part_ml[(slot + h * RB + row) * 2] = M, p.part_ml[(slot + h * RB + row) * 2 + 1] = L;
     }
   }
   if (p.nsplit == 1) return;
   // The CTA that finishes last merges the splits of its unit.
   __threadfence();
-  worker_sync();
+  __syncthreads();
   if (tid == 0) *last_s = atomicAdd(p.done + u, 1u) == (unsigned)p.nsplit - 1u;
-  worker_sync();
+  __syncthreads();
   if (!*last_s) return;
   __threadfence();
-  float* wgt = reinterpret_cast<float*>(smem);   // [RB][nsplit] weights of the splits
-  const int64_t slot0 = (int64_t)u * p.nsplit * RB;
-  for (int row = w; row < out_rows; row += PR_NW) {
+  float* wgt = reinterpret_cast<float*>(smem);   // [hb][RB][nsplit] weights of the splits
+  const int64_t slot0 = (int64_t)u * p.nsplit * hb * RB;
+  for (int hr = w; hr < hb * out_rows; hr += NW) {
+    const int h = hr / out_rows, row = hr - h * out_rows, at = h * RB + row;
     float m2[PR_MAX_SPLIT / 32], l2[PR_MAX_SPLIT / 32], M = -CUDART_INF_F, L = 0.f;
 #pragma unroll
     for (int i = 0; i < PR_MAX_SPLIT / 32; ++i) {
       const int sp = lane + 32 * i;
-      const float2 ml = sp < p.nsplit ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + (slot0 + (int64_t)sp * RB + row) * 2))
+      const float2 ml = sp < p.nsplit ? __ldcg(reinterpret_cast<const float2*>(p.part_ml + (slot0 + (int64_t)sp * hb * RB + at) * 2))
                                       : make_float2(-CUDART_INF_F, 0.f);
       m2[i] = ml.x, l2[i] = ml.y, M = fmaxf(M, ml.x);
     }
@@ -567,34 +635,41 @@ __global__ void __launch_bounds__(32 * (PR_NW + 1), 1)
     L = warp_sum(L);
 #pragma unroll
     for (int i = 0; i < PR_MAX_SPLIT / 32; ++i)
-      if (lane + 32 * i < p.nsplit) wgt[row * p.nsplit + lane + 32 * i] = m2[i];
-    if (lane == 0) red_ml[row] = L, write_lse(row, M, L);
+      if (lane + 32 * i < p.nsplit) wgt[at * p.nsplit + lane + 32 * i] = m2[i];
+    if (lane == 0) red_ml[at] = L, write_lse(h, row, M, L);
   }
-  worker_sync();
-  for (int i = tid; i < out_rows * D; i += 32 * PR_NW) {
-    const int row = i / D, c = i - row * D;
+  __syncthreads();
+  for (int i = tid; i < hb * out_rows * D; i += 32 * NW) {
+    const int c = i % D, hr = i / D, h = hr / out_rows, row = hr - h * out_rows, at = h * RB + row;
     float acc = 0.f;
 #pragma unroll 8
-    for (int sp = 0; sp < p.nsplit; ++sp) acc = fmaf(wgt[row * p.nsplit + sp], __ldcg(p.part_o + (slot0 + (int64_t)sp * RB + row) * D + c), acc);
-    write_out(row, c, red_ml[row] != 0.f ? acc / red_ml[row] : 0.f);
+    for (int sp = 0; sp < p.nsplit; ++sp) acc = fmaf(wgt[at * p.nsplit + sp], __ldcg(p.part_o + (slot0 + (int64_t)sp * hb * RB + at) * D + c), acc);
+    write_out(h, row, c, red_ml[at] != 0.f ? acc / red_ml[at] : 0.f);
   }
 }
 
 // ---- host side ---------------------------------------------------------------------------------------
-static int rows_mt(const PopeShape& s) { return (int64_t)s.Nq * (s.H / s.Hk) > 16 ? 2 : 1; }
+static int rows_rq(const PopeShape& s) {   // groups of eight rows in a block
+  const int64_t rows = (int64_t)s.Nq * (s.H / s.Hk);
+  return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+}
 static int rows_blocks(const PopeShape& s) {
   const int64_t rows = (int64_t)s.Nq * (s.H / s.Hk);
-  return (int)((rows + 16 * rows_mt(s) - 1) / (16 * rows_mt(s)));
+  return (int)((rows + 8 * rows_rq(s) - 1) / (8 * rows_rq(s)));
 }
+// warps of a CTA: as many as the registers of their outputs (32 per group of eight rows) allow
+constexpr int rows_nw(bool q8, int rq) { return rq == 4 ? 8 : q8 ? 16 : 12; }
+// Key heads of a CTA: two share the copies of the cosines and sines, which at 8 bits are as many bytes as K and V or twice that.
+static int rows_hb(const PopeShape& s, int store) { return store != POPE_STORE_16 && s.Hk % 2 == 0 ? 2 : 1; }
 
-// Key ranges per unit: whole waves of one CTA per SM times a CTA's tiles plus what it costs beside them (about four tiles' time).
-static int rows_split(const PopeShape& s) {
+// Key ranges per unit: whole waves of one CTA per SM times a CTA's tiles plus what it costs beside them.
+static int rows_split(const PopeShape& s, int store) {
   const int tiles = (s.Nk + PR_TILE - 1) / PR_TILE;
-  const int64_t units = (int64_t)s.B * s.Hk * rows_blocks(s);
+  const int64_t units = (int64_t)s.B * s.Hk / rows_hb(s, store) * rows_blocks(s);
   int best = 1;
   int64_t best_cost = INT64_MAX;
   for (int n = 1; n <= std::min(tiles, PR_MAX_SPLIT); ++n) {
-    const int64_t cost = (units * n + 147) / 148 * ((tiles + n - 1) / n + 4);
+    const int64_t cost = (units * n + 147) / 148 * ((tiles + n - 1) / n + 8);
     if (cost < best_cost) best = n, best_cost = cost;
   }
   return best;
@@ -604,9 +679,9 @@ static int rows_split(const PopeShape& s) {
 struct RowsWs {
   size_t part_o, part_ml, table, total;
 };
-static RowsWs rows_ws(const PopeShape& s) {
+static RowsWs rows_ws(const PopeShape& s, int store) {
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
-  const size_t units = (size_t)s.B * s.Hk * rows_blocks(s), slots = units * rows_split(s) * 16 * rows_mt(s);
+  const size_t units = (size_t)s.B * s.Hk * rows_blocks(s), slots = units * rows_split(s, store) * 8 * rows_rq(s);
   RowsWs w;
   w.part_o = up(units * sizeof(unsigned int));
   w.part_ml = w.part_o + up(slots * s.d * sizeof(float));
@@ -614,18 +689,22 @@ static RowsWs rows_ws(const PopeShape& s) {
   w.total = w.table + up((size_t)s.Nk * s.r * 4);
   return w;
 }
-size_t paged_rows_workspace(const PopePagedAttnArgs& a) { return rows_ws(a.shape).total; }
+size_t paged_rows_workspace(const PopePagedAttnArgs& a) { return rows_ws(a.shape, a.cache.store).total; }
 
-template <typename T, int STORE, int D, int MT> static cudaError_t paged_rows_t(const PopePagedAttnArgs& a, cudaStream_t st) {
+template <typename T, int STORE, int D, int RQ> static cudaError_t paged_rows_t(const PopePagedAttnArgs& a, cudaStream_t st) {
   constexpr bool Q8 = STORE != POPE_STORE_16;
+  constexpr int NW = rows_nw(Q8, RQ), RB = 8 * RQ, FPI = Q8 ? 64 : 32, DP = (D + FPI - 1) / FPI * FPI, KBLK = (D * (Q8 ? 1 : 2) + 127) / 128;
   const PopeShape& s = a.shape;
   const PopePagedKV& kv = a.cache.kv;
-  const RowsWs ws = rows_ws(s);
+  const RowsWs ws = rows_ws(s, STORE);
   uint8_t* base = static_cast<uint8_t*>(a.workspace);
   __half* table = reinterpret_cast<__half*>(base + ws.table);
   PagedRowsP p = {};
-  p.B = s.B, p.H = s.H, p.Hk = s.Hk, p.G = s.H / s.Hk, p.Nq = s.Nq, p.Nk = s.Nk, p.r = s.r, p.nsplit = rows_split(s), p.blocks = rows_blocks(s);
+  p.H = s.H, p.Hk = s.Hk, p.G = s.H / s.Hk, p.Nq = s.Nq, p.Nk = s.Nk, p.r = s.r;
+  p.nsplit = rows_split(s, STORE), p.blocks = rows_blocks(s), p.hb = rows_hb(s, STORE);
   p.page_size = kv.page_size, p.max_pages = kv.max_pages_per_seq, p.num_pages = kv.num_pages;
+  const int tiles = (s.Nk + PR_TILE - 1) / PR_TILE;
+  p.npg_smem = (int)((int64_t)((tiles + p.nsplit - 1) / p.nsplit) * PR_TILE / kv.page_size) + 2;
   p.scale_log2 = a.softmax_scale * LOG2E;
   p.page_table = kv.page_table, p.seq_lens = kv.seq_lens, p.counts = a.counts;
   p.k_scales = a.cache.k_scales, p.v_scales = a.cache.v_scales;
@@ -651,21 +730,20 @@ template <typename T, int STORE, int D, int MT> static cudaError_t paged_rows_t(
   ok = ok && (s.r > 0 ? make_wide_tmap(&mt, table, false, s.r, s.Nk, 2, 1, s.r, (int64_t)s.Nk * s.r, 0, PR_TILE) : (mt = mk, true));
   if (!ok) return cudaErrorNotSupported;
 
-  constexpr int RB = 16 * MT, FPI = Q8 ? 64 : 32, DP = (D + FPI - 1) / FPI * FPI, KBLK = (D * (Q8 ? 1 : 2) + 127) / 128;
-  const int tblk = (s.r + 63) / 64, RP = (s.r + FPI - 1) / FPI * FPI;
-  const size_t stage = (size_t)(2 * KBLK + 2 * tblk) * PR_BLOCK + (Q8 ? 1024 : 0), red = (size_t)PR_NW * RB * D * 4;
+  const int tblk = (s.r + 63) / 64, RP = (s.r + FPI - 1) / FPI * FPI, rings = NW / (PR_WPT * p.hb);
+  const size_t stage = (size_t)(p.hb * 2 * KBLK + 2 * tblk) * PR_BLOCK + (Q8 ? 1024 : 0), red = (size_t)NW * RB * D * 4;
   const size_t pitch = (DP + RP) * 2 + ((DP + RP) % 64 == 0 ? 64 : 0);
-  const size_t fixed = 1024 + RB * pitch + (size_t)PR_NW * RB * 8 + RB * 8 + 2 * (size_t)s.r * 4 + 2 * 8 * 8 + 64;
-  int nst = (int)((kMaxDynamicSmem - fixed) / stage);
-  p.nstages = nst > 8 ? 8 : nst;
-  if (p.nstages < 2) return cudaErrorInvalidValue;
-  const size_t smem = fixed + std::max(p.nstages * stage, red);
+  const size_t fixed = 1024 + p.hb * RB * pitch + (size_t)NW * RB * 8 + p.hb * RB * 4 + RB * 4 + p.hb * 2 * (size_t)s.r * 4 + rings * 4 * 12 + 16 +
+                       (size_t)p.npg_smem * 4;
+  p.stages = (int)std::min<size_t>(4, (kMaxDynamicSmem - fixed) / (stage * rings));
+  if (fixed > (size_t)kMaxDynamicSmem || p.stages < 1) return cudaErrorInvalidValue;
+  const size_t smem = fixed + std::max(rings * p.stages * stage, red);
   if (smem > (size_t)kMaxDynamicSmem) return cudaErrorInvalidValue;
-  const auto kernel = paged_rows_kernel<T, STORE, D, MT>;
+  const auto kernel = paged_rows_kernel<T, STORE, D, RQ, NW>;
   cudaError_t e;
-  if ((e = ensure_max_smem<paged_rows_kernel<T, STORE, D, MT>>()) != cudaSuccess) return e;
-  const unsigned units = (unsigned)(s.B * s.Hk * p.blocks);
-  const dim3 grid(units * (unsigned)p.nsplit), block(32 * (PR_NW + 1));
+  if ((e = ensure_max_smem<paged_rows_kernel<T, STORE, D, RQ, NW>>()) != cudaSuccess) return e;
+  const unsigned units = (unsigned)(s.B * (s.Hk / p.hb) * p.blocks);
+  const dim3 grid(units * (unsigned)p.nsplit), block(32 * NW);
   // behind the table kernel, which also zeroes the counters
   if (s.r > 0) {
     if ((e = launch_trig_tables(a.embed, s.Nk, s.r, nullptr, nullptr, table, table + (size_t)s.Nk * s.r, st, 1, 1, p.done, (int)units)) != cudaSuccess) return e;
@@ -675,12 +753,13 @@ template <typename T, int STORE, int D, int MT> static cudaError_t paged_rows_t(
   kernel<<<grid, block, smem, st>>>(p, mk, mv, mt);
   return cudaGetLastError();
 }
-template <typename T, int STORE, int D> static cudaError_t paged_rows_m(const PopePagedAttnArgs& a, cudaStream_t st) {
-  return rows_mt(a.shape) == 1 ? paged_rows_t<T, STORE, D, 1>(a, st) : paged_rows_t<T, STORE, D, 2>(a, st);
+template <typename T, int STORE, int D> static cudaError_t paged_rows_q(const PopePagedAttnArgs& a, cudaStream_t st) {
+  const int rq = rows_rq(a.shape);
+  return rq == 1 ? paged_rows_t<T, STORE, D, 1>(a, st) : rq == 2 ? paged_rows_t<T, STORE, D, 2>(a, st) : paged_rows_t<T, STORE, D, 4>(a, st);
 }
 template <typename T, int STORE> static cudaError_t paged_rows_d(const PopePagedAttnArgs& a, cudaStream_t st) {
   const int d = a.shape.d;
-  return d == 64 ? paged_rows_m<T, STORE, 64>(a, st) : d == 96 ? paged_rows_m<T, STORE, 96>(a, st) : paged_rows_m<T, STORE, 128>(a, st);
+  return d == 64 ? paged_rows_q<T, STORE, 64>(a, st) : d == 96 ? paged_rows_q<T, STORE, 96>(a, st) : paged_rows_q<T, STORE, 128>(a, st);
 }
 template <typename T> static cudaError_t paged_rows_s(const PopePagedAttnArgs& a, cudaStream_t st) {
   switch (a.cache.store) {
