@@ -20,8 +20,8 @@
 // Qc = a_q cos(fq - b), Qs = a_q sin(fq - b): the head's bias sits in the query.
 //
 // 8-bit codes: K' and Q' are fp16 whatever the compute type (11 bits instead of 8).  Plain features enter their products as codes,
-// exact in fp16, and the key's scale is applied to the sum.  Magnitudes of rows beyond 2^15 are brought down by a factor that returns
-// with the scores.  V enters as its codes too, and its scale s_j goes into the probability: p_j s_j = 2^(score + log2 s_j - m), with m the
+// exact in fp16, and the key's scale is applied to the sum.  Keys beyond 2^15, whose magnitudes could leave fp16's range, take their
+// products one by one in fp32; a query beyond it is brought down by a factor that returns with its scores.  V enters as its codes too, and its scale s_j goes into the probability: p_j s_j = 2^(score + log2 s_j - m), with m the
 // running maximum of that sum, so that it stays in fp16's range whatever the scales are, while the softmax's own sum adds
 // 2^(score - m) in fp32.
 #include <algorithm>
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(32 * NW, 1)
   }
   for (int i = tid; i < hb * r; i += 32 * NW) {
     const int h = i / r, c = i - h * r;
-    sincosf(p.bias[(hk0 + h) * p.bias_sh + c], &bias_cs[(2 * h + 1) * r + c], &bias_cs[2 * h * r + c]);
+    sincos_reduced(p.bias[(hk0 + h) * p.bias_sh + c], &bias_cs[(2 * h + 1) * r + c], &bias_cs[2 * h * r + c]);
   }
   __syncthreads();
 
@@ -258,8 +258,8 @@ __global__ void __launch_bounds__(32 * NW, 1)
       qc[j] = live && c < D ? to_f32<T>(qrow[c]) : 0.f, qs[j] = 0.f;
       if (live && c < r) {
         float sn, cs;
-        sincosf(p.freqs[(int64_t)pos * p.sfn + c], &sn, &cs);
-        const float a = softplus_f(qc[j]) * (LN2_IN_Q ? LN2 : 1.f);
+        sincos_reduced(p.freqs[(int64_t)pos * p.sfn + c], &sn, &cs);   // (the results are rounded to 11 bits or less)
+        const float a = softplus_fast(qc[j]) * (LN2_IN_Q ? LN2 : 1.f);
         qc[j] = a * (cs * bcs[c] + sn * bcs[r + c]), qs[j] = a * (sn * bcs[c] - cs * bcs[r + c]);
       }
       mx = fmaxf(mx, fmaxf(fabsf(qc[j]), fabsf(qs[j])));
@@ -324,112 +324,128 @@ __global__ void __launch_bounds__(32 * NW, 1)
         sco[m][e] = 0.f;
         if constexpr (Q8) plain[m][e] = 0.f;
       }
-    float ks[2] = {1.f, 1.f}, kd[2] = {1.f, 1.f};   // 8-bit: a key's scale, and the factor that brings its magnitudes down
+    float ks[2] = {1.f, 1.f};   // 8-bit: the scales of the lane's keys
     bool big = false;
     if constexpr (Q8) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        ks[n] = scl[sub * 16 + n * 8 + g];
-        const float top = ks[n] * kCodeTop<STORE>;
-        if (top > PR_BIG) kd[n] = PR_BIG / top, big = true;
-      }
+      for (int n = 0; n < 2; ++n) ks[n] = scl[sub * 16 + n * 8 + g], big = big || ks[n] * kCodeTop<STORE> > PR_BIG;
       big = __any_sync(0xffffffffu, big);
     }
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int ch = 4 * i + t;
-      const bool rot_i = i * FPI < r, all_i = (i + 1) * FPI <= r;   // any, all features of these lanes rotated (the same for all lanes)
-      uint32_t rw[2][4];
-#pragma unroll
+    if (Q8 && big) {   // magnitudes that leave fp16's range: the products one by one, in fp32
+#pragma unroll 1
       for (int n = 0; n < 2; ++n) {
         const int row = sub * 16 + n * 8 + g;
-        const uint4 raw = *reinterpret_cast<const uint4*>(st + (ch >> 3) * PR_BLOCK + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
-        rw[n][0] = raw.x, rw[n][1] = raw.y, rw[n][2] = raw.z, rw[n][3] = raw.w;
-      }
+#pragma unroll 1
+        for (int f0 = 0; f0 < D; f0 += 4) {
+          float2 y[2];
+          codes_times<STORE>(*reinterpret_cast<const uint32_t*>(st + row * 128 + (((f0 >> 4) ^ (row & 7)) << 4) + (f0 & 15)), ks[n], y);
+          float x[4] = {y[0].x, y[0].y, y[1].x, y[1].y};
+#pragma unroll 1
+          for (int e = 0; e < 4; ++e) {
+            const int f = f0 + e;
+            float c = x[0], sn = 0.f;
+            x[0] = x[1], x[1] = x[2], x[2] = x[3];
+            if (f < r) {
+              const uint8_t* trow = tt + (f >> 6) * PR_BLOCK + row * 128 + ((((f >> 3) & 7) ^ (row & 7)) << 4) + (f & 7) * 2;
+              const float a = softplus_fast(c) * LOG2E;
+              c = a * __half2float(*reinterpret_cast<const __half*>(trow)), sn = a * __half2float(*reinterpret_cast<const __half*>(trow + tblk * PR_BLOCK));
+            }
 #pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        const int f0 = ch * VL + h * 8;   // first of the lane's eight features
-        uint32_t kc[2][4], kn[2][4];      // fragments of both keys: features (f0, f0 + 1), ...
-        if (!rot_i) {
+            for (int m = 0; m < RQ; ++m)
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            if constexpr (!Q8) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) kc[n][e] = rw[n][e];
-            } else {
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                uint32_t x[2];
-                codes_to_half<STORE>(rw[n][h * 2 + e], x);
-                kc[n][2 * e] = x[0], kc[n][2 * e + 1] = x[1];
+              for (int j = 0; j < 2; ++j) {
+                const __half* qrow = reinterpret_cast<const __half*>(qsm + (hloc * RB + m * 8 + 2 * t + j) * pitch) + f;
+                float d = fmaf(c, __half2float(qrow[0]), n == 0 ? sco[m][j] : sco[m][2 + j]);
+                if (f < r) d = fmaf(sn, __half2float(qrow[DP]), d);
+                if (n == 0) sco[m][j] = d;
+                else sco[m][2 + j] = d;
               }
-            }
           }
-        } else {
-          const bool rot = all_i || f0 < r;
+        }
+      }
+    } else {
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const int row = sub * 16 + n * 8 + g;
-            const uint8_t* trow = tt + (f0 >> 6) * PR_BLOCK + row * 128 + ((((f0 >> 3) & 7) ^ (row & 7)) << 4);
-            const uint4 cr = *reinterpret_cast<const uint4*>(trow);
-            const uint4 sr = *reinterpret_cast<const uint4*>(trow + tblk * PR_BLOCK);   // (zeros where nothing is rotated)
-            uint32_t cw[4] = {cr.x, cr.y, cr.z, cr.w};
-            const uint32_t sw[4] = {sr.x, sr.y, sr.z, sr.w};
-            float2 x[4];
-            if constexpr (!Q8) {
+      for (int i = 0; i < NI; ++i) {
+        const int ch = 4 * i + t;
+        uint32_t rw[2][4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) x[e] = mul2(unpack2<T>(rw[n][e]), make_float2(LOG2E, LOG2E));
-            } else {
-              float2 y[2];
+        for (int n = 0; n < 2; ++n) {
+          const int row = sub * 16 + n * 8 + g;
+          const uint4 raw = *reinterpret_cast<const uint4*>(st + (ch >> 3) * PR_BLOCK + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
+          rw[n][0] = raw.x, rw[n][1] = raw.y, rw[n][2] = raw.z, rw[n][3] = raw.w;
+        }
+        // (the conditions are the same for all lanes; where a group of features is rotated in part, both parts work on it: the cosines and sines
+        // of plain features have arrived as zeros, and rotated features are zeros to the plain part)
+        if (i * FPI < r) {
 #pragma unroll
-              for (int e = 0; e < 2; ++e) codes_times<STORE>(rw[n][h * 2 + e], ks[n] * LOG2E, y), x[2 * e] = y[0], x[2 * e + 1] = y[1];
-            }
-            if (all_i) {
+          for (int h = 0; h < NH; ++h) {
+            const int f0 = ch * VL + h * 8;   // first of the lane's eight features
+            uint32_t kc[2][4], kn[2][4];      // fragments of both keys: features (f0, f0 + 1), ...
 #pragma unroll
-              for (int e = 0; e < 4; ++e) x[e] = softplus_log2(x[e]);
-            } else {   // plain features among them: in the same units, with a cosine of one
+            for (int n = 0; n < 2; ++n) {
+              const int row = sub * 16 + n * 8 + g;
+              const uint8_t* trow = tt + (f0 >> 6) * PR_BLOCK + row * 128 + ((((f0 >> 3) & 7) ^ (row & 7)) << 4);
+              const uint4 cr = *reinterpret_cast<const uint4*>(trow), sr = *reinterpret_cast<const uint4*>(trow + tblk * PR_BLOCK);
+              const uint32_t cw[4] = {cr.x, cr.y, cr.z, cr.w}, sw[4] = {sr.x, sr.y, sr.z, sr.w};
+              float2 x[4];
+              if constexpr (!Q8) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = mul2(unpack2<T>(rw[n][e]), make_float2(LOG2E, LOG2E));
+              } else {
+                float2 y[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) codes_times<STORE>(rw[n][h * 2 + e], ks[n] * LOG2E, y), x[2 * e] = y[0], x[2 * e + 1] = y[1];
+              }
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const float2 a = softplus_log2(x[e]);
-                const float f = LN2_IN_Q ? LN2 : 1.f;
-                x[e] = rot ? a : mul2(x[e], make_float2(f, f));
-                if (!rot) cw[e] = 0x3c003c00u;
+                x[e] = softplus_log2(x[e]);
+                if constexpr (!LN2_IN_Q) x[e] = mul2(x[e], make_float2(LN2, LN2));
+                if constexpr (HALF) {
+                  const uint32_t a = pack2<__half>(x[e].x, x[e].y);
+                  kc[n][e] = hmul2(a, cw[e]), kn[n][e] = hmul2(a, sw[e]);
+                } else {
+                  const float2 c = mul2(x[e], unpack2<__half>(cw[e])), v = mul2(x[e], unpack2<__half>(sw[e]));
+                  kc[n][e] = pack2<TM>(c.x, c.y), kn[n][e] = pack2<TM>(v.x, v.y);
+                }
               }
             }
-            if constexpr (!LN2_IN_Q) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) x[e] = mul2(x[e], make_float2(LN2, LN2));
-            }
-            if (Q8 && big) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) x[e] = mul2(x[e], make_float2(kd[n], kd[n]));
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if constexpr (HALF) {
-                const uint32_t a = pack2<__half>(x[e].x, x[e].y);
-                kc[n][e] = hmul2(a, cw[e]), kn[n][e] = hmul2(a, sw[e]);
-              } else {
-                const float2 c = mul2(x[e], unpack2<__half>(cw[e])), v = mul2(x[e], unpack2<__half>(sw[e]));
-                kc[n][e] = pack2<TM>(c.x, c.y), kn[n][e] = pack2<TM>(v.x, v.y);
-              }
+            for (int m = 0; m < RQ; ++m) {
+              const uint8_t* qa = qlane + m * 8 * pitch + (i * FPI + h * 8) * 2;
+              const uint4 qc = *reinterpret_cast<const uint4*>(qa), qs = *reinterpret_cast<const uint4*>(qa + DP * 2);
+              mma16816<TM>(sco[m], kc[0][0], kc[1][0], kc[0][1], kc[1][1], qc.x, qc.y);
+              mma16816<TM>(sco[m], kc[0][2], kc[1][2], kc[0][3], kc[1][3], qc.z, qc.w);
+              mma16816<TM>(sco[m], kn[0][0], kn[1][0], kn[0][1], kn[1][1], qs.x, qs.y);
+              mma16816<TM>(sco[m], kn[0][2], kn[1][2], kn[0][3], kn[1][3], qs.z, qs.w);
             }
           }
         }
+        if ((i + 1) * FPI > r) {
 #pragma unroll
-        for (int m = 0; m < RQ; ++m) {
-          const uint8_t* qa = qlane + m * 8 * pitch + (i * FPI + h * 8) * 2;
-          const uint4 qc = *reinterpret_cast<const uint4*>(qa);
-          if (rot_i) {
-            const uint4 qs = *reinterpret_cast<const uint4*>(qa + DP * 2);
-            mma16816<TM>(sco[m], kc[0][0], kc[1][0], kc[0][1], kc[1][1], qc.x, qc.y);
-            mma16816<TM>(sco[m], kc[0][2], kc[1][2], kc[0][3], kc[1][3], qc.z, qc.w);
-            mma16816<TM>(sco[m], kn[0][0], kn[1][0], kn[0][1], kn[1][1], qs.x, qs.y);
-            mma16816<TM>(sco[m], kn[0][2], kn[1][2], kn[0][3], kn[1][3], qs.z, qs.w);
-          } else {
-            float(&acc)[4] = Q8 ? plain[Q8 ? m : 0] : sco[m];
-            mma16816<TM>(acc, kc[0][0], kc[1][0], kc[0][1], kc[1][1], qc.x, qc.y);
-            mma16816<TM>(acc, kc[0][2], kc[1][2], kc[0][3], kc[1][3], qc.z, qc.w);
+          for (int h = 0; h < NH; ++h) {
+            const uint32_t keep = ch * VL + h * 8 >= r ? 0xffffffffu : 0u;
+            uint32_t kc[2][4];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              if constexpr (!Q8) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) kc[n][e] = rw[n][e] & keep;
+              } else {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  uint32_t x[2];
+                  codes_to_half<STORE>(rw[n][h * 2 + e] & keep, x);
+                  kc[n][2 * e] = x[0], kc[n][2 * e + 1] = x[1];
+                }
+              }
+            }
+#pragma unroll
+            for (int m = 0; m < RQ; ++m) {
+              const uint4 qc = *reinterpret_cast<const uint4*>(qlane + m * 8 * pitch + (i * FPI + h * 8) * 2);
+              float(&acc)[4] = Q8 ? plain[Q8 ? m : 0] : sco[m];
+              mma16816<TM>(acc, kc[0][0], kc[1][0], kc[0][1], kc[1][1], qc.x, qc.y);
+              mma16816<TM>(acc, kc[0][2], kc[1][2], kc[0][3], kc[1][3], qc.z, qc.w);
+            }
           }
         }
       }
@@ -440,7 +456,6 @@ __global__ void __launch_bounds__(32 * NW, 1)
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
         vs[n] = scl[PR_TILE + sub * 16 + n * 8 + g], lvs[n] = fmaxf(lg2_approx(vs[n]), -100.f);
-        kd[n] = big ? fmaxf(1.f, ks[n] * (kCodeTop<STORE> / PR_BIG)) : 1.f;   // (from here on what returns with the scores)
       }
     }
     const bool clean = key0 + 16 <= min(ke, first_pos + 1);   // every row sees every key of this warp
@@ -452,7 +467,7 @@ __global__ void __launch_bounds__(32 * NW, 1)
       for (int e = 0; e < 4; ++e) {
         const int n = e >> 1;
         float v = sco[m][e];
-        if constexpr (Q8) v = fmaf(plain[m][e], ks[n], v * kd[n]);
+        if constexpr (Q8) v = fmaf(plain[m][e], ks[n], v);
         v *= sc_of[m][e & 1];
         if (!clean && key0 + n * 8 + g > min(ke - 1, pos_of[m][e & 1])) v = -CUDART_INF_F;
         sco[m][e] = v;
@@ -564,46 +579,72 @@ __global__ void __launch_bounds__(32 * NW, 1)
       if (g == 0) red_ml[(w * RB + m * 8 + 2 * t + e) * 2] = m_run[m][e], red_ml[(w * RB + m * 8 + 2 * t + e) * 2 + 1] = l_run[m][e];
     }
   __syncthreads();   // every tile has been read: the ring takes the warps' outputs
+  // [NW][RB][D], the groups of four features of a row exchanged so that the lanes of a store fall on distinct banks
   float* red_o = reinterpret_cast<float*>(smem);
+  auto place = [](int row, int c4) { return c4 ^ ((row >> 1 & 3) << (Q8 ? 0 : 1)); };
 #pragma unroll
   for (int m = 0; m < RQ; ++m)
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int e = 0; e < 2; ++e) {
+      const int row = m * 8 + 2 * t + e;
+      float* dst = red_o + (size_t)(w * RB + row) * D;
+      if constexpr (Q8) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int c = Q8 ? g * FL + 2 * n + (e >> 1) : n * 16 + g + (e >> 1) * 8;
-        red_o[(w * RB + m * 8 + 2 * t + (e & 1)) * D + c] = o[m][n][e];
+        for (int n = 0; n < NT; n += 2)
+          *reinterpret_cast<float4*>(dst + 4 * place(row, (g * FL) / 4 + n / 2)) = make_float4(o[m][n][e], o[m][n][2 + e], o[m][n + 1][e], o[m][n + 1][2 + e]);
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int f = 0; f < 2; ++f) dst[4 * place(row, n * 4 + f * 2 + (g >> 2)) + (g & 3)] = o[m][n][2 * f + e];
       }
-  __syncthreads();
-  auto write_out = [&](int h, int row, int c, float x) {
-    const int rho = rb * RB + row, tok = rho / p.G, head = hk0 + h + (rho - tok * p.G) * p.Hk;
-    static_cast<T*>(p.out)[b * p.so.b + head * p.so.h + (int64_t)tok * p.so.n + c] = from_f32<T>(x);
+    }
+  const int out_rows = min(RB, p.Nq * p.G - rb * RB);   // (padding is written too)
+  auto row_of = [&](int hr, int* tok, int* head) {      // row of the block (and of its head) -> token and query head
+    const int h = hr / out_rows, rho = rb * RB + hr - h * out_rows;
+    *tok = rho / p.G, *head = hk0 + h + (rho - *tok * p.G) * p.Hk;
+    return h * RB + hr - h * out_rows;
   };
-  auto write_lse = [&](int h, int row, float M, float L) {
-    const int rho = rb * RB + row, tok = rho / p.G, head = hk0 + h + (rho - tok * p.G) * p.Hk;
+  auto write_out = [&](int tok, int head, int c4, float4 x, float L) {
+    const float inv = L != 0.f ? 1.f / L : 0.f;
+    T* dst = static_cast<T*>(p.out) + b * p.so.b + head * p.so.h + (int64_t)tok * p.so.n + 4 * c4;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(x.x * inv, x.y * inv), pack2<T>(x.z * inv, x.w * inv));
+  };
+  auto write_lse = [&](int tok, int head, float M, float L) {
     if (p.lse) p.lse[((int64_t)b * p.H + head) * p.Nq + tok] = L != 0.f ? M * LN2 + logf(L) : -CUDART_INF_F;
   };
-  const int out_rows = min(RB, p.Nq * p.G - rb * RB);   // (padding is written too)
+  auto warp_of = [&](int k, int h) { return ((k / PR_WPT) * hb + h) * PR_WPT + k % PR_WPT; };   // warp k of head h
   const int64_t slot = ((int64_t)u * p.nsplit + split) * hb * RB;
-  for (int i = tid; i < hb * out_rows * D; i += 32 * NW) {
-    const int c = i % D, hr = i / D, h = hr / out_rows, row = hr - h * out_rows;
-    float M = -CUDART_INF_F, L = 0.f, acc = 0.f;
-    auto warp_of = [&](int k) { return ((k / PR_WPT) * hb + h) * PR_WPT + k % PR_WPT; };   // warp k of this head
-    for (int k = 0; k < NW / hb; ++k) M = fmaxf(M, red_ml[(warp_of(k) * RB + row) * 2]);
-    const float mu = M == -CUDART_INF_F ? 0.f : M;
+  float* row_sum = row_scale;   // (the scales have been read)
+  for (int hr = w; hr < hb * out_rows; hr += NW) {   // a warp per row: the weights of the warps, in the place of their maxima
+    int tok, head;
+    const int at = row_of(hr, &tok, &head), h = at / RB, row = at - h * RB;
+    float m1 = -CUDART_INF_F, l1 = 0.f;
+    float* ml = red_ml + (warp_of(lane % (NW / hb), h) * RB + row) * 2;
+    if (lane < NW / hb && row_pos[row] >= 0) m1 = ml[0], l1 = ml[1];   // (no query: where every query sees every key these rows were not told apart)
+    const float M = warp_max(m1), f = ex2_approx(m1 - (M == -CUDART_INF_F ? 0.f : M));   // 0 for a warp without visible keys
+    const float L = warp_sum(l1 * f);
+    if (lane < NW / hb) ml[0] = f;
+    if (lane == 0) {
+      row_sum[at] = L;
+      if (p.nsplit == 1) write_lse(tok, head, M, L);
+      else p.part_ml[(slot + at) * 2] = M, p.part_ml[(slot + at) * 2 + 1] = L;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < hb * out_rows * (D / 4); i += 32 * NW) {
+    const int c4 = i % (D / 4), hr = i / (D / 4);
+    int tok, head;
+    const int at = row_of(hr, &tok, &head), h = at / RB, row = at - h * RB;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int k = 0; k < NW / hb; ++k) {
-      const int at = warp_of(k) * RB + row;
-      const float f = ex2_approx(red_ml[at * 2] - mu);   // 0 for a warp without visible keys
-      L = fmaf(red_ml[at * 2 + 1], f, L), acc = fmaf(red_o[(size_t)at * D + c], f, acc);
+      const int from = warp_of(k, h) * RB + row;
+      const float f = red_ml[from * 2];
+      const float4 x = *reinterpret_cast<const float4*>(red_o + (size_t)from * D + 4 * place(row, c4));
+      if (f != 0.f) acc.x = fmaf(f, x.x, acc.x), acc.y = fmaf(f, x.y, acc.y), acc.z = fmaf(f, x.z, acc.z), acc.w = fmaf(f, x.w, acc.w);
     }
-    if (row_pos[row] < 0) M = -CUDART_INF_F, L = acc = 0.f;   // (where every query sees every key the other rows of the block were not told apart)
-    if (p.nsplit == 1) {
-      write_out(h, row, c, L != 0.f ? acc / L : 0.f);
-      if (c == 0) write_lse(h, row, M, L);
-    } else {
-      p.part_o[(slot + h * RB + row) * D + c] = acc;
-      if (c == 0) p.part_ml[(slot + h * RB + row) * 2] = M, p.part_ml[(slot + h * RB + row) * 2 + 1] = L;
-    }
+    if (p.nsplit == 1) write_out(tok, head, c4, acc, row_sum[at]);
+    else *reinterpret_cast<float4*>(p.part_o + (slot + at) * D + 4 * c4) = acc;
   }
   if (p.nsplit == 1) return;
   // The CTA that finishes last merges the splits of its unit.
@@ -616,7 +657,8 @@ __global__ void __launch_bounds__(32 * NW, 1)
   float* wgt = reinterpret_cast<float*>(smem);   // [hb][RB][nsplit] weights of the splits
   const int64_t slot0 = (int64_t)u * p.nsplit * hb * RB;
   for (int hr = w; hr < hb * out_rows; hr += NW) {
-    const int h = hr / out_rows, row = hr - h * out_rows, at = h * RB + row;
+    int tok, head;
+    const int at = row_of(hr, &tok, &head);
     float m2[PR_MAX_SPLIT / 32], l2[PR_MAX_SPLIT / 32], M = -CUDART_INF_F, L = 0.f;
 #pragma unroll
     for (int i = 0; i < PR_MAX_SPLIT / 32; ++i) {
@@ -636,15 +678,21 @@ __global__ void __launch_bounds__(32 * NW, 1)
 #pragma unroll
     for (int i = 0; i < PR_MAX_SPLIT / 32; ++i)
       if (lane + 32 * i < p.nsplit) wgt[at * p.nsplit + lane + 32 * i] = m2[i];
-    if (lane == 0) red_ml[at] = L, write_lse(h, row, M, L);
+    if (lane == 0) row_sum[at] = L, write_lse(tok, head, M, L);
   }
   __syncthreads();
-  for (int i = tid; i < hb * out_rows * D; i += 32 * NW) {
-    const int c = i % D, hr = i / D, h = hr / out_rows, row = hr - h * out_rows, at = h * RB + row;
-    float acc = 0.f;
+  for (int i = tid; i < hb * out_rows * (D / 4); i += 32 * NW) {
+    const int c4 = i % (D / 4), hr = i / (D / 4);
+    int tok, head;
+    const int at = row_of(hr, &tok, &head);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
-    for (int sp = 0; sp < p.nsplit; ++sp) acc = fmaf(wgt[at * p.nsplit + sp], __ldcg(p.part_o + (slot0 + (int64_t)sp * hb * RB + at) * D + c), acc);
-    write_out(h, row, c, red_ml[at] != 0.f ? acc / red_ml[at] : 0.f);
+    for (int sp = 0; sp < p.nsplit; ++sp) {
+      const float f = wgt[at * p.nsplit + sp];
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + (slot0 + (int64_t)sp * hb * RB + at) * D + 4 * c4));
+      acc.x = fmaf(f, x.x, acc.x), acc.y = fmaf(f, x.y, acc.y), acc.z = fmaf(f, x.z, acc.z), acc.w = fmaf(f, x.w, acc.w);
+    }
+    write_out(tok, head, c4, acc, row_sum[at]);
   }
 }
 

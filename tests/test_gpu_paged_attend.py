@@ -136,6 +136,28 @@ def test_layouts_and_scales(store, new):
         R.check(cache.attend(q, emb, softmax_scale=scale)[:, :, -3:], ref[0], ref[2], ref[3])
 
 
+@pytest.mark.parametrize("store", [None, I8, F8])
+@pytest.mark.parametrize("new", [2, 40])
+def test_magnitudes_beyond_fp16(store, new):
+    """bf16 keys up to 3e5 against small queries, queries up to 3e5 against small keys, values from 1e-30 to 1e30."""
+    g = torch.Generator(device=DEV).manual_seed(new)
+    hk, d, r, n = 2, 64, 32, 150
+    k = torch.randn(1, hk, n, d, device=DEV, generator=g)
+    v = torch.randn(1, hk, n, d, device=DEV, generator=g)
+    q = torch.randn(1, 4, new, d, device=DEV, generator=g)
+    emb = table(r, hk, n, g)
+    rows = torch.arange(n, device=DEV)
+    for dk, dq, dv in ((1e5, 1e-5, 1.0), (1e-5, 1e5, 1e30), (1.0, 1.0, 1e-30), (1.0, 1.0, 1e30)):
+        cache = make(1, hk, d, BF, store, n)
+        many = (rows % 3 == 1)[:, None]
+        cache.append((torch.where(many, k * dk, k)).bfloat16(), (v * dv).bfloat16())
+        qq = (q * dq).bfloat16()
+        vals = held(cache)
+        ref = R.attend(qq, [x[0] for x in vals], [x[1] for x in vals], emb[0], emb[1], [n], [new], 0.125, store)
+        got = cache.attend(qq, emb).double().cpu() / dv
+        R.check(got, ref[0] / dv, ref[2] / dv, ref[3] / dv)
+
+
 def test_counts_out_of_range_are_clamped_and_no_rows_are_none():
     g = torch.Generator(device=DEV).manual_seed(1)
     cache = make(2, 1, 64, BF, None, 200)
