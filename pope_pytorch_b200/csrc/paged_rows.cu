@@ -37,7 +37,6 @@ struct PagedRowsP {
   int page_size, max_pages, num_pages, npg_smem;         // (sequence, key head); hb: key heads that a CTA takes
   float scale_log2;
   const int32_t *page_table, *seq_lens, *counts;
-  const float *k_scales, *v_scales;
   const float *freqs, *bias;
   int64_t sfn, bias_sh;
   const void* q;
@@ -153,7 +152,7 @@ constexpr float PR_BIG = 32768.f;   // magnitudes of fp16 operands stay below tw
 template <typename T, int STORE, int D, int RQ, int NW>
 __global__ void __launch_bounds__(32 * NW, 1)
     paged_rows_kernel(PagedRowsP p, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
-                      const __grid_constant__ CUtensorMap tmap_t) {
+                      const __grid_constant__ CUtensorMap tmap_t, const __grid_constant__ CUtensorMap tmap_ks, const __grid_constant__ CUtensorMap tmap_vs) {
   constexpr bool Q8 = STORE != POPE_STORE_16;
   using TM = std::conditional_t<Q8, __half, T>;            // operand type of the products
   constexpr bool HALF = std::is_same_v<TM, __half>;
@@ -172,8 +171,8 @@ __global__ void __launch_bounds__(32 * NW, 1)
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int r = p.r, tblk = (r + 63) / 64, RP = (r + FPI - 1) / FPI * FPI, hb = p.hb;
   const int rings = NW / (PR_WPT * hb);                                // tiles in work at a time, a ring of stages for each
-  const int head_bytes = 2 * KBLK * PR_BLOCK, trig_at = hb * head_bytes, scale_at = trig_at + 2 * tblk * PR_BLOCK;
-  const int stage_bytes = scale_at + (Q8 ? 1024 : 0);                 // [head][K blocks, V blocks][cos][sin][head][k scales, v scales]
+  const int v_at = hb * KBLK * PR_BLOCK, trig_at = 2 * v_at, scale_at = trig_at + 2 * tblk * PR_BLOCK;
+  const int stage_bytes = scale_at + (Q8 ? 1024 : 0);   // [K block][head], [V block][head], [trig block][cos, sin], [k, v][head] scales
   const int pitch = (DP + RP) * 2 + ((DP + RP) % 64 == 0 ? 64 : 0);   // an odd multiple of 64 bytes: eight rows x 64 bytes on distinct banks
   const size_t ring = (size_t)rings * p.stages * stage_bytes, red_bytes = (size_t)NW * RB * D * 4;
   uint8_t* qsm = smem + (ring > red_bytes ? ring : red_bytes);        // Q': [hb][RB] rows of (cos or plain features, sin features)
@@ -218,67 +217,77 @@ __global__ void __launch_bounds__(32 * NW, 1)
   }
   __syncthreads();
 
-  // One thread: the copies of tile jt into stage `at` (ring * stages + stage)
+  // One thread: the copies of tile jt into stage `at` (ring * stages + stage).  (Issuing one takes more than 100 clocks: as few as possible,
+  // in boxes over all of the CTA's key heads.  A box for each head, array and scale, ten copies a tile where there are five now, took
+  // 1300 clocks of one of the warps that share the tile, and 10000 of the first warp before it could start.)
   auto load_tile = [&](int jt, int at) {
-    const int key0 = kb + jt * PR_TILE, row = key0 % p.page_size, pg = pages_s[key0 / p.page_size - kb / p.page_size];
+    const int key0 = kb + jt * PR_TILE, lp = key0 / p.page_size, row = key0 - lp * p.page_size, pg = pages_s[lp - kb / p.page_size];
     uint8_t* st = smem + (size_t)at * stage_bytes;
     uint64_t* bar = &full[at];
     mbar_expect_tx(bar, (uint32_t)(scale_at + (Q8 ? hb * 8 * PR_TILE : 0)));
-    for (int h = 0; h < hb; ++h)
 #pragma unroll
-      for (int c = 0; c < KBLK; ++c) {
-        tma_load_4d(st + h * head_bytes + c * PR_BLOCK, &tmap_k, bar, c * EPB, row, hk0 + h, pg);
-        tma_load_4d(st + h * head_bytes + (KBLK + c) * PR_BLOCK, &tmap_v, bar, c * EPB, row, hk0 + h, pg);
-      }
-    for (int c = 0; c < tblk; ++c) {
-      tma_load_4d(st + trig_at + c * PR_BLOCK, &tmap_t, bar, c * 64, key0, 0, 0);
-      tma_load_4d(st + trig_at + (tblk + c) * PR_BLOCK, &tmap_t, bar, c * 64, key0, 1, 0);
-    }
+    for (int c = 0; c < KBLK; ++c) tma_load_4d(st + c * hb * PR_BLOCK, &tmap_k, bar, c * 128, row, hk0, pg);
+    for (int c = 0; c < tblk; ++c) tma_load_4d(st + trig_at + 2 * c * PR_BLOCK, &tmap_t, bar, c * 64, key0, 0, 0);
     if constexpr (Q8) {
-      for (int h = 0; h < hb; ++h) {
-        const int64_t from = ((int64_t)pg * p.Hk + hk0 + h) * p.page_size + row;
-        uint8_t* sc = st + scale_at + h * 8 * PR_TILE;
-        bulk_load(sc, p.k_scales + from, 4 * PR_TILE, bar), bulk_load(sc + 4 * PR_TILE, p.v_scales + from, 4 * PR_TILE, bar);
-      }
+      tma_load_4d(st + scale_at, &tmap_ks, bar, row, hk0, pg, 0);
+      tma_load_4d(st + scale_at + hb * 4 * PR_TILE, &tmap_vs, bar, row, hk0, pg, 0);
     }
+#pragma unroll
+    for (int c = 0; c < KBLK; ++c) tma_load_4d(st + v_at + c * hb * PR_BLOCK, &tmap_v, bar, c * 128, row, hk0, pg);
   };
-  if (tid == 0)
-    for (int jt = 0; jt < min(T_tiles, rings * p.stages); ++jt) load_tile(jt, jt % rings * p.stages + jt / rings);
+  for (int jt = w; jt < min(T_tiles, rings * p.stages); jt += NW)
+    if (lane == 0) load_tile(jt, jt % rings * p.stages + jt / rings);
+  __syncwarp();
 
-  for (int i = w; i < hb * RB; i += NW) {   // a warp per row of Q'
-    const int h = i / RB, row = i - h * RB;
-    const int rho = rb * RB + row, tok = rho / p.G, head = hk0 + h + (rho - tok * p.G) * p.Hk, pos = len - cnt + tok;
-    const bool live = row < rows && pos >= 0;
-    const T* qrow = static_cast<const T*>(p.q) + b * p.sq.b + head * p.sq.h + (int64_t)tok * p.sq.n;
-    const float* bcs = bias_cs + 2 * h * r;
-    float qc[DP / 32], qs[DP / 32], mx = 0.f;
+  constexpr int QU = 4;   // rows of Q' that a warp has in work: their loads go out together
+  for (int i0 = w; i0 < hb * RB; i0 += QU * NW) {
+    float x[QU][DP / 32], f[QU][DP / 32];
+    bool live[QU];
 #pragma unroll
-    for (int j = 0; j < DP / 32; ++j) {
-      const int c = lane + 32 * j;
-      qc[j] = live && c < D ? to_f32<T>(qrow[c]) : 0.f, qs[j] = 0.f;
-      if (live && c < r) {
-        float sn, cs;
-        sincos_reduced(p.freqs[(int64_t)pos * p.sfn + c], &sn, &cs);   // (the results are rounded to 11 bits or less)
-        const float a = softplus_fast(qc[j]) * (LN2_IN_Q ? LN2 : 1.f);
-        qc[j] = a * (cs * bcs[c] + sn * bcs[r + c]), qs[j] = a * (sn * bcs[c] - cs * bcs[r + c]);
+    for (int k = 0; k < QU; ++k) {
+      const int i = i0 + k * NW, h = i / RB, row = i - h * RB;
+      const int rho = rb * RB + row, tok = rho / p.G, head = hk0 + h + (rho - tok * p.G) * p.Hk, pos = len - cnt + tok;
+      live[k] = h < hb && row < rows && pos >= 0;
+      if (lane == 0 && h == 0) row_pos[row] = live[k] ? pos : -1;
+      const T* qrow = static_cast<const T*>(p.q) + b * p.sq.b + head * p.sq.h + (int64_t)tok * p.sq.n;
+#pragma unroll
+      for (int j = 0; j < DP / 32; ++j) {
+        const int c = lane + 32 * j;
+        x[k][j] = live[k] && c < D ? to_f32<T>(qrow[c]) : 0.f;
+        f[k][j] = live[k] && c < r ? p.freqs[(int64_t)pos * p.sfn + c] : 0.f;
       }
-      mx = fmaxf(mx, fmaxf(fabsf(qc[j]), fabsf(qs[j])));
     }
-    float down = 1.f;
-    if constexpr (Q8) {
-      mx = warp_max(mx);
-      if (mx > PR_BIG && mx < CUDART_INF_F) down = PR_BIG / mx;
-    }
-    TM* dst = reinterpret_cast<TM*>(qsm + i * pitch);
 #pragma unroll
-    for (int j = 0; j < DP / 32; ++j) {
-      const int c = lane + 32 * j;
-      dst[c] = from_f32<TM>(qc[j] * down);
-      if (c < RP) dst[DP + c] = from_f32<TM>(qs[j] * down);
-    }
-    if (lane == 0) {
-      row_scale[i] = p.scale_log2 / down;
-      if (h == 0) row_pos[row] = live ? pos : -1;
+    for (int k = 0; k < QU; ++k) {
+      const int i = i0 + k * NW, h = i / RB;
+      if (h >= hb) break;
+      const float* bcs = bias_cs + 2 * h * r;
+      float qs[DP / 32], mx = 0.f;
+#pragma unroll
+      for (int j = 0; j < DP / 32; ++j) {
+        const int c = lane + 32 * j;
+        qs[j] = 0.f;
+        if (live[k] && c < r) {
+          float sn, cs;
+          sincos_reduced(f[k][j], &sn, &cs);   // (the results are rounded to 11 bits or less)
+          const float a = softplus_fast(x[k][j]) * (LN2_IN_Q ? LN2 : 1.f);
+          x[k][j] = a * (cs * bcs[c] + sn * bcs[r + c]), qs[j] = a * (sn * bcs[c] - cs * bcs[r + c]);
+        }
+        mx = fmaxf(mx, fmaxf(fabsf(x[k][j]), fabsf(qs[j])));
+      }
+      float down = 1.f;
+      if constexpr (Q8) {
+        mx = warp_max(mx);
+        if (mx > PR_BIG && mx < CUDART_INF_F) down = PR_BIG / mx;
+      }
+      TM* dst = reinterpret_cast<TM*>(qsm + i * pitch);
+#pragma unroll
+      for (int j = 0; j < DP / 32; ++j) {
+        const int c = lane + 32 * j;
+        dst[c] = from_f32<TM>(x[k][j] * down);
+        if (c < RP) dst[DP + c] = from_f32<TM>(qs[j] * down);
+      }
+      if (lane == 0) row_scale[i] = p.scale_log2 / down;
     }
   }
   __syncthreads();
@@ -309,8 +318,9 @@ __global__ void __launch_bounds__(32 * NW, 1)
     const int at = rg * p.stages + s;
     uint8_t* st = smem + (size_t)at * stage_bytes;
     const uint8_t* tt = st + trig_at;
-    const float* scl = reinterpret_cast<const float*>(st + scale_at) + hloc * 2 * PR_TILE;
-    st += hloc * head_bytes;
+    const float* scl = reinterpret_cast<const float*>(st + scale_at) + hloc * PR_TILE;
+    uint8_t* vt = st + v_at + hloc * PR_BLOCK;
+    st += hloc * PR_BLOCK;
     if (!mbar_wait(&full[at], par, WAIT_LIMIT)) {
       failed = true;
       break;
@@ -346,9 +356,9 @@ __global__ void __launch_bounds__(32 * NW, 1)
             float c = x[0], sn = 0.f;
             x[0] = x[1], x[1] = x[2], x[2] = x[3];
             if (f < r) {
-              const uint8_t* trow = tt + (f >> 6) * PR_BLOCK + row * 128 + ((((f >> 3) & 7) ^ (row & 7)) << 4) + (f & 7) * 2;
+              const uint8_t* trow = tt + (f >> 6) * 2 * PR_BLOCK + row * 128 + ((((f >> 3) & 7) ^ (row & 7)) << 4) + (f & 7) * 2;
               const float a = softplus_fast(c) * LOG2E;
-              c = a * __half2float(*reinterpret_cast<const __half*>(trow)), sn = a * __half2float(*reinterpret_cast<const __half*>(trow + tblk * PR_BLOCK));
+              c = a * __half2float(*reinterpret_cast<const __half*>(trow)), sn = a * __half2float(*reinterpret_cast<const __half*>(trow + PR_BLOCK));
             }
 #pragma unroll
             for (int m = 0; m < RQ; ++m)
@@ -371,7 +381,7 @@ __global__ void __launch_bounds__(32 * NW, 1)
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           const int row = sub * 16 + n * 8 + g;
-          const uint4 raw = *reinterpret_cast<const uint4*>(st + (ch >> 3) * PR_BLOCK + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
+          const uint4 raw = *reinterpret_cast<const uint4*>(st + (ch >> 3) * hb * PR_BLOCK + row * 128 + (((ch & 7) ^ (row & 7)) << 4));
           rw[n][0] = raw.x, rw[n][1] = raw.y, rw[n][2] = raw.z, rw[n][3] = raw.w;
         }
         // (the conditions are the same for all lanes; where a group of features is rotated in part, both parts work on it: the cosines and sines
@@ -384,8 +394,8 @@ __global__ void __launch_bounds__(32 * NW, 1)
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
               const int row = sub * 16 + n * 8 + g;
-              const uint8_t* trow = tt + (f0 >> 6) * PR_BLOCK + row * 128 + ((((f0 >> 3) & 7) ^ (row & 7)) << 4);
-              const uint4 cr = *reinterpret_cast<const uint4*>(trow), sr = *reinterpret_cast<const uint4*>(trow + tblk * PR_BLOCK);
+              const uint8_t* trow = tt + (f0 >> 6) * 2 * PR_BLOCK + row * 128 + ((((f0 >> 3) & 7) ^ (row & 7)) << 4);
+              const uint4 cr = *reinterpret_cast<const uint4*>(trow), sr = *reinterpret_cast<const uint4*>(trow + PR_BLOCK);
               const uint32_t cw[4] = {cr.x, cr.y, cr.z, cr.w}, sw[4] = {sr.x, sr.y, sr.z, sr.w};
               float2 x[4];
               if constexpr (!Q8) {
@@ -455,7 +465,7 @@ __global__ void __launch_bounds__(32 * NW, 1)
     if constexpr (Q8) {
 #pragma unroll
       for (int n = 0; n < 2; ++n) {
-        vs[n] = scl[PR_TILE + sub * 16 + n * 8 + g], lvs[n] = fmaxf(lg2_approx(vs[n]), -100.f);
+        vs[n] = scl[hb * PR_TILE + sub * 16 + n * 8 + g], lvs[n] = fmaxf(lg2_approx(vs[n]), -100.f);
       }
     }
     const bool clean = key0 + 16 <= min(ke, first_pos + 1);   // every row sees every key of this warp
@@ -501,12 +511,11 @@ __global__ void __launch_bounds__(32 * NW, 1)
       pb[m][0] = movmatrix_trans(pack2<TM>(pr[0], pr[1])), pb[m][1] = movmatrix_trans(pack2<TM>(pr[2], pr[3]));
     }
     // ---- O^T += V^T P^T ---------------------------------------------------------------------------------
-    uint8_t* vt = st + KBLK * PR_BLOCK;
     if constexpr (!Q8) {
       if (key0 + 16 > ke) {   // rows behind the last key may hold anything, and 0 * NaN is NaN
         const int dead = min(16, key0 + 16 - ke);
         for (int i = lane; i < dead * KBLK * 8; i += 32)
-          *reinterpret_cast<uint4*>(vt + (i / 8 / dead) * PR_BLOCK + (sub * 16 + 16 - dead + i / 8 % dead) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(vt + (i / 8 / dead) * hb * PR_BLOCK + (sub * 16 + 16 - dead + i / 8 % dead) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
         __syncwarp();
       }
       const int row = sub * 16 + (lane & 7) + ((lane >> 4) << 3);
@@ -514,7 +523,7 @@ __global__ void __launch_bounds__(32 * NW, 1)
       for (int n = 0; n < NT; ++n) {
         uint32_t af[4];   // features 16 n + g and + 8 of keys 2 t, 2 t + 1, then of keys 2 t + 8, 2 t + 9
         const int ch = 2 * n + ((lane >> 3) & 1);
-        ldmatrix_x4_trans(af, smem_u32(vt + (ch >> 3) * PR_BLOCK + row * 128 + (((ch & 7) ^ (row & 7)) << 4)));
+        ldmatrix_x4_trans(af, smem_u32(vt + (ch >> 3) * hb * PR_BLOCK + row * 128 + (((ch & 7) ^ (row & 7)) << 4)));
 #pragma unroll
         for (int m = 0; m < RQ; ++m) mma16816<TM>(o[m][n], af[0], af[1], af[2], af[3], pb[m][0], pb[m][1]);
       }
@@ -706,9 +715,13 @@ static int rows_blocks(const PopeShape& s) {
   return (int)((rows + 8 * rows_rq(s) - 1) / (8 * rows_rq(s)));
 }
 // warps of a CTA: as many as the registers of their outputs (32 per group of eight rows) allow
-constexpr int rows_nw(bool q8, int rq) { return rq == 4 ? 8 : q8 ? 16 : 12; }
-// Key heads of a CTA: two share the copies of the cosines and sines, which at 8 bits are as many bytes as K and V or twice that.
-static int rows_hb(const PopeShape& s, int store) { return store != POPE_STORE_16 && s.Hk % 2 == 0 ? 2 : 1; }
+constexpr int rows_nw(int rq) { return rq == 4 ? 8 : rq == 2 ? 12 : 16; }
+// Key heads of a CTA: they share the copies of the cosines and sines, which at 8 bits are as many bytes as K and V or twice that.
+static int rows_hb(const PopeShape& s, int store) {
+  const int pairs = rows_nw(rows_rq(s)) / PR_WPT;
+  if (store == POPE_STORE_16) return 1;
+  return s.Hk % 4 == 0 && pairs % 4 == 0 ? 4 : s.Hk % 2 == 0 && pairs % 2 == 0 ? 2 : 1;
+}
 
 // Key ranges per unit: whole waves of one CTA per SM times a CTA's tiles plus what it costs beside them.
 static int rows_split(const PopeShape& s, int store) {
@@ -741,7 +754,7 @@ size_t paged_rows_workspace(const PopePagedAttnArgs& a) { return rows_ws(a.shape
 
 template <typename T, int STORE, int D, int RQ> static cudaError_t paged_rows_t(const PopePagedAttnArgs& a, cudaStream_t st) {
   constexpr bool Q8 = STORE != POPE_STORE_16;
-  constexpr int NW = rows_nw(Q8, RQ), RB = 8 * RQ, FPI = Q8 ? 64 : 32, DP = (D + FPI - 1) / FPI * FPI, KBLK = (D * (Q8 ? 1 : 2) + 127) / 128;
+  constexpr int NW = rows_nw(RQ), RB = 8 * RQ, FPI = Q8 ? 64 : 32, DP = (D + FPI - 1) / FPI * FPI, KBLK = (D * (Q8 ? 1 : 2) + 127) / 128;
   const PopeShape& s = a.shape;
   const PopePagedKV& kv = a.cache.kv;
   const RowsWs ws = rows_ws(s, STORE);
@@ -755,7 +768,6 @@ template <typename T, int STORE, int D, int RQ> static cudaError_t paged_rows_t(
   p.npg_smem = (int)((int64_t)((tiles + p.nsplit - 1) / p.nsplit) * PR_TILE / kv.page_size) + 2;
   p.scale_log2 = a.softmax_scale * LOG2E;
   p.page_table = kv.page_table, p.seq_lens = kv.seq_lens, p.counts = a.counts;
-  p.k_scales = a.cache.k_scales, p.v_scales = a.cache.v_scales;
   p.freqs = a.embed.freqs, p.bias = a.embed.bias, p.sfn = a.embed.sf.n, p.bias_sh = a.embed.bias_stride_h;
   p.q = a.q, p.out = a.out, p.sq = Strides(a.sq), p.so = Strides(a.so), p.lse = a.lse;
   p.done = reinterpret_cast<unsigned int*>(base);
@@ -763,19 +775,15 @@ template <typename T, int STORE, int D, int RQ> static cudaError_t paged_rows_t(
   p.status = tc_status_ptr();
   if (!p.status) return cudaErrorInvalidSymbol;
 
-  CUtensorMap mk, mv, mt;
-  const bool bf16 = s.dtype == POPE_BF16;
-  const int64_t row = s.d, head = row * kv.page_size, page = head * s.Hk;
-  bool ok;
-  if constexpr (Q8) {
-    ok = make_code_tmap(&mk, kv.k_pages, s.d, kv.page_size, s.Hk, kv.num_pages, row, head, page, PR_TILE) &&
-         make_code_tmap(&mv, kv.v_pages, s.d, kv.page_size, s.Hk, kv.num_pages, row, head, page, PR_TILE);
-  } else {
-    ok = make_wide_tmap(&mk, kv.k_pages, bf16, s.d, kv.page_size, s.Hk, kv.num_pages, row, head, page, PR_TILE) &&
-         make_wide_tmap(&mv, kv.v_pages, bf16, s.d, kv.page_size, s.Hk, kv.num_pages, row, head, page, PR_TILE);
-  }
-  // (without rotated features nothing is copied through the third map)
-  ok = ok && (s.r > 0 ? make_wide_tmap(&mt, table, false, s.r, s.Nk, 2, 1, s.r, (int64_t)s.Nk * s.r, 0, PR_TILE) : (mt = mk, true));
+  CUtensorMap mk, mv, mt, mks, mvs;
+  const int row_bytes = Q8 ? s.d : 2 * s.d;
+  bool ok = make_page_tmap(&mk, kv.k_pages, row_bytes, kv.page_size, s.Hk, kv.num_pages, PR_TILE, p.hb) &&
+            make_page_tmap(&mv, kv.v_pages, row_bytes, kv.page_size, s.Hk, kv.num_pages, PR_TILE, p.hb);
+  // (the maps of what a call does not have are not used)
+  ok = ok && (s.r > 0 ? make_trig_tmap(&mt, table, s.Nk, s.r, PR_TILE) : (mt = mk, true));
+  ok = ok && (Q8 ? make_page_tmap(&mks, a.cache.k_scales, 0, kv.page_size, s.Hk, kv.num_pages, PR_TILE, p.hb) &&
+                       make_page_tmap(&mvs, a.cache.v_scales, 0, kv.page_size, s.Hk, kv.num_pages, PR_TILE, p.hb)
+                 : (mks = mvs = mk, true));
   if (!ok) return cudaErrorNotSupported;
 
   const int tblk = (s.r + 63) / 64, RP = (s.r + FPI - 1) / FPI * FPI, rings = NW / (PR_WPT * p.hb);
@@ -795,10 +803,10 @@ template <typename T, int STORE, int D, int RQ> static cudaError_t paged_rows_t(
   // behind the table kernel, which also zeroes the counters
   if (s.r > 0) {
     if ((e = launch_trig_tables(a.embed, s.Nk, s.r, nullptr, nullptr, table, table + (size_t)s.Nk * s.r, st, 1, 1, p.done, (int)units)) != cudaSuccess) return e;
-    return launch_dependent(kernel, grid, block, smem, st, p, mk, mv, mt);
+    return launch_dependent(kernel, grid, block, smem, st, p, mk, mv, mt, mks, mvs);
   }
   if (p.nsplit > 1 && (e = cudaMemsetAsync(p.done, 0, units * sizeof(unsigned int), st)) != cudaSuccess) return e;
-  kernel<<<grid, block, smem, st>>>(p, mk, mv, mt);
+  kernel<<<grid, block, smem, st>>>(p, mk, mv, mt, mks, mvs);
   return cudaGetLastError();
 }
 template <typename T, int STORE, int D> static cudaError_t paged_rows_q(const PopePagedAttnArgs& a, cudaStream_t st) {

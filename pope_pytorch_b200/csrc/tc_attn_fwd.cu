@@ -69,7 +69,7 @@ static TmapEncodeFn tmap_encoder() {
 // dummy (multiple of 16 bytes, increasing); an axis with more entries must come with a usable stride.
 static bool tmap_4d(CUtensorMap* out, CUtensorMapDataType dt, int esz, const void* base, int cols, int rows, int heads,
                     int batch, int64_t sn, int64_t sh, int64_t sb, int box_cols, int box_rows, CUtensorMapSwizzle swz,
-                    CUtensorMapL2promotion promo = CU_TENSOR_MAP_L2_PROMOTION_L2_128B) {
+                    CUtensorMapL2promotion promo = CU_TENSOR_MAP_L2_PROMOTION_L2_128B, int box_heads = 1) {
   TmapEncodeFn encode = tmap_encoder();
   if (!encode) return false;
   cuuint64_t dims[4] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)batch};
@@ -82,7 +82,7 @@ static bool tmap_4d(CUtensorMap* out, CUtensorMapDataType dt, int esz, const voi
   for (int i = 0; i < 3; ++i)
     if (strides[i] % 16 != 0) return false;
   if ((reinterpret_cast<uintptr_t>(base) & 15) != 0) return false;
-  cuuint32_t box[4] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
+  cuuint32_t box[4] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, (cuuint32_t)box_heads, 1}, estr[4] = {1, 1, 1, 1};
   return encode(out, dt, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz, promo,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -100,9 +100,21 @@ bool make_wide_tmap(CUtensorMap* out, const void* base, bool is_bf16, int d, int
                  batch, sn, sh, sb, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-// rows of one-byte codes cut into boxes of 128 bytes x box_rows rows, 128-byte swizzled
-bool make_code_tmap(CUtensorMap* out, const void* base, int d, int rows, int heads, int batch, int64_t sn, int64_t sh, int64_t sb, int box_rows) {
-  return tmap_4d(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, d, rows, heads, batch, sn, sh, sb, 128, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+// a paged pool, (page, key head, row, byte), cut into boxes of 128 bytes x box_rows rows x box_heads heads, 128-byte swizzled (a box reaches
+// past shorter rows, which arrive as zeros there); with row_bytes 0 its fp32 row scales, (page, key head, row), in plain boxes
+bool make_page_tmap(CUtensorMap* out, const void* base, int row_bytes, int page_size, int heads, int pages, int box_rows, int box_heads) {
+  if (row_bytes == 0)
+    return tmap_4d(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, page_size, heads, pages, 1, page_size, (int64_t)page_size * heads, 0, box_rows, box_heads,
+                   CU_TENSOR_MAP_SWIZZLE_NONE);
+  const int64_t head = (int64_t)row_bytes * page_size;
+  return tmap_4d(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, row_bytes, page_size, heads, pages, row_bytes, head, head * heads, 128, box_rows,
+                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, box_heads);
+}
+
+// the fp16 cos and sin tables, (cos / sin, position, feature), cut into boxes of 64 features x box_rows positions x both, 128-byte swizzled
+bool make_trig_tmap(CUtensorMap* out, const void* table, int n, int r, int box_rows) {
+  return tmap_4d(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, table, r, n, 2, 1, r, (int64_t)n * r, 0, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B,
+                 CU_TENSOR_MAP_L2_PROMOTION_L2_128B, 2);
 }
 
 // An operand image ([tile][chunk][64 rows x 16 B]) seen as (1 KB run, tile, chunk): a box of (1 KB, 2 tiles, all chunks)

@@ -135,8 +135,11 @@ inline ExpandJob expand_job(const void* x, const PopeStride3& sx, int batch, int
 // 16-bit (feature, row, head, batch) view cut into boxes of 64 features (128-byte rows) x box_rows rows, 128-byte swizzled
 bool make_wide_tmap(CUtensorMap* out, const void* base, bool is_bf16, int d, int rows, int heads, int batch, int64_t sn,
                     int64_t sh, int64_t sb, int box_rows);
-// one-byte codes, boxes of 128 bytes x box_rows rows, 128-byte swizzled (a box reaches past shorter rows, which arrive as zeros there)
-bool make_code_tmap(CUtensorMap* out, const void* base, int d, int rows, int heads, int batch, int64_t sn, int64_t sh, int64_t sb, int box_rows);
+// a paged pool in boxes of 128 bytes x box_rows rows x box_heads key heads, 128-byte swizzled (a box reaches past shorter rows, which arrive as
+// zeros there); row_bytes 0: its fp32 row scales in boxes of box_rows x box_heads
+bool make_page_tmap(CUtensorMap* out, const void* base, int row_bytes, int page_size, int heads, int pages, int box_rows, int box_heads);
+// fp16 cos / sin tables [2][n][r] in boxes of 64 features x box_rows positions x both, 128-byte swizzled
+bool make_trig_tmap(CUtensorMap* out, const void* table, int n, int r, int box_rows);
 // an operand image as (1 KB run, tile, chunk): box = (1 KB, 2 tiles, all chunks) = one resident 128-row operand
 bool make_image_tmap(CUtensorMap* out, const void* img, int64_t ntiles, int chunks);
 // ch / sh = fp16 cos / sin of the phase table, [positions][r].  All jobs share d and the dtype; one launch.
