@@ -340,6 +340,7 @@ int pope_b200_attn_paged(const PopePagedAttnArgs* a, void* stream) {
   if (rc == POPE_OK) rc = check_store(a->cache, a->shape.B);
   if (rc != POPE_OK) return rc;
   if (!a->q || !a->out) return POPE_ERR_BAD_ARG;
+  if (!rows_on_16_bytes(a->out, a->so)) return POPE_ERR_MISALIGNED;
   if (!pope::attn_paged_supported(*a)) return POPE_ERR_UNSUPPORTED;
   const size_t need = pope::attn_paged_workspace(*a);
   if (need > 0 && (!a->workspace || a->workspace_bytes < need)) return POPE_ERR_WORKSPACE;

@@ -163,7 +163,6 @@ __global__ void __launch_bounds__(32 * NW, 1)
   constexpr int NI = (D + FPI - 1) / FPI, DP = NI * FPI;
   constexpr int NH = VL / 8;
   constexpr int KBLK = (D * (Q8 ? 1 : 2) + 127) / 128;     // 128-byte blocks of a row
-  constexpr int EPB = Q8 ? 128 : 64;                       // elements of one
   constexpr int NT = D / 16;                               // output feature tiles
   constexpr int FL = D / 8;                                // 8-bit V: neighbouring features of a lane
 

@@ -1,0 +1,662 @@
+// Attention of a chunk of new tokens over a paged cache on the Blackwell tensor cores (tcgen05 + TMEM), sm_100a only: for chunks whose rows per
+// key head are many (paged_rows.cu takes the others).
+//
+// The query rows that share a key head are packed, row = token * group + head, and a CTA owns 128 of them: the heads of a group read K and V
+// once.  Three launches:
+//   tables : fp16 cos / sin rows of the positions
+//   images : K' = [a cos | plain | a sin] of every (sequence, key head), read through the page table (8-bit codes are turned into values here),
+//            in 128-row tiles in the order in which the tensor core reads them; every row block sweeps the keys, so they are expanded once.
+//            Of a cache that holds 8 bits also V, as 16-bit rows.
+//   sweep  : S = Q' K'^T with Q' in tensor memory, online softmax, O += P V with P in tensor memory, 128 keys a step; K' by one bulk copy, V by
+//            tensor-map boxes from the pages.  Small grids are cut along the keys; the CTA that finishes a row block last merges its parts.
+// Row i of sequence b stands at p = len - count + i and sees the keys up to p: a step whose last key is not beyond the first row's position
+// needs no mask.
+#include <algorithm>
+#include <type_traits>
+
+#include "kernels.h"
+#include "paged.cuh"
+
+namespace pope {
+
+// ---- images --------------------------------------------------------------------------------------------
+struct PagedImageP {
+  PagedPtrs c;
+  int B, Nk, r, RP;          // RP: r rounded up to 16, columns r .. of the sines are zero
+  const __half *ch, *sh;     // fp16 cos / sin, [Nk][r]
+  const float* bias;
+  int64_t bias_sh;
+  uint8_t* kimg;             // [unit][128-row tile][chunk][128 rows][16 B]
+  void* vrows;               // 8-bit stores: [unit][rows][D]
+  int tiles;                 // 64-row tiles of a unit's image
+  unsigned int* done;
+  int ndone;
+};
+
+// One 64-row tile per CTA (the rows of a tile lie in one page).  256 threads: a thread keeps one 16-byte column of the rows it touches.
+template <typename T, int STORE, int D>
+__global__ void __launch_bounds__(256) paged_image_kernel(PagedImageP p) {
+  constexpr bool Q8 = STORE != POPE_STORE_16;
+  constexpr int DC = D / 8, RPP = 256 / DC, NIT = (IMAGE_ROWS + RPP - 1) / RPP;
+  extern __shared__ __align__(16) uint8_t stage[];
+  const int tid = threadIdx.x, tile = blockIdx.x, u = blockIdx.y, b = u / p.c.Hk, hk = u % p.c.Hk, r = p.r;
+  pdl_wait();
+  pdl_trigger();
+  if (blockIdx.x == 0 && blockIdx.y == 0)
+    for (int i = tid; i < p.ndone; i += 256) p.done[i] = 0;
+  const int len = max(0, min(p.c.seq_lens[b], p.Nk)), key0 = tile * IMAGE_ROWS;
+  if (key0 >= (len + 127) / 128 * 128) return;   // (tiles come in pairs)
+  const int rows = max(0, min(IMAGE_ROWS, len - key0));
+  __shared__ int64_t row0_s;
+  if (tid == 0) row0_s = rows > 0 ? paged_row(p.c, b, hk, key0) : 0;
+  const int KC = DC + p.RP / 8;
+  float* bias_c = reinterpret_cast<float*>(stage + KC * CS64);
+  float* bias_s = bias_c + r;
+  for (int i = tid; i < r; i += 256) sincos_reduced(p.bias[hk * p.bias_sh + i], &bias_s[i], &bias_c[i]);
+  __syncthreads();
+  const int64_t row0 = max(row0_s, (int64_t)0);   // (a page outside the pool: reported, another one read)
+  const int c = tid % DC, first = tid / DC;
+  const bool active = first < RPP, rotated = c * 8 < r;
+  uint4 raw[NIT];
+  float scale[NIT];
+  auto load = [&](const uint8_t* pool, const float* scales) {
+#pragma unroll
+    for (int it = 0; it < NIT; ++it) {
+      const int row = first + it * RPP;
+      raw[it] = make_uint4(0, 0, 0, 0), scale[it] = 0.f;
+      if (!active || row >= rows) continue;
+      if constexpr (Q8) {
+        const uint2 x = *reinterpret_cast<const uint2*>(pool + (row0 + row) * D + c * 8);
+        raw[it].x = x.x, raw[it].y = x.y, scale[it] = scales[row0 + row];
+      } else {
+        raw[it] = *reinterpret_cast<const uint4*>(pool + ((row0 + row) * D + c * 8) * 2);
+      }
+    }
+  };
+  auto values = [&](int it, float2 (&x)[4]) {
+    if constexpr (Q8) {
+      float lo[4], hi[4];
+      codes_to_f32<STORE>(raw[it].x, lo), codes_to_f32<STORE>(raw[it].y, hi);
+      const float s = scale[it];
+      x[0] = make_float2(lo[0] * s, lo[1] * s), x[1] = make_float2(lo[2] * s, lo[3] * s);
+      x[2] = make_float2(hi[0] * s, hi[1] * s), x[3] = make_float2(hi[2] * s, hi[3] * s);
+    } else {
+      x[0] = unpack2<T>(raw[it].x), x[1] = unpack2<T>(raw[it].y), x[2] = unpack2<T>(raw[it].z), x[3] = unpack2<T>(raw[it].w);
+    }
+  };
+  load(p.c.k, p.c.k_scales);
+  if (rotated) {
+    float cb[8], sb[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) cb[e] = bias_c[c * 8 + e], sb[e] = bias_s[c * 8 + e];
+    uint4 cq[NIT], sq[NIT];
+#pragma unroll
+    for (int it = 0; it < NIT; ++it) {
+      const int row = first + it * RPP;
+      cq[it] = sq[it] = make_uint4(0, 0, 0, 0);   // (rows behind the last key become zeros)
+      if (active && row < rows) {
+        cq[it] = *reinterpret_cast<const uint4*>(p.ch + (int64_t)(key0 + row) * r + c * 8);
+        sq[it] = *reinterpret_cast<const uint4*>(p.sh + (int64_t)(key0 + row) * r + c * 8);
+      }
+    }
+#pragma unroll
+    for (int it = 0; it < NIT; ++it) {
+      const int row = first + it * RPP;
+      if (!active || row >= IMAGE_ROWS) continue;
+      const uint32_t cw[4] = {cq[it].x, cq[it].y, cq[it].z, cq[it].w}, sw[4] = {sq[it].x, sq[it].y, sq[it].z, sq[it].w};
+      float2 x[4];
+      values(it, x);
+      uint32_t o1[4], o2[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 cv = unpack2<__half>(cw[e]), sv = unpack2<__half>(sw[e]);   // cos(f + b), sin(f + b)
+        const float c0 = cv.x * cb[2 * e] - sv.x * sb[2 * e], s0 = sv.x * cb[2 * e] + cv.x * sb[2 * e];
+        const float c1 = cv.y * cb[2 * e + 1] - sv.y * sb[2 * e + 1], s1 = sv.y * cb[2 * e + 1] + cv.y * sb[2 * e + 1];
+        const float a0 = softplus_fast(x[e].x), a1 = softplus_fast(x[e].y);
+        o1[e] = pack2<T>(a0 * c0, a1 * c1), o2[e] = pack2<T>(a0 * s0, a1 * s1);
+      }
+      *reinterpret_cast<uint4*>(stage + c * CS64 + row * 16) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
+      *reinterpret_cast<uint4*>(stage + (DC + c) * CS64 + row * 16) = make_uint4(o2[0], o2[1], o2[2], o2[3]);
+    }
+  } else {
+#pragma unroll
+    for (int it = 0; it < NIT; ++it) {
+      const int row = first + it * RPP;
+      if (!active || row >= IMAGE_ROWS) continue;
+      uint4 o = raw[it];
+      if constexpr (Q8) {
+        float2 x[4];
+        values(it, x);
+        o = make_uint4(pack2<T>(x[0].x, x[0].y), pack2<T>(x[1].x, x[1].y), pack2<T>(x[2].x, x[2].y), pack2<T>(x[3].x, x[3].y));
+      }
+      *reinterpret_cast<uint4*>(stage + c * CS64 + row * 16) = o;
+      if (c * 8 < p.RP) *reinterpret_cast<uint4*>(stage + (DC + c) * CS64 + row * 16) = make_uint4(0, 0, 0, 0);
+    }
+  }
+  if constexpr (Q8) {   // V of the same rows, zeros behind the last key
+    load(p.c.v, p.c.v_scales);
+#pragma unroll
+    for (int it = 0; it < NIT; ++it) {
+      const int row = first + it * RPP;
+      if (!active || row >= IMAGE_ROWS) continue;
+      float2 x[4];
+      values(it, x);
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.vrows) + ((int64_t)u * p.tiles * IMAGE_ROWS + key0 + row) * D + c * 8) =
+          make_uint4(pack2<T>(x[0].x, x[0].y), pack2<T>(x[1].x, x[1].y), pack2<T>(x[2].x, x[2].y), pack2<T>(x[3].x, x[3].y));
+    }
+  }
+  __syncthreads();
+  // the image leaves in its own byte order, coalesced: tiles 2 t and 2 t + 1 share a 128-row tile
+  uint8_t* out = p.kimg + (((int64_t)u * p.tiles + tile) >> 1) * ((int64_t)2 * IMAGE_ROWS * KC * 16) + (tile & 1) * (IMAGE_ROWS * 16);
+  for (int i = tid; i < IMAGE_ROWS * KC; i += 256) {
+    const int cc = i / IMAGE_ROWS, row = i - cc * IMAGE_ROWS;
+    *reinterpret_cast<uint4*>(out + cc * (2 * IMAGE_ROWS * 16) + row * 16) = *reinterpret_cast<const uint4*>(stage + cc * CS64 + row * 16);
+  }
+}
+
+// ---- sweep -----------------------------------------------------------------------------------------------
+struct PagedSweepP {
+  int H, Hk, G, Nq, Nk, r, RP, nsplit, blocks, tiles;   // blocks: row blocks per unit; tiles: 64-row tiles of a unit's image
+  int page_size, max_pages, num_pages, q_wide;          // q_wide: rows of q on 16-byte boundaries
+  float scale_log2;                                     // its magnitude; the sign sits in Q'
+  uint32_t q_sign;
+  const int32_t *page_table, *seq_lens, *counts;
+  const void* q;
+  void* o;
+  float* lse;
+  Strides sq, so;
+  const uint8_t* kimg;
+  const __half *ch, *sh;
+  float *part_o, *part_ml;   // [row block][split][128][D], [row block][split][128][max (log2 units), sum]
+  unsigned int *done, *status;
+};
+
+constexpr int PS_ROWS = 128, PS_KEYS = 128;
+constexpr int PS_SM_WARPS = 8;                     // softmax warps: two threads per query row
+constexpr int PS_KLOAD = 8, PS_S = 9, PS_PV = 10, PS_VLOAD = 11;
+constexpr int PS_THREADS = 32 * 12;
+constexpr uint32_t PS_TS = 128, PS_TO = 384;       // first TMEM column of the S / P buffers and of O (Q' starts at 0)
+constexpr int PS_MAX_SPLIT = 32;
+enum {
+  PS_KFULL = 0,    // [2] K' tile landed
+  PS_KFREE = 2,    // [2] S of the tile has completed
+  PS_PVDONE = 4,   // [2] O += P V of the tile has completed: S / P buffer free
+  PS_SFULL = 6,    // [2] the scores are in TMEM
+  PS_PFULL = 8,    // [2] the probabilities are in TMEM (and V's rows behind the last key are zero)
+  PS_QFULL = 10,
+  PS_ODONE = 11,
+  PS_VFULL = 12,   // [2] V tile landed
+  PS_VFREE = 14,   // [2] O += P V of the tile has completed: V stage free
+  PS_COUNT = 16
+};
+
+template <typename T, int D, bool Q8>
+__global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP p, const __grid_constant__ CUtensorMap tmap_v) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  constexpr int VB = (D + 63) / 64, VBUF = VB * PS_KEYS * 128;   // V stage: [64-feature block][128 keys][128 B], swizzled
+  constexpr int CSV = PS_KEYS * 16;
+  const int KD = D + p.RP, KSTEPS = KD >> 4, KBUF = PS_KEYS * KD * 2;
+  uint8_t* Ks = smem;
+  uint8_t* Vs = Ks + 2 * KBUF;                                    // (KBUF is a multiple of 4 KB)
+  float* xch = reinterpret_cast<float*>(Vs + 2 * VBUF);           // [2 step parities][2 parts][128 rows] row maxima
+  uint64_t* bars = reinterpret_cast<uint64_t*>(xch + 4 * PS_ROWS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + PS_COUNT);
+  unsigned int* last_s = tmem_slot + 1;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (warp == PS_S) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  if (tid == 0) {
+    for (int i = 0; i < PS_COUNT; ++i) mbar_init(&bars[i], i == PS_PFULL || i == PS_PFULL + 1 || i == PS_QFULL ? PS_SM_WARPS : 1);
+    mbar_init_fence();
+  }
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  // unit (sequence, key head), row block (late ones, which see more keys, first), key range
+  const int split = blockIdx.x % p.nsplit, ub = blockIdx.x / p.nsplit, u = ub / p.blocks, rb = p.blocks - 1 - ub % p.blocks;
+  const int b = u / p.Hk, hk = u % p.Hk;
+  const int len = max(0, min(p.seq_lens[b], p.Nk)), cnt = p.counts ? max(0, min(p.counts[b], p.Nq)) : p.Nq;
+  const int rows = min(PS_ROWS, cnt * p.G - rb * PS_ROWS);                            // of this block that are queries
+  const int first_pos = len - cnt + rb * PS_ROWS / p.G;                               // position of the first one
+  const int kend = rows > 0 ? max(0, min(len, len - cnt + (rb * PS_ROWS + rows - 1) / p.G + 1)) : 0;
+  const int tiles_all = (kend + PS_KEYS - 1) / PS_KEYS;
+  const int t0 = (int)((int64_t)tiles_all * split / p.nsplit), T_tiles = (int)((int64_t)tiles_all * (split + 1) / p.nsplit) - t0;
+  bool failed = false;
+
+  if (warp == PS_KLOAD) {
+    if (lane == 0) {
+      const uint8_t* kimg = p.kimg + ((int64_t)u * (p.tiles / 2) + t0) * KBUF;
+      int j = 0;
+      for (; j < T_tiles; ++j) {
+        const int buf = j & 1;
+        if (j >= 2) failed = !mbar_wait(&bars[PS_KFREE + buf], ((j - 2) >> 1) & 1, WAIT_LIMIT);
+        if (failed) break;
+        mbar_expect_tx(&bars[PS_KFULL + buf], KBUF);
+        bulk_load(Ks + buf * KBUF, kimg + (int64_t)j * KBUF, KBUF, &bars[PS_KFULL + buf]);
+      }
+      if (failed) drain_copies(&bars[PS_KFULL], 2, j - 2, j);
+    }
+    __syncwarp();
+  } else if (warp == PS_VLOAD) {
+    int page = 0;   // lane l: the page of half tile (j & ~15) * 2 + l
+    for (int j = 0; j < T_tiles; ++j) {
+      const int buf = j & 1, key0 = (t0 + j) * PS_KEYS;
+      if (!Q8 && (j & 15) == 0) {
+        const int key = key0 + lane * 64, lp = key / p.page_size;
+        page = 0;
+        if (key < kend) {
+          page = lp < p.max_pages ? p.page_table[(int64_t)b * p.max_pages + lp] : -1;
+          if (page < 0 || page >= p.num_pages) page = 0, atomicOr(p.status, 2u);
+        }
+      }
+      const int pg0 = __shfl_sync(0xffffffffu, page, (j & 15) * 2), pg1 = __shfl_sync(0xffffffffu, page, (j & 15) * 2 + 1);
+      if (lane == 0) {
+        if (j >= 2) failed = !mbar_wait(&bars[PS_VFREE + buf], ((j - 2) >> 1) & 1, WAIT_LIMIT);
+        if (failed) {
+          drain_copies(&bars[PS_VFULL], 2, j - 2, j);
+        } else {
+          const int halves = Q8 || key0 + 64 < kend ? 2 : 1;   // (a second half without keys may have no page)
+          mbar_expect_tx(&bars[PS_VFULL + buf], halves * VB * 64 * 128);
+          for (int i = 0; i < halves; ++i) {
+            const int key = key0 + 64 * i;
+#pragma unroll
+            for (int c = 0; c < VB; ++c)
+              tma_load_4d(Vs + buf * VBUF + c * (PS_KEYS * 128) + i * (64 * 128), &tmap_v, &bars[PS_VFULL + buf], c * 64, Q8 ? key : key % p.page_size, hk,
+                          Q8 ? b : i ? pg1 : pg0);
+          }
+        }
+      }
+      failed = __shfl_sync(0xffffffffu, (int)failed, 0) != 0;
+      if (failed) break;
+    }
+  } else if (warp == PS_S) {
+    if (lane == 0) {
+      const uint32_t idesc = instr_desc(TcFmt<T>::fmt, PS_ROWS, PS_KEYS, false, false);
+      const uint32_t ks_addr = smem_u32(Ks);
+      if (!mbar_wait(&bars[PS_QFULL], 0, WAIT_LIMIT)) failed = true;
+      for (int j = 0; j < T_tiles && !failed; ++j) {
+        const int buf = j & 1;
+        failed = !mbar_wait(&bars[PS_KFULL + buf], (j >> 1) & 1, WAIT_LIMIT);
+        if (j >= 2 && !failed) failed = !mbar_wait(&bars[PS_PVDONE + buf], ((j - 2) >> 1) & 1, WAIT_LIMIT);
+        if (failed) break;
+        fence_after_sync();
+        const uint32_t d = tmem + PS_TS + buf * PS_KEYS;
+        const uint64_t bd = smem_desc(ks_addr + buf * KBUF, CSV, 128);
+        uint32_t blo = desc_lo(bd), at = tmem;
+#pragma unroll 4
+        for (int ks = 0; ks < KSTEPS; ++ks) {
+          mma_ts_lh(d, at, blo, desc_hi(bd), idesc, ks > 0 ? 1u : 0u);
+          at += 8, blo += (2 * CSV) >> 4;
+        }
+        mma_commit(&bars[PS_SFULL + buf]);
+        mma_commit(&bars[PS_KFREE + buf]);
+      }
+    }
+    __syncwarp();
+  } else if (warp == PS_PV) {
+    if (lane == 0) {
+      const uint32_t idesc = instr_desc(TcFmt<T>::fmt, PS_ROWS, D, false, true);
+      const uint32_t vs_addr = smem_u32(Vs);
+      for (int j = 0; j < T_tiles && !failed; ++j) {
+        const int buf = j & 1;
+        failed = !mbar_wait(&bars[PS_VFULL + buf], (j >> 1) & 1, WAIT_LIMIT);
+        if (!failed) failed = !mbar_wait(&bars[PS_PFULL + buf], (j >> 1) & 1, WAIT_LIMIT);
+        if (failed) break;
+        fence_after_sync();
+        const uint32_t a = tmem + PS_TS + buf * PS_KEYS;
+        // B = V, MN-major: 64-feature blocks 16 KB apart, 8-key groups 1 KB apart, 2 KB per 16 keys
+        const uint64_t bd = smem_desc_sw128(vs_addr + buf * VBUF, PS_KEYS * 128, 1024);
+#pragma unroll
+        for (int ks = 0; ks < PS_KEYS / 16; ++ks)   // P of keys [64 t, 64 t + 64) sits in the first 32 columns of part t
+          mma_ts_lh(tmem + PS_TO, a + (ks * 16 / 64) * 64 + (ks * 16 % 64) / 2, desc_lo(bd) + ks * (2048 >> 4), desc_hi(bd), idesc, (j > 0 || ks > 0) ? 1u : 0u);
+        if (j == T_tiles - 1) mma_commit(&bars[PS_ODONE]);
+        mma_commit(&bars[PS_PVDONE + buf]);
+        mma_commit(&bars[PS_VFREE + buf]);
+      }
+    }
+    __syncwarp();
+  } else {
+    // =============================== softmax: two threads per query row ==========================
+    const int rloc = tid & 127, part = tid >> 7;
+    const int rho = rb * PS_ROWS + rloc, tok = rho / p.G, head = hk + (rho - tok * p.G) * p.Hk, pos = len - cnt + tok;
+    const bool live = rloc < rows && pos >= 0;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const int row_bar = 1 + (warp & 3);   // named barrier of the two warps that share 32 rows
+    auto row_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(row_bar) : "memory"); };
+    auto all_sync = []() { asm volatile("bar.sync 5, %0;" ::"n"(32 * PS_SM_WARPS) : "memory"); };
+    {
+      // Q' = [a cos f | plain | a sin f], expanded here from q and the fp16 tables straight into tensor memory; rows that are no queries are zero
+      constexpr int DC = D >> 3;
+      const T* qrow = static_cast<const T*>(p.q) + b * p.sq.b + head * p.sq.h + (int64_t)tok * p.sq.n;
+      const int64_t trow = (int64_t)pos * p.r;
+      for (int c = part; c < DC; c += 2) {
+        uint32_t rw[4] = {0, 0, 0, 0};
+        if (live && p.q_wide) {
+          const uint4 raw = *reinterpret_cast<const uint4*>(qrow + c * 8);
+          rw[0] = raw.x, rw[1] = raw.y, rw[2] = raw.z, rw[3] = raw.w;
+        } else if (live) {
+          const uint16_t* q16 = reinterpret_cast<const uint16_t*>(qrow + c * 8);
+          for (int e = 0; e < 4; ++e) rw[e] = q16[2 * e] | (uint32_t)q16[2 * e + 1] << 16;
+        }
+        if (c * 8 < p.r) {
+          uint4 cq = make_uint4(0, 0, 0, 0), sq = cq;
+          if (live) {
+            cq = *reinterpret_cast<const uint4*>(p.ch + trow + c * 8);
+            sq = *reinterpret_cast<const uint4*>(p.sh + trow + c * 8);
+          }
+          const uint32_t cw[4] = {cq.x, cq.y, cq.z, cq.w}, sw[4] = {sq.x, sq.y, sq.z, sq.w};
+          uint32_t o1[4], o2[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 xv = unpack2<T>(rw[e]), cv = unpack2<__half>(cw[e]), sv = unpack2<__half>(sw[e]);
+            const float a0 = live ? softplus_fast(xv.x) : 0.f, a1 = live ? softplus_fast(xv.y) : 0.f;
+            o1[e] = pack2<T>(a0 * cv.x, a1 * cv.y) ^ p.q_sign, o2[e] = pack2<T>(a0 * sv.x, a1 * sv.y) ^ p.q_sign;
+          }
+          tmem_st4(tmem + lane_base + c * 4, o1[0], o1[1], o1[2], o1[3]);
+          tmem_st4(tmem + lane_base + (DC + c) * 4, o2[0], o2[1], o2[2], o2[3]);
+        } else {
+          tmem_st4(tmem + lane_base + c * 4, rw[0] ^ p.q_sign, rw[1] ^ p.q_sign, rw[2] ^ p.q_sign, rw[3] ^ p.q_sign);
+          if (c * 8 < p.RP) tmem_st4(tmem + lane_base + (DC + c) * 4, 0, 0, 0, 0);
+        }
+      }
+      tmem_st_wait();
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[PS_QFULL]);
+    }
+    float m_run = -CUDART_INF_F, l_run = 0.f;
+    const int limit = live ? min(pos, kend - 1) : -1;   // last key that this row sees
+
+    for (int j = 0; j < T_tiles; ++j) {
+      const int buf = j & 1, key0 = (t0 + j) * PS_KEYS, n0 = key0 + part * 64;   // first key of this thread's columns
+      const bool all_vis = key0 + PS_KEYS <= min(kend, first_pos + 1);   // (the same for all threads; rows that are no queries are dropped at the end)
+      const int lim = limit - n0;
+      const uint64_t vis = lim >= 63 ? ~0ull : (lim < 0 ? 0ull : ((2ull << lim) - 1ull));
+      if (!failed) failed = !mbar_wait(&bars[PS_SFULL + buf], (j >> 1) & 1, WAIT_LIMIT);
+      fence_after_sync();
+      const uint32_t s_addr = tmem + lane_base + PS_TS + buf * PS_KEYS + part * 64;
+      uint32_t sv[2][32];
+      tmem_ld32(s_addr, sv[0]);
+      tmem_ld32(s_addr + 32, sv[1]);
+      tmem_ld_wait();
+      float m4[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+      if (all_vis) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(sv[q][i]), __uint_as_float(sv[q][i + 1]));
+      } else {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const uint32_t vq = (uint32_t)(vis >> (32 * q));
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if ((vq >> i) & 1u) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(sv[q][i]));
+        }
+      }
+      float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+      xch[(buf * 2 + part) * PS_ROWS + rloc] = mx;
+      row_sync();
+      mx = fmaxf(mx, xch[(buf * 2 + 1 - part) * PS_ROWS + rloc]);
+      const float m_new = fmaxf(m_run, mx == -CUDART_INF_F ? mx : mx * p.scale_log2);
+      // a stale maximum is kept while it is within 2^8 of the true one
+      const bool need = m_new > m_run + 8.f;
+      float alpha = 1.f;
+      if (need) {
+        alpha = ex2_approx(m_run - m_new);
+        l_run *= alpha;
+        m_run = m_new;
+      }
+      if (j > 0 && __any_sync(0xffffffffu, need)) {
+        if (!failed) failed = !mbar_wait(&bars[PS_PVDONE + (1 - buf)], ((j - 1) >> 1) & 1, WAIT_LIMIT);
+        fence_after_sync();
+        const uint32_t o_addr = tmem + lane_base + PS_TO + part * (D / 2);
+#pragma unroll
+        for (int c0 = 0; c0 < D / 2; c0 += 16) {
+          uint32_t ov[16];
+          tmem_ld16(o_addr + c0, ov);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+          tmem_st16(o_addr + c0, ov);
+        }
+        tmem_st_wait();
+      }
+      const float m_use = m_run == -CUDART_INF_F ? 0.f : m_run;
+      float ls4[4] = {0.f, 0.f, 0.f, 0.f};
+      uint32_t pk[2][16];
+      auto exponentials = [&](auto masked) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const uint32_t vq = (uint32_t)(vis >> (32 * q));
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float p0 = ex2_approx(fmaf(__uint_as_float(sv[q][2 * i]), p.scale_log2, -m_use));
+            float p1 = ex2_approx(fmaf(__uint_as_float(sv[q][2 * i + 1]), p.scale_log2, -m_use));
+            if (decltype(masked)::value) {
+              p0 = ((vq >> (2 * i)) & 1u) ? p0 : 0.f;
+              p1 = ((vq >> (2 * i + 1)) & 1u) ? p1 : 0.f;
+            }
+            ls4[i & 3] += p0 + p1;
+            pk[q][i] = pack2<T>(p0, p1);
+          }
+        }
+      };
+      if (all_vis) exponentials(std::false_type());
+      else exponentials(std::true_type());
+      l_run += (ls4[0] + ls4[1]) + (ls4[2] + ls4[3]);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) tmem_st16(s_addr + q * 16, pk[q]);
+      tmem_st_wait();
+      if (!Q8 && key0 + PS_KEYS > kend) {   // rows behind the last key may hold anything, and 0 * NaN is NaN
+        if (!failed) failed = !mbar_wait(&bars[PS_VFULL + buf], (j >> 1) & 1, WAIT_LIMIT);
+        const int dead = key0 + PS_KEYS - kend;
+        for (int i = tid; i < dead * VB * 8; i += 32 * PS_SM_WARPS)
+          *reinterpret_cast<uint4*>(Vs + buf * VBUF + (i / 8 / dead) * (PS_KEYS * 128) + (PS_KEYS - dead + i / 8 % dead) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+        fence_async_smem();
+      }
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[PS_PFULL + buf]);
+    }
+
+    // ---- epilogue: O / l and LSE, or this range's part of them ----------------------------------------
+    row_sync();   // (every thread of the row is past its last look at the row maxima)
+    xch[part * PS_ROWS + rloc] = l_run;
+    row_sync();
+    const float l_tot = live ? xch[rloc] + xch[PS_ROWS + rloc] : 0.f;
+    if (T_tiles > 0 && !failed) failed = !mbar_wait(&bars[PS_ODONE], 0, WAIT_LIMIT);
+    fence_after_sync();
+    const bool whole = p.nsplit == 1, out_row = rho < p.Nq * p.G;   // (padding is written too)
+    const float inv = l_tot != 0.f ? (whole ? 1.f / l_tot : 1.f) : 0.f;
+    const uint32_t o_addr = tmem + lane_base + PS_TO + part * (D / 2);
+    T* orow = static_cast<T*>(p.o) + b * p.so.b + head * p.so.h + (int64_t)tok * p.so.n + part * (D / 2);
+    const int64_t slot = (int64_t)ub * p.nsplit + split;
+    float* prow = p.part_o + (slot * PS_ROWS + rloc) * D + part * (D / 2);
+#pragma unroll
+    for (int c0 = 0; c0 < D / 2; c0 += 16) {
+      uint32_t ov[16];
+      tmem_ld16(o_addr + c0, ov);
+      tmem_ld_wait();
+      float x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = l_tot != 0.f ? __uint_as_float(ov[i]) * inv : 0.f;   // (without a visible key O may hold anything)
+      if (out_row && whole) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 8)
+          *reinterpret_cast<uint4*>(orow + c0 + i) =
+              make_uint4(pack2<T>(x[i], x[i + 1]), pack2<T>(x[i + 2], x[i + 3]), pack2<T>(x[i + 4], x[i + 5]), pack2<T>(x[i + 6], x[i + 7]));
+      } else if (out_row) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(prow + c0 + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+      }
+    }
+    if (part == 0 && out_row) {
+      if (!whole) p.part_ml[(slot * PS_ROWS + rloc) * 2] = l_tot != 0.f ? m_run : -CUDART_INF_F, p.part_ml[(slot * PS_ROWS + rloc) * 2 + 1] = l_tot;
+      else if (p.lse) p.lse[((int64_t)b * p.H + head) * p.Nq + tok] = l_tot != 0.f ? m_run * LN2 + logf(l_tot) : -CUDART_INF_F;
+    }
+    if (!whole) {
+      // the CTA that finishes a row block last merges its parts
+      __threadfence();
+      all_sync();
+      if (tid == 0) *last_s = atomicAdd(p.done + ub, 1u) == (unsigned)p.nsplit - 1u;
+      all_sync();
+      if (*last_s) {
+        __threadfence();
+        float* wgt = reinterpret_cast<float*>(Ks);   // [split][128 rows] weights, then the rows' 1 / sum
+        const int64_t slot0 = (int64_t)ub * p.nsplit;
+        if (tid < PS_ROWS && out_row) {
+          float M = -CUDART_INF_F, L = 0.f;
+          for (int s = 0; s < p.nsplit; ++s) M = fmaxf(M, __ldcg(p.part_ml + ((slot0 + s) * PS_ROWS + rloc) * 2));
+          const float mu = M == -CUDART_INF_F ? 0.f : M;
+          for (int s = 0; s < p.nsplit; ++s) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + ((slot0 + s) * PS_ROWS + rloc) * 2));
+            const float f = ex2_approx(ml.x - mu);
+            wgt[s * PS_ROWS + rloc] = f, L = fmaf(ml.y, f, L);
+          }
+          wgt[p.nsplit * PS_ROWS + rloc] = L != 0.f ? 1.f / L : 0.f;
+          if (p.lse) p.lse[((int64_t)b * p.H + head) * p.Nq + tok] = L != 0.f ? M * LN2 + logf(L) : -CUDART_INF_F;
+        }
+        all_sync();
+        for (int i = tid; i < PS_ROWS * (D / 4); i += 32 * PS_SM_WARPS) {
+          const int row = i / (D / 4), c4 = i - row * (D / 4), rr = rb * PS_ROWS + row, t = rr / p.G, h = hk + (rr - t * p.G) * p.Hk;
+          if (t >= p.Nq) break;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+          for (int s = 0; s < p.nsplit; ++s) {
+            const float f = wgt[s * PS_ROWS + row];
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + ((slot0 + s) * PS_ROWS + row) * D + 4 * c4));
+            acc.x = fmaf(f, x.x, acc.x), acc.y = fmaf(f, x.y, acc.y), acc.z = fmaf(f, x.z, acc.z), acc.w = fmaf(f, x.w, acc.w);
+          }
+          const float f = wgt[p.nsplit * PS_ROWS + row];
+          *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + b * p.so.b + h * p.so.h + (int64_t)t * p.so.n + 4 * c4) =
+              make_uint2(pack2<T>(acc.x * f, acc.y * f), pack2<T>(acc.z * f, acc.w * f));
+        }
+      }
+    }
+  }
+  if (failed) atomicOr(p.status, 1u);
+  fence_before_sync();
+  __syncthreads();
+  if (warp == PS_S) tmem_dealloc(tmem, 512);
+}
+
+// ---- host side -----------------------------------------------------------------------------------------
+static int sweep_blocks(const PopeShape& s) { return (int)(((int64_t)s.Nq * (s.H / s.Hk) + PS_ROWS - 1) / PS_ROWS); }
+
+// Key ranges per row block: whole waves of one CTA per SM times a CTA's steps plus what it costs beside them (Q', the epilogue and the merge,
+// about ten steps' time).
+static int sweep_split(const PopeShape& s) {
+  const int tiles = (s.Nk + PS_KEYS - 1) / PS_KEYS;
+  const int64_t units = (int64_t)s.B * s.Hk * sweep_blocks(s);
+  int best = 1;
+  int64_t best_cost = INT64_MAX;
+  for (int n = 1; n <= std::min(tiles, PS_MAX_SPLIT); ++n) {
+    const int64_t cost = (units * n + 147) / 148 * ((tiles + n - 1) / n + (n > 1 ? 10 : 6));
+    if (cost < best_cost) best = n, best_cost = cost;
+  }
+  return best;
+}
+
+// workspace: [tables][K' images][16-bit V rows][counters][parts][their maxima and sums]
+struct SweepWs {
+  size_t kimg, vrows, done, part_o, part_ml, total;
+};
+static SweepWs sweep_ws(const PopeShape& s, int store) {
+  auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+  const size_t units = (size_t)s.B * s.Hk, blocks = units * sweep_blocks(s), rows = image_tiles(s.Nk) * IMAGE_ROWS;
+  const size_t parts = sweep_split(s) > 1 ? blocks * sweep_split(s) * PS_ROWS : 0;
+  SweepWs w;
+  w.kimg = trig_tables_bytes(s.Nk, s.r);
+  w.vrows = w.kimg + up(units * rows * (s.d + round_up(s.r, 16)) * 2);
+  w.done = w.vrows + (store == POPE_STORE_16 ? 0 : up(units * rows * s.d * 2));
+  w.part_o = w.done + up(blocks * sizeof(unsigned int));
+  w.part_ml = w.part_o + up(parts * s.d * sizeof(float));
+  w.total = w.part_ml + up(parts * 2 * sizeof(float));
+  return w;
+}
+size_t paged_sweep_workspace(const PopePagedAttnArgs& a) { return sweep_ws(a.shape, a.cache.store).total; }
+
+template <typename T, int STORE, int D> static cudaError_t paged_sweep_t(const PopePagedAttnArgs& a, cudaStream_t st) {
+  constexpr bool Q8 = STORE != POPE_STORE_16;
+  const PopeShape& s = a.shape;
+  const PopePagedKV& kv = a.cache.kv;
+  const SweepWs ws = sweep_ws(s, STORE);
+  uint8_t* base = static_cast<uint8_t*>(a.workspace);
+  const TrigTables tt = trig_tables_at(base, s.Nk, s.r);
+  const int tiles = (int)image_tiles(s.Nk), RP = round_up(s.r, 16);
+  PagedImageP im;
+  im.c = paged_ptrs(a.cache, s.Hk, s.d);
+  if (!im.c.status) return cudaErrorInvalidSymbol;
+  im.B = s.B, im.Nk = s.Nk, im.r = s.r, im.RP = RP, im.tiles = tiles;
+  im.ch = static_cast<const __half*>(tt.ch), im.sh = static_cast<const __half*>(tt.sh);
+  im.bias = a.embed.bias, im.bias_sh = a.embed.bias_stride_h;
+  im.kimg = base + ws.kimg, im.vrows = base + ws.vrows;
+  im.done = reinterpret_cast<unsigned int*>(base + ws.done), im.ndone = s.B * s.Hk * sweep_blocks(s);
+  PagedSweepP p = {};
+  p.H = s.H, p.Hk = s.Hk, p.G = s.H / s.Hk, p.Nq = s.Nq, p.Nk = s.Nk, p.r = s.r, p.RP = RP, p.tiles = tiles;
+  p.nsplit = sweep_split(s), p.blocks = sweep_blocks(s);
+  p.page_size = kv.page_size, p.max_pages = kv.max_pages_per_seq, p.num_pages = kv.num_pages;
+  auto wide = [](const void* ptr, const PopeStride3& t) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && t.b % 8 == 0 && t.h % 8 == 0 && t.n % 8 == 0; };
+  p.q_wide = wide(a.q, a.sq);
+  p.scale_log2 = std::abs(a.softmax_scale) * LOG2E, p.q_sign = a.softmax_scale < 0.f ? 0x80008000u : 0u;
+  p.page_table = kv.page_table, p.seq_lens = kv.seq_lens, p.counts = a.counts;
+  p.q = a.q, p.o = a.out, p.lse = a.lse, p.sq = Strides(a.sq), p.so = Strides(a.so);
+  p.kimg = im.kimg, p.ch = im.ch, p.sh = im.sh;
+  p.part_o = reinterpret_cast<float*>(base + ws.part_o), p.part_ml = reinterpret_cast<float*>(base + ws.part_ml);
+  p.done = im.done, p.status = im.c.status;
+  CUtensorMap tmap_v;
+  const int rows = tiles * IMAGE_ROWS;
+  const int64_t page = (int64_t)kv.page_size * s.d;
+  const bool bf16 = s.dtype == POPE_BF16;
+  const bool ok = Q8 ? make_wide_tmap(&tmap_v, im.vrows, bf16, s.d, rows, s.Hk, s.B, s.d, (int64_t)rows * s.d, (int64_t)rows * s.d * s.Hk, 64)
+                     : make_wide_tmap(&tmap_v, kv.v_pages, bf16, s.d, kv.page_size, s.Hk, kv.num_pages, s.d, page, page * s.Hk, 64);
+  if (!ok) return cudaErrorNotSupported;
+  const int KD = s.d + RP;
+  // (every CTA allocates all 512 TMEM columns: two must not share an SM)
+  const size_t smem = std::max<size_t>(2 * (size_t)PS_KEYS * KD * 2 + 2 * (size_t)((s.d + 63) / 64) * PS_KEYS * 128 + 4 * PS_ROWS * 4 + PS_COUNT * 8 + 16 + 1024, 120 * 1024);
+  cudaError_t e = ensure_max_smem<paged_sweep_kernel<T, D, Q8>>();
+  if (e != cudaSuccess) return e;
+  if (s.r > 0 && (e = launch_trig_tables(a.embed, s.Nk, s.r, nullptr, nullptr, tt.ch, tt.sh, st)) != cudaSuccess) return e;
+  const size_t ismem = (size_t)(KD / 8) * CS64 + 2 * (size_t)s.r * sizeof(float);
+  if ((e = launch_dependent(paged_image_kernel<T, STORE, D>, dim3((unsigned)((s.Nk + 127) / 128 * 2), (unsigned)(s.B * s.Hk)), dim3(256), ismem, st, im)) != cudaSuccess) return e;
+  return launch_dependent(paged_sweep_kernel<T, D, Q8>, dim3((unsigned)(s.B * s.Hk * p.blocks * p.nsplit)), dim3(PS_THREADS), smem, st, p, tmap_v);
+}
+template <typename T, int STORE> static cudaError_t paged_sweep_d(const PopePagedAttnArgs& a, cudaStream_t st) {
+  const int d = a.shape.d;
+  return d == 64 ? paged_sweep_t<T, STORE, 64>(a, st) : d == 96 ? paged_sweep_t<T, STORE, 96>(a, st) : paged_sweep_t<T, STORE, 128>(a, st);
+}
+template <typename T> static cudaError_t paged_sweep_s(const PopePagedAttnArgs& a, cudaStream_t st) {
+  switch (a.cache.store) {
+    case POPE_STORE_INT8: return paged_sweep_d<T, POPE_STORE_INT8>(a, st);
+    case POPE_STORE_E4M3: return paged_sweep_d<T, POPE_STORE_E4M3>(a, st);
+    default: return paged_sweep_d<T, POPE_STORE_16>(a, st);
+  }
+}
+cudaError_t paged_sweep(const PopePagedAttnArgs& a, cudaStream_t st) {
+  return a.shape.dtype == POPE_BF16 ? paged_sweep_s<__nv_bfloat16>(a, st) : paged_sweep_s<__half>(a, st);
+}
+
+// ---- which of the two ------------------------------------------------------------------------------------
+bool attn_paged_supported(const PopePagedAttnArgs& a) {
+  const PopeShape& s = a.shape;
+  if (s.dtype != POPE_BF16 && s.dtype != POPE_F16) return false;
+  if (s.d != 64 && s.d != 96 && s.d != 128) return false;
+  if (s.r % 8 != 0 || (s.r > 0 && (a.embed.sf.b != 0 || a.embed.sf.h != 0))) return false;
+  return a.cache.kv.page_size % 64 == 0;
+}
+
+// Rows that share a key head, up to which one pass over the keys per block of 32 is taken
+static bool few_rows(const PopeShape& s) { return (int64_t)s.Nq * (s.H / s.Hk) <= 64; }
+
+size_t attn_paged_workspace(const PopePagedAttnArgs& a) { return few_rows(a.shape) ? paged_rows_workspace(a) : paged_sweep_workspace(a); }
+
+cudaError_t attn_paged(const PopePagedAttnArgs& a, cudaStream_t st) { return few_rows(a.shape) ? paged_rows(a, st) : paged_sweep(a, st); }
+
+}  // namespace pope

@@ -52,6 +52,11 @@ def attend(q, k, v, freqs, bias, lens, counts, scale, store=None):
                 ds2 = scale ** 2 * both.square().sum(-1) * (4 * u * u + 2 * 2.0 ** -22) / 3
                 out[i, head, row], lse[i, head, row] = o, torch.logsumexp(s, 0)
                 worst[i, head, row] = 1.1 * (u_out * o.abs() + 2 * u * (p @ vv.abs()) + (p * ds) @ (vv.abs() + o.abs()))
+                if ds2.max() > 1 / 64:
+                    # scores that are off by an eighth and more: exp(ds) - 1 is no longer ds, and the first order says nothing about the
+                    # 2-norm.  What holds: out is a mean of the rows of v whatever the scores are, so two of them differ by 2 max |v| at most.
+                    rms2[i, head, row] = (2 * vv.abs().max(0).values) ** 2
+                    continue
                 rms2[i, head, row] = (u_out * o) ** 2 / 3 + (p * p) @ vv.square() * 2 * u * u / 3 + (p * p * ds2) @ (vv - o).square()
     return out, lse, worst, rms2.sqrt()
 
