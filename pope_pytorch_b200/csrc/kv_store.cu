@@ -59,50 +59,60 @@ __device__ __forceinline__ uint2 quantise8(const uint4& raw, float* scale) {
   return make_uint2(out[0], out[1]);
 }
 
-// Row `tensor` (0 = k, 1 = v) of token i, head hk: every lane of the warp calls this; `on` = the lane has a row at all.
-template <typename T, int STORE, int D, int LPR>
-__device__ __forceinline__ void write_row(const KvWriteP& p, int b, int hk, int i, int tensor, int len, int lane, bool on) {
-  on = on && lane * 8 < D;
-  const Strides& s = tensor ? p.sv : p.sk;
-  const T* src = static_cast<const T*>(tensor ? p.v : p.k) + b * s.b + hk * s.h + (int64_t)i * s.n + lane * 8;
-  uint4 raw = make_uint4(0, 0, 0, 0);
-  if (on) raw = *reinterpret_cast<const uint4*>(src);
-  float scale;
-  const uint2 codes = quantise8<T, STORE, LPR>(raw, &scale);
-  if (!on) return;
-  const int64_t row = paged_row(p.c, b, hk, len + i);
-  if (row < 0) return;
-  *reinterpret_cast<uint2*>((tensor ? p.c.v : p.c.k) + row * D + lane * 8) = codes;
-  if (lane == 0) (tensor ? p.c.v_scales : p.c.k_scales)[row] = scale;
+// Up to KW_ROWS rows of k and of v for a group of LPR lanes: all their loads go out before the first store (one row after the other, 32768
+// tokens of 8 key heads of 128 took 63 us).  `at(j, &hk, &i)` names row j and says whether there is one; every lane of the warp calls this.
+constexpr int KW_ROWS = 4;
+template <typename T, int STORE, int D, int LPR, typename At>
+__device__ __forceinline__ void write_rows(const KvWriteP& p, int b, int len, int lane, At at) {
+  uint4 raw[KW_ROWS][2];
+  int64_t row[KW_ROWS];
+#pragma unroll
+  for (int j = 0; j < KW_ROWS; ++j) {
+    int hk = 0, i = 0;
+    const bool on = at(j, &hk, &i) && lane * 8 < D;
+    row[j] = -1;
+    raw[j][0] = raw[j][1] = make_uint4(0, 0, 0, 0);
+    if (!on) continue;
+    row[j] = paged_row(p.c, b, hk, len + i);
+    raw[j][0] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.k) + b * p.sk.b + hk * p.sk.h + (int64_t)i * p.sk.n + lane * 8);
+    raw[j][1] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.v) + b * p.sv.b + hk * p.sv.h + (int64_t)i * p.sv.n + lane * 8);
+  }
+#pragma unroll
+  for (int j = 0; j < KW_ROWS; ++j)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      float scale;
+      const uint2 codes = quantise8<T, STORE, LPR>(raw[j][t], &scale);
+      if (row[j] < 0) continue;
+      *reinterpret_cast<uint2*>((t ? p.c.v : p.c.k) + row[j] * D + lane * 8) = codes;
+      if (lane == 0) (t ? p.c.v_scales : p.c.k_scales)[row[j]] = scale;
+    }
 }
 
-constexpr int KW_ROWS = 4;   // rows of each of k and v that a group of lanes takes
 template <typename T, int STORE, int D>
 __global__ void __launch_bounds__(256) kv_write_kernel(KvWriteP p) {
   constexpr int LPR = D == 64 ? 8 : 16;
   const int group = threadIdx.x / LPR, lane = threadIdx.x % LPR, b = blockIdx.z;
   pdl_wait();
-  const int len = p.c.seq_lens[b];
-#pragma unroll
-  for (int j = 0; j < KW_ROWS; ++j) {
-    const int i = (blockIdx.x * KW_ROWS + j) * (256 / LPR) + group;
-    write_row<T, STORE, D, LPR>(p, b, blockIdx.y, i, 0, len, lane, i < p.n_new);
-    write_row<T, STORE, D, LPR>(p, b, blockIdx.y, i, 1, len, lane, i < p.n_new);
-  }
+  write_rows<T, STORE, D, LPR>(p, b, p.c.seq_lens[b], lane, [&](int j, int* hk, int* i) {
+    *hk = blockIdx.y, *i = (blockIdx.x * KW_ROWS + j) * (256 / LPR) + group;
+    return *i < p.n_new;
+  });
 }
 
 // A few tokens (a decode step): one CTA per sequence, which advances the length itself once all of its threads have read it.
-constexpr int KW_STEP_ROWS = 512;
+constexpr int KW_STEP_ROWS = 256, KW_STEP_THREADS = 1024;   // key heads x tokens: what the groups of a CTA take at a time
 template <typename T, int STORE, int D>
-__global__ void __launch_bounds__(256) kv_write_step_kernel(KvWriteP p) {
+__global__ void __launch_bounds__(KW_STEP_THREADS) kv_write_step_kernel(KvWriteP p) {
   constexpr int LPR = D == 64 ? 8 : 16;
   const int group = threadIdx.x / LPR, lane = threadIdx.x % LPR, b = blockIdx.x;
   pdl_wait();
   const int len = p.c.seq_lens[b], rows = p.c.Hk * p.n_new;
-  for (int first = 0; first < 2 * rows; first += 256 / LPR) {   // (whole warps stay in the loop: the maxima are warp operations)
-    const int at = first + group, row = at >> 1;
-    write_row<T, STORE, D, LPR>(p, b, min(row, rows - 1) / p.n_new, row % p.n_new, at & 1, len, lane, row < rows);
-  }
+  write_rows<T, STORE, D, LPR>(p, b, len, lane, [&](int j, int* hk, int* i) {
+    const int row = j * (KW_STEP_THREADS / LPR) + group;
+    *hk = row / p.n_new, *i = row - *hk * p.n_new;
+    return row < rows;
+  });
   __syncthreads();
   if (p.advance && threadIdx.x == 0) p.c.seq_lens[b] = len + p.n_new;
 }
@@ -119,7 +129,7 @@ template <typename T, int STORE, int D> static cudaError_t kv_write_t(const Pope
   if (!p.c.status) return cudaErrorInvalidSymbol;
   p.n_new = a.n_new, p.advance = a.advance;
   p.k = a.k, p.v = a.v, p.sk = Strides(a.sk), p.sv = Strides(a.sv);
-  if ((int64_t)a.Hk * a.n_new * 2 <= KW_STEP_ROWS) return launch_dependent(kv_write_step_kernel<T, STORE, D>, dim3(a.B), dim3(256), 0, st, p);
+  if ((int64_t)a.Hk * a.n_new <= KW_STEP_ROWS) return launch_dependent(kv_write_step_kernel<T, STORE, D>, dim3(a.B), dim3(KW_STEP_THREADS), 0, st, p);
   constexpr int rows = KW_ROWS * 256 / (D == 64 ? 8 : 16);
   const dim3 grid((unsigned)((a.n_new + rows - 1) / rows), (unsigned)a.Hk, (unsigned)a.B);
   cudaError_t e = launch_dependent(kv_write_kernel<T, STORE, D>, grid, dim3(256), 0, st, p);

@@ -58,4 +58,7 @@ template <int STORE> __device__ __forceinline__ void codes_to_f32(uint32_t w, fl
   }
 }
 
+// fp16 cos / sin tables of a call, [2][n][r]; also zeroes `nzero` counters.  One launch.
+cudaError_t launch_paged_tables(const PopeEmbed& e, int n, int r, void* ch, void* sh, unsigned int* zero, int nzero, cudaStream_t st);
+
 }  // namespace pope

@@ -801,7 +801,7 @@ template <typename T, int STORE, int D, int RQ> static cudaError_t paged_rows_t(
   const dim3 grid(units * (unsigned)p.nsplit), block(32 * NW);
   // behind the table kernel, which also zeroes the counters
   if (s.r > 0) {
-    if ((e = launch_trig_tables(a.embed, s.Nk, s.r, nullptr, nullptr, table, table + (size_t)s.Nk * s.r, st, 1, 1, p.done, (int)units)) != cudaSuccess) return e;
+    if ((e = launch_paged_tables(a.embed, s.Nk, s.r, table, table + (size_t)s.Nk * s.r, p.done, (int)units, st)) != cudaSuccess) return e;
     return launch_dependent(kernel, grid, block, smem, st, p, mk, mv, mt, mks, mvs);
   }
   if (p.nsplit > 1 && (e = cudaMemsetAsync(p.done, 0, units * sizeof(unsigned int), st)) != cudaSuccess) return e;

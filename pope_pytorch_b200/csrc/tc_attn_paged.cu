@@ -19,6 +19,40 @@
 
 namespace pope {
 
+// ---- tables --------------------------------------------------------------------------------------------
+// A thread takes four features of a position.  The results are rounded to fp16 (2^-12): the reduced sine and cosine (2^-20) do.  (The table
+// kernel of the other paths, accurate and a feature per thread, takes 14.6 us for 32768 positions of 64.)
+__global__ void __launch_bounds__(256) paged_tables_kernel(const float* freqs, int64_t sfn, int n, int r, int wide, __half* ch, __half* sh, unsigned int* zero,
+                                                           int nzero) {
+  pdl_wait();
+  pdl_trigger();
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < nzero; i += 256) zero[i] = 0;
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (at >= (int64_t)n * r) return;
+  const int64_t pos = at / r;
+  const float* f = freqs + pos * sfn + (at - pos * r);
+  float x[4], s[4], c[4];
+  if (wide) {
+    const float4 v = *reinterpret_cast<const float4*>(f);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = f[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sincos_reduced(x[i], &s[i], &c[i]);
+  *reinterpret_cast<uint2*>(ch + at) = make_uint2(pack2<__half>(c[0], c[1]), pack2<__half>(c[2], c[3]));
+  *reinterpret_cast<uint2*>(sh + at) = make_uint2(pack2<__half>(s[0], s[1]), pack2<__half>(s[2], s[3]));
+}
+
+cudaError_t launch_paged_tables(const PopeEmbed& e, int n, int r, void* ch, void* sh, unsigned int* zero, int nzero, cudaStream_t st) {
+  const int wide = (reinterpret_cast<uintptr_t>(e.freqs) & 15) == 0 && e.sf.n % 4 == 0;
+  const int64_t threads = (int64_t)n * r / 4;   // (r is a multiple of 8)
+  return launch_dependent(paged_tables_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, e.freqs, e.sf.n, n, r, wide, static_cast<__half*>(ch),
+                          static_cast<__half*>(sh), zero, nzero);
+}
+
 // ---- images --------------------------------------------------------------------------------------------
 struct PagedImageP {
   PagedPtrs c;
@@ -35,9 +69,9 @@ struct PagedImageP {
 
 // One 64-row tile per CTA (the rows of a tile lie in one page).  256 threads: a thread keeps one 16-byte column of the rows it touches.
 template <typename T, int STORE, int D>
-__global__ void __launch_bounds__(256) paged_image_kernel(PagedImageP p) {
+__global__ void __launch_bounds__(256, 6) paged_image_kernel(PagedImageP p) {
   constexpr bool Q8 = STORE != POPE_STORE_16;
-  constexpr int DC = D / 8, RPP = 256 / DC, NIT = (IMAGE_ROWS + RPP - 1) / RPP;
+  constexpr int DC = D / 8, RPP = 256 / DC, NIT = 2;   // (two rows at a time: all of a thread's at once left room for four CTAs)
   extern __shared__ __align__(16) uint8_t stage[];
   const int tid = threadIdx.x, tile = blockIdx.x, u = blockIdx.y, b = u / p.c.Hk, hk = u % p.c.Hk, r = p.r;
   pdl_wait();
@@ -59,10 +93,10 @@ __global__ void __launch_bounds__(256) paged_image_kernel(PagedImageP p) {
   const bool active = first < RPP, rotated = c * 8 < r;
   uint4 raw[NIT];
   float scale[NIT];
-  auto load = [&](const uint8_t* pool, const float* scales) {
+  auto load = [&](const uint8_t* pool, const float* scales, int base) {
 #pragma unroll
     for (int it = 0; it < NIT; ++it) {
-      const int row = first + it * RPP;
+      const int row = first + it * RPP + base;
       raw[it] = make_uint4(0, 0, 0, 0), scale[it] = 0.f;
       if (!active || row >= rows) continue;
       if constexpr (Q8) {
@@ -84,15 +118,15 @@ __global__ void __launch_bounds__(256) paged_image_kernel(PagedImageP p) {
       x[0] = unpack2<T>(raw[it].x), x[1] = unpack2<T>(raw[it].y), x[2] = unpack2<T>(raw[it].z), x[3] = unpack2<T>(raw[it].w);
     }
   };
-  load(p.c.k, p.c.k_scales);
+#pragma unroll 1
+  for (int base = 0; base < IMAGE_ROWS; base += NIT * RPP) {
+  load(p.c.k, p.c.k_scales, base);
   if (rotated) {
-    float cb[8], sb[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) cb[e] = bias_c[c * 8 + e], sb[e] = bias_s[c * 8 + e];
+    const float *cb = bias_c + c * 8, *sb = bias_s + c * 8;
     uint4 cq[NIT], sq[NIT];
 #pragma unroll
     for (int it = 0; it < NIT; ++it) {
-      const int row = first + it * RPP;
+      const int row = first + it * RPP + base;
       cq[it] = sq[it] = make_uint4(0, 0, 0, 0);   // (rows behind the last key become zeros)
       if (active && row < rows) {
         cq[it] = *reinterpret_cast<const uint4*>(p.ch + (int64_t)(key0 + row) * r + c * 8);
@@ -101,7 +135,7 @@ __global__ void __launch_bounds__(256) paged_image_kernel(PagedImageP p) {
     }
 #pragma unroll
     for (int it = 0; it < NIT; ++it) {
-      const int row = first + it * RPP;
+      const int row = first + it * RPP + base;
       if (!active || row >= IMAGE_ROWS) continue;
       const uint32_t cw[4] = {cq[it].x, cq[it].y, cq[it].z, cq[it].w}, sw[4] = {sq[it].x, sq[it].y, sq[it].z, sq[it].w};
       float2 x[4];
@@ -121,7 +155,7 @@ __global__ void __launch_bounds__(256) paged_image_kernel(PagedImageP p) {
   } else {
 #pragma unroll
     for (int it = 0; it < NIT; ++it) {
-      const int row = first + it * RPP;
+      const int row = first + it * RPP + base;
       if (!active || row >= IMAGE_ROWS) continue;
       uint4 o = raw[it];
       if constexpr (Q8) {
@@ -134,16 +168,17 @@ __global__ void __launch_bounds__(256) paged_image_kernel(PagedImageP p) {
     }
   }
   if constexpr (Q8) {   // V of the same rows, zeros behind the last key
-    load(p.c.v, p.c.v_scales);
+    load(p.c.v, p.c.v_scales, base);
 #pragma unroll
     for (int it = 0; it < NIT; ++it) {
-      const int row = first + it * RPP;
+      const int row = first + it * RPP + base;
       if (!active || row >= IMAGE_ROWS) continue;
       float2 x[4];
       values(it, x);
       *reinterpret_cast<uint4*>(static_cast<T*>(p.vrows) + ((int64_t)u * p.tiles * IMAGE_ROWS + key0 + row) * D + c * 8) =
           make_uint4(pack2<T>(x[0].x, x[0].y), pack2<T>(x[1].x, x[1].y), pack2<T>(x[2].x, x[2].y), pack2<T>(x[3].x, x[3].y));
     }
+  }
   }
   __syncthreads();
   // the image leaves in its own byte order, coalesced: tiles 2 t and 2 t + 1 share a 128-row tile
@@ -623,7 +658,7 @@ template <typename T, int STORE, int D> static cudaError_t paged_sweep_t(const P
   const size_t smem = std::max<size_t>(2 * (size_t)PS_KEYS * KD * 2 + 2 * (size_t)((s.d + 63) / 64) * PS_KEYS * 128 + 4 * PS_ROWS * 4 + PS_COUNT * 8 + 16 + 1024, 120 * 1024);
   cudaError_t e = ensure_max_smem<paged_sweep_kernel<T, D, Q8>>();
   if (e != cudaSuccess) return e;
-  if (s.r > 0 && (e = launch_trig_tables(a.embed, s.Nk, s.r, nullptr, nullptr, tt.ch, tt.sh, st)) != cudaSuccess) return e;
+  if (s.r > 0 && (e = launch_paged_tables(a.embed, s.Nk, s.r, tt.ch, tt.sh, nullptr, 0, st)) != cudaSuccess) return e;
   const size_t ismem = (size_t)(KD / 8) * CS64 + 2 * (size_t)s.r * sizeof(float);
   if ((e = launch_dependent(paged_image_kernel<T, STORE, D>, dim3((unsigned)((s.Nk + 127) / 128 * 2), (unsigned)(s.B * s.Hk)), dim3(256), ismem, st, im)) != cudaSuccess) return e;
   return launch_dependent(paged_sweep_kernel<T, D, Q8>, dim3((unsigned)(s.B * s.Hk * p.blocks * p.nsplit)), dim3(PS_THREADS), smem, st, p, tmap_v);
