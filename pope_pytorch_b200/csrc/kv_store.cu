@@ -16,51 +16,29 @@ struct KvWriteP {
   Strides sk, sv;
 };
 
-// The largest magnitude over the lanes of a row, as bits: ordered like the values, with infinities and NaNs above all of them.
-template <int LPR> __device__ __forceinline__ uint32_t row_max_bits(uint32_t m) {
-#pragma unroll
-  for (int o = LPR / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  return m;
-}
-
-// Eight values of a row (raw words), the row's maximum over its LPR lanes -> eight codes and the scale.
-template <typename T, int STORE, int LPR>
-__device__ __forceinline__ uint2 quantise8(const uint4& raw, float* scale) {
+// Eight values of a row (raw words) times the row's M / A -> eight codes; M / A = 0 stands for a row that is held as zeros.
+template <typename T, int STORE> __device__ __forceinline__ uint2 quantise8(const uint4& raw, float inv) {
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) m = max(m, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
-  m = row_max_bits<LPR>(m);
-  const bool finite = m < (sizeof(T) == 2 && TcFmt<T>::fmt == FMT_BF16 ? 0x7f80u : 0x7c00u);
-  const float top = unpack2<T>(m).x;
-  if (!finite || top < ROW_LEAST) {
-    *scale = finite ? 0.f : __int_as_float(0x7fffffff);
-    return make_uint2(0, 0);
-  }
-  *scale = __fdiv_rn(top, kCodeTop<STORE>);
-  const float inv = __fdiv_rn(kCodeTop<STORE>, top);
   uint32_t out[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const float2 a = unpack2<T>(w[2 * i]), b = unpack2<T>(w[2 * i + 1]);
-    const float y[4] = {__fmul_rn(a.x, inv), __fmul_rn(a.y, inv), __fmul_rn(b.x, inv), __fmul_rn(b.y, inv)};
+    const float2 m = make_float2(inv, inv), a = mul2(unpack2<T>(w[2 * i]), m), b = mul2(unpack2<T>(w[2 * i + 1]), m);
     if constexpr (STORE == POPE_STORE_INT8) {
       // |y| <= 127 + 2^-16: y + 1.5 * 2^23 rounds it to an integer, ties to even, whose low byte is the code
-      uint32_t c[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) c[e] = __float_as_uint(__fadd_rn(y[e], 12582912.f));
-      out[i] = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+      const float2 magic = make_float2(12582912.f, 12582912.f), c = add2(a, magic), d = add2(b, magic);
+      out[i] = __byte_perm(__byte_perm(__float_as_uint(c.x), __float_as_uint(c.y), 0x0040), __byte_perm(__float_as_uint(d.x), __float_as_uint(d.y), 0x0040), 0x5410);
     } else {
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3), hi = __nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3);
       out[i] = lo | hi << 16;
     }
   }
-  return make_uint2(out[0], out[1]);
+  return inv != 0.f ? make_uint2(out[0], out[1]) : make_uint2(0, 0);
 }
 
-// Up to KW_ROWS rows of k and of v for a group of LPR lanes: all their loads go out before the first store (one row after the other, 32768
-// tokens of 8 key heads of 128 took 63 us).  `at(j, &hk, &i)` names row j and says whether there is one; every lane of the warp calls this.
+// Four rows of k and of v for a group of LPR lanes, eight values a lane: all their loads go out before the first store.  The maxima of the eight
+// rows are found together: a lane halves the rows it carries with every step and ends up with one, for which it takes the two
+// divisions; then M / A goes back to all lanes.  (Row by row, with every lane dividing for every row, 32768 tokens of 8 key heads of 128
+// took 61 us.)  `at(j, &hk, &i)` names row j and says whether there is one; every lane of the warp calls this.
 constexpr int KW_ROWS = 4;
 template <typename T, int STORE, int D, int LPR, typename At>
 __device__ __forceinline__ void write_rows(const KvWriteP& p, int b, int len, int lane, At at) {
@@ -77,16 +55,39 @@ __device__ __forceinline__ void write_rows(const KvWriteP& p, int b, int len, in
     raw[j][0] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.k) + b * p.sk.b + hk * p.sk.h + (int64_t)i * p.sk.n + lane * 8);
     raw[j][1] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.v) + b * p.sv.b + hk * p.sv.h + (int64_t)i * p.sv.n + lane * 8);
   }
+  // magnitudes as bits: ordered like the values, with infinities and NaNs above all of them
+  uint32_t m[2 * KW_ROWS];
 #pragma unroll
-  for (int j = 0; j < KW_ROWS; ++j)
+  for (int i = 0; i < 2 * KW_ROWS; ++i) {
+    const uint4 x = raw[i >> 1][i & 1];
+    const uint32_t a = __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu));
+    m[i] = max(a & 0xffffu, a >> 16);
+  }
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      float scale;
-      const uint2 codes = quantise8<T, STORE, LPR>(raw[j][t], &scale);
-      if (row[j] < 0) continue;
-      *reinterpret_cast<uint2*>((t ? p.c.v : p.c.k) + row[j] * D + lane * 8) = codes;
-      if (lane == 0) (t ? p.c.v_scales : p.c.k_scales)[row[j]] = scale;
+  for (int n = KW_ROWS; n >= 1; n /= 2) {
+    const bool hi = (lane & n) != 0;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const uint32_t give = hi ? m[i] : m[i + n], keep = hi ? m[i + n] : m[i];
+      m[i] = max(keep, __shfl_xor_sync(0xffffffffu, give, n));
     }
+  }
+  if (LPR == 16) m[0] = max(m[0], __shfl_xor_sync(0xffffffffu, m[0], 8));
+  // row lane % 8: A, the scale A / M and the factor M / A
+  const bool finite = m[0] < (TcFmt<T>::fmt == FMT_BF16 ? 0x7f80u : 0x7c00u);
+  const float top = unpack2<T>(m[0]).x;
+  const bool held = finite && top >= ROW_LEAST;
+  const float inv = held ? __fdiv_rn(kCodeTop<STORE>, top) : 0.f;
+  const float scale = held ? __fdiv_rn(top, kCodeTop<STORE>) : finite ? 0.f : __int_as_float(0x7fffffff);
+#pragma unroll
+  for (int i = 0; i < 2 * KW_ROWS; ++i) {
+    const float f = __shfl_sync(0xffffffffu, inv, i, LPR);
+    const int64_t to = row[i >> 1];
+    const uint2 codes = quantise8<T, STORE>(raw[i >> 1][i & 1], f);
+    if (to < 0) continue;
+    *reinterpret_cast<uint2*>((i & 1 ? p.c.v : p.c.k) + to * D + lane * 8) = codes;
+    if (lane == i) (i & 1 ? p.c.v_scales : p.c.k_scales)[to] = scale;
+  }
 }
 
 template <typename T, int STORE, int D>

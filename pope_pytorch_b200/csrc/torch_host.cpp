@@ -561,23 +561,26 @@ std::tuple<Tensor, Tensor> kv_read(const Pages& p, int64_t row, int64_t first, i
   return {k, v};
 }
 
-// q (b, h, n, d): the newest tokens of every sequence, counts (b) of them where given -> (out, lse (b, h, n))
-std::tuple<Tensor, Tensor> kv_attend(const Pages& p, const Tensor& q_, const Tensor& freqs_, const Tensor& bias_, const optional<Tensor>& counts,
-                                     double scale, int64_t nk) {
+// q (b, h, n, d): the newest tokens of every sequence, counts (b) of them where given -> (out, lse (b, h, n) or None)
+std::tuple<Tensor, optional<Tensor>> kv_attend(const Pages& p, const Tensor& q_, const Tensor& freqs_, const Tensor& bias_, const optional<Tensor>& counts,
+                                               double scale, int64_t nk, bool want_lse) {
   validate_embed(q_, q_.size(0), q_.size(1), p.k.size(1), freqs_, bias_);
   py::gil_scoped_release nogil;
   c10::cuda::OptionalCUDAGuard guard(p.k.device());
-  at::NoGradGuard off;
+  at::AutoDispatchBelowADInplaceOrView below;   // (no gradients pass through a cache)
   const Tensor q = inner_contig(q_), freqs = fp32_rows(freqs_), bias = fp32_rows(bias_);
   const int r = (int)freqs.size(-1);
-  Tensor out = at::empty_like(q), lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+  Tensor out = at::empty_like(q);
+  optional<Tensor> lse;
+  if (want_lse) lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
   if (q.size(2) == 0) return {out, lse};
   PopePagedAttnArgs a = {};
   a.struct_bytes = sizeof(a), a.softmax_scale = (float)scale;
   a.shape = {(int32_t)q.size(0), (int32_t)q.size(1), (int32_t)p.k.size(1), (int32_t)q.size(2), (int32_t)nk, (int32_t)q.size(3), r, dtype_of(q)};
   a.embed = embed_of(freqs, bias, r), a.cache = p.held();
   if (counts) a.counts = counts->const_data_ptr<int32_t>();
-  a.q = q.const_data_ptr(), a.sq = s3(q), a.out = out.mutable_data_ptr(), a.so = s3(out), a.lse = lse.mutable_data_ptr<float>();
+  a.q = q.const_data_ptr(), a.sq = s3(q), a.out = out.mutable_data_ptr(), a.so = s3(out);
+  if (lse) a.lse = lse->mutable_data_ptr<float>();
   const Tensor ws = workspace(POPE_OP_ATTN_PAGED, a, q);
   check(pope_b200_attn_paged(&a, stream_of(q)), "pope_b200_attn_paged");
   return {out, lse};

@@ -19,6 +19,7 @@ in the CUDA library; there is no fallback.
 """
 from __future__ import annotations
 
+from operator import gt
 from typing import List, Optional, Sequence, Union
 
 import torch
@@ -71,11 +72,13 @@ class PageAllocator:
     def rollback(self, counts: Sequence[int]) -> None:
         """Take the newest ``counts[b]`` keys off every sequence; pages that then hold none go back to the pool, the newest
         first, so that they are handed out again in the same order."""
+        lens, size = self.lens, self.page_size
         for b, n in enumerate(counts):
-            self.lens[b] -= n
-            keep = -(-self.lens[b] // self.page_size)
-            self.free.extend(reversed(self.table[b][keep:]))
-            del self.table[b][keep:]
+            lens[b] = left = lens[b] - n
+            held = self.table[b]
+            if (keep := -(-left // size)) < len(held):
+                self.free.extend(reversed(held[keep:]))
+                del held[keep:]
 
     def release(self, b: int) -> None:
         """Return every page of sequence ``b`` to the pool."""
@@ -172,15 +175,16 @@ class PagedKVCache:
     def rollback(self, counts: Union[int, Sequence[int]]) -> None:
         """Forget the newest ``counts[b]`` tokens of every sequence (one number: of each); what remains stays as it is.  Drafted
         tokens that were not accepted, for one."""
+        lens = self.alloc.lens
         counts = [counts] * self.batch if isinstance(counts, int) else [int(n) for n in counts]
         if len(counts) != self.batch:
             raise ValueError("one count per sequence")
-        if any(not 0 <= n <= held for n, held in zip(counts, self.alloc.lens)):
+        if min(counts) < 0 or any(map(gt, counts, lens)):
             raise ValueError("a sequence does not hold that many tokens")
         rows = [b for b, n in enumerate(counts) if n]
         if rows:
             self.alloc.rollback(counts)
-            N._ops().kv_map(self._pages(), [-1 - b for b in rows], [self.alloc.lens[b] for b in rows])
+            N._ops().kv_map(self._pages(), [-1 - b for b in rows], [lens[b] for b in rows])
 
     # ---- the operators -------------------------------------------------------------------------
     def append(self, k: torch.Tensor, v: torch.Tensor) -> None:
@@ -227,8 +231,8 @@ class PagedKVCache:
         if self.store is None:
             out, lse = N._ops().kv_decode(self._pages(), q, freqs, bias, scale, nk)
         else:
-            out, lse = N._ops().kv_attend(self._pages(), q, freqs, bias, None, scale, nk)
-            lse = lse[..., 0]
+            out, lse = N._ops().kv_attend(self._pages(), q, freqs, bias, None, scale, nk, return_lse)
+            lse = lse[..., 0] if return_lse else None
         return (out, lse) if return_lse else out
 
     def attend(self, q: torch.Tensor, pos_emb, counts: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None,
@@ -256,7 +260,7 @@ class PagedKVCache:
                 raise ValueError("counts must be (batch,)")
             counts = counts.contiguous()
         scale = self.head_dim ** -0.5 if softmax_scale is None else softmax_scale
-        out, lse = N._ops().kv_attend(self._pages(), q, freqs, bias, counts, scale, nk)
+        out, lse = N._ops().kv_attend(self._pages(), q, freqs, bias, counts, scale, nk, return_lse)
         return (out, lse) if return_lse else out
 
     def read(self, b: int, start: int = 0, stop: Optional[int] = None):

@@ -24,7 +24,7 @@ class Recorder:
     def kv_read(self, pages, row, first, n, bf16):
         self.reads.append((row, first, n, bf16))
 
-    def kv_attend(self, pages, q, freqs, bias, counts, scale, nk):
+    def kv_attend(self, pages, q, freqs, bias, counts, scale, nk, want_lse):
         self.attended.append((counts, scale, nk))
         return q, q[..., 0]
 
