@@ -47,6 +47,8 @@ size_t attn_paged_workspace(const PopePagedAttnArgs& a);
 cudaError_t attn_paged(const PopePagedAttnArgs& a, cudaStream_t st);
 size_t paged_rows_workspace(const PopePagedAttnArgs& a);   // few rows per key head
 cudaError_t paged_rows(const PopePagedAttnArgs& a, cudaStream_t st);
+size_t paged_stream_workspace(const PopePagedAttnArgs& a); // some
+cudaError_t paged_stream(const PopePagedAttnArgs& a, cudaStream_t st);
 size_t paged_sweep_workspace(const PopePagedAttnArgs& a);  // many
 cudaError_t paged_sweep(const PopePagedAttnArgs& a, cudaStream_t st);
 // phase table, clamped bias and the clamp's gradient

@@ -8,7 +8,7 @@
 //            in 128-row tiles in the order in which the tensor core reads them; every row block sweeps the keys, so they are expanded once.
 //            Of a cache that holds 8 bits also V, as 16-bit rows.
 //   sweep  : S = Q' K'^T with Q' in tensor memory, online softmax, O += P V with P in tensor memory, 128 keys a step; K' by one bulk copy, V by
-//            tensor-map boxes from the pages.  Small grids are cut along the keys; the CTA that finishes a row block last merges its parts.
+//            tensor-map boxes from the pages.  Small grids are cut along the keys, a fourth launch merges the parts.
 // Row i of sequence b stands at p = len - count + i and sees the keys up to p: a step whose last key is not beyond the first row's position
 // needs no mask.
 #include <algorithm>
@@ -16,6 +16,7 @@
 
 #include "kernels.h"
 #include "paged.cuh"
+#include "paged_out.cuh"
 
 namespace pope {
 
@@ -53,6 +54,45 @@ cudaError_t launch_paged_tables(const PopeEmbed& e, int n, int r, void* ch, void
                           static_cast<__half*>(sh), zero, nzero);
 }
 
+// ---- merge ---------------------------------------------------------------------------------------------
+// A warp per row: a lane takes the maximum and the sum of one part, then four features of all of them.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) paged_merge_kernel(PagedOut e, int blocks, int blocks_per_unit) {
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);   // row block, row
+  const int ub = (int)(at / PAGED_ROWS), row = (int)(at % PAGED_ROWS);
+  if (ub >= blocks) return;
+  const int u = ub / blocks_per_unit, rb = blocks_per_unit - 1 - ub % blocks_per_unit, b = u / e.Hk, hk = u % e.Hk;
+  const int rho = rb * PAGED_ROWS + row, tok = rho / e.G, head = hk + (rho - tok * e.G) * e.Hk;
+  if (tok >= e.Nq) return;
+  const int64_t slot0 = (int64_t)ub * e.nsplit;
+  float2 ml = make_float2(-CUDART_INF_F, 0.f);
+  if (lane < e.nsplit) ml = *reinterpret_cast<const float2*>(e.part_ml + ((slot0 + lane) * PAGED_ROWS + row) * 2);
+  const float M = warp_max(ml.x), f = ex2_approx(ml.x - (M == -CUDART_INF_F ? 0.f : M)), L = warp_sum(ml.y * f), inv = L != 0.f ? 1.f / L : 0.f;
+  if (e.lse && lane == 0) e.lse[((int64_t)b * e.H + head) * e.Nq + tok] = L != 0.f ? M * LN2 + logf(L) : -CUDART_INF_F;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int s = 0; s < e.nsplit; ++s) {
+    const float w = __shfl_sync(0xffffffffu, f, s);
+    if (lane * 4 >= D) continue;
+    const float4 x = *reinterpret_cast<const float4*>(e.part_o + ((slot0 + s) * PAGED_ROWS + row) * D + lane * 4);
+    acc.x = fmaf(w, x.x, acc.x), acc.y = fmaf(w, x.y, acc.y), acc.z = fmaf(w, x.z, acc.z), acc.w = fmaf(w, x.w, acc.w);
+  }
+  if (lane * 4 < D)
+    *reinterpret_cast<uint2*>(static_cast<T*>(e.o) + b * e.so.b + head * e.so.h + (int64_t)tok * e.so.n + lane * 4) =
+        make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+}
+template <typename T> static cudaError_t paged_merge_d(const PagedOut& e, int d, int blocks, int per_unit, cudaStream_t st) {
+  const dim3 grid((unsigned)((int64_t)blocks * PAGED_ROWS / 8)), block(256);
+  return d == 64   ? launch_dependent(paged_merge_kernel<T, 64>, grid, block, 0, st, e, blocks, per_unit)
+         : d == 96 ? launch_dependent(paged_merge_kernel<T, 96>, grid, block, 0, st, e, blocks, per_unit)
+                   : launch_dependent(paged_merge_kernel<T, 128>, grid, block, 0, st, e, blocks, per_unit);
+}
+cudaError_t launch_paged_merge(const PagedOut& e, int dtype, int d, int blocks, int per_unit, cudaStream_t st) {
+  return dtype == POPE_BF16 ? paged_merge_d<__nv_bfloat16>(e, d, blocks, per_unit, st) : paged_merge_d<__half>(e, d, blocks, per_unit, st);
+}
+
 // ---- images --------------------------------------------------------------------------------------------
 struct PagedImageP {
   PagedPtrs c;
@@ -63,8 +103,6 @@ struct PagedImageP {
   uint8_t* kimg;             // [unit][128-row tile][chunk][128 rows][16 B]
   void* vrows;               // 8-bit stores: [unit][rows][D]
   int tiles;                 // 64-row tiles of a unit's image
-  unsigned int* done;
-  int ndone;
 };
 
 // One 64-row tile per CTA (the rows of a tile lie in one page).  256 threads: a thread keeps one 16-byte column of the rows it touches.
@@ -76,8 +114,6 @@ __global__ void __launch_bounds__(256, 6) paged_image_kernel(PagedImageP p) {
   const int tid = threadIdx.x, tile = blockIdx.x, u = blockIdx.y, b = u / p.c.Hk, hk = u % p.c.Hk, r = p.r;
   pdl_wait();
   pdl_trigger();
-  if (blockIdx.x == 0 && blockIdx.y == 0)
-    for (int i = tid; i < p.ndone; i += 256) p.done[i] = 0;
   const int len = max(0, min(p.c.seq_lens[b], p.Nk)), key0 = tile * IMAGE_ROWS;
   if (key0 >= (len + 127) / 128 * 128) return;   // (tiles come in pairs)
   const int rows = max(0, min(IMAGE_ROWS, len - key0));
@@ -191,27 +227,24 @@ __global__ void __launch_bounds__(256, 6) paged_image_kernel(PagedImageP p) {
 
 // ---- sweep -----------------------------------------------------------------------------------------------
 struct PagedSweepP {
-  int H, Hk, G, Nq, Nk, r, RP, nsplit, blocks, tiles;   // blocks: row blocks per unit; tiles: 64-row tiles of a unit's image
+  int Hk, G, Nq, Nk, r, RP, nsplit, blocks, tiles;   // blocks: row blocks per unit; tiles: 64-row tiles of a unit's image
   int page_size, max_pages, num_pages, q_wide;          // q_wide: rows of q on 16-byte boundaries
   float scale_log2;                                     // its magnitude; the sign sits in Q'
   uint32_t q_sign;
   const int32_t *page_table, *seq_lens, *counts;
   const void* q;
-  void* o;
-  float* lse;
-  Strides sq, so;
+  Strides sq;
   const uint8_t* kimg;
   const __half *ch, *sh;
-  float *part_o, *part_ml;   // [row block][split][128][D], [row block][split][128][max (log2 units), sum]
-  unsigned int *done, *status;
+  PagedOut e;
+  unsigned int* status;
 };
 
-constexpr int PS_ROWS = 128, PS_KEYS = 128;
-constexpr int PS_SM_WARPS = 8;                     // softmax warps: two threads per query row
+constexpr int PS_ROWS = PAGED_ROWS, PS_KEYS = 128;
+constexpr int PS_SM_WARPS = PAGED_SM_WARPS;
 constexpr int PS_KLOAD = 8, PS_S = 9, PS_PV = 10, PS_VLOAD = 11;
 constexpr int PS_THREADS = 32 * 12;
 constexpr uint32_t PS_TS = 128, PS_TO = 384;       // first TMEM column of the S / P buffers and of O (Q' starts at 0)
-constexpr int PS_MAX_SPLIT = 32;
 enum {
   PS_KFULL = 0,    // [2] K' tile landed
   PS_KFREE = 2,    // [2] S of the tile has completed
@@ -237,7 +270,6 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP 
   float* xch = reinterpret_cast<float*>(Vs + 2 * VBUF);           // [2 step parities][2 parts][128 rows] row maxima
   uint64_t* bars = reinterpret_cast<uint64_t*>(xch + 4 * PS_ROWS);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + PS_COUNT);
-  unsigned int* last_s = tmem_slot + 1;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (warp == PS_S) {
@@ -253,6 +285,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP 
   fence_after_sync();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
+  pdl_trigger();
   // unit (sequence, key head), row block (late ones, which see more keys, first), key range
   const int split = blockIdx.x % p.nsplit, ub = blockIdx.x / p.nsplit, u = ub / p.blocks, rb = p.blocks - 1 - ub % p.blocks;
   const int b = u / p.Hk, hk = u % p.Hk;
@@ -364,7 +397,6 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP 
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const int row_bar = 1 + (warp & 3);   // named barrier of the two warps that share 32 rows
     auto row_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(row_bar) : "memory"); };
-    auto all_sync = []() { asm volatile("bar.sync 5, %0;" ::"n"(32 * PS_SM_WARPS) : "memory"); };
     {
       // Q' = [a cos f | plain | a sin f], expanded here from q and the fp16 tables straight into tensor memory; rows that are no queries are zero
       constexpr int DC = D >> 3;
@@ -501,80 +533,8 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP 
       if (lane == 0) mbar_arrive(&bars[PS_PFULL + buf]);
     }
 
-    // ---- epilogue: O / l and LSE, or this range's part of them ----------------------------------------
-    row_sync();   // (every thread of the row is past its last look at the row maxima)
-    xch[part * PS_ROWS + rloc] = l_run;
-    row_sync();
-    const float l_tot = live ? xch[rloc] + xch[PS_ROWS + rloc] : 0.f;
     if (T_tiles > 0 && !failed) failed = !mbar_wait(&bars[PS_ODONE], 0, WAIT_LIMIT);
-    fence_after_sync();
-    const bool whole = p.nsplit == 1, out_row = rho < p.Nq * p.G;   // (padding is written too)
-    const float inv = l_tot != 0.f ? (whole ? 1.f / l_tot : 1.f) : 0.f;
-    const uint32_t o_addr = tmem + lane_base + PS_TO + part * (D / 2);
-    T* orow = static_cast<T*>(p.o) + b * p.so.b + head * p.so.h + (int64_t)tok * p.so.n + part * (D / 2);
-    const int64_t slot = (int64_t)ub * p.nsplit + split;
-    float* prow = p.part_o + (slot * PS_ROWS + rloc) * D + part * (D / 2);
-#pragma unroll
-    for (int c0 = 0; c0 < D / 2; c0 += 16) {
-      uint32_t ov[16];
-      tmem_ld16(o_addr + c0, ov);
-      tmem_ld_wait();
-      float x[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = l_tot != 0.f ? __uint_as_float(ov[i]) * inv : 0.f;   // (without a visible key O may hold anything)
-      if (out_row && whole) {
-#pragma unroll
-        for (int i = 0; i < 16; i += 8)
-          *reinterpret_cast<uint4*>(orow + c0 + i) =
-              make_uint4(pack2<T>(x[i], x[i + 1]), pack2<T>(x[i + 2], x[i + 3]), pack2<T>(x[i + 4], x[i + 5]), pack2<T>(x[i + 6], x[i + 7]));
-      } else if (out_row) {
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(prow + c0 + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-      }
-    }
-    if (part == 0 && out_row) {
-      if (!whole) p.part_ml[(slot * PS_ROWS + rloc) * 2] = l_tot != 0.f ? m_run : -CUDART_INF_F, p.part_ml[(slot * PS_ROWS + rloc) * 2 + 1] = l_tot;
-      else if (p.lse) p.lse[((int64_t)b * p.H + head) * p.Nq + tok] = l_tot != 0.f ? m_run * LN2 + logf(l_tot) : -CUDART_INF_F;
-    }
-    if (!whole) {
-      // the CTA that finishes a row block last merges its parts
-      __threadfence();
-      all_sync();
-      if (tid == 0) *last_s = atomicAdd(p.done + ub, 1u) == (unsigned)p.nsplit - 1u;
-      all_sync();
-      if (*last_s) {
-        __threadfence();
-        float* wgt = reinterpret_cast<float*>(Ks);   // [split][128 rows] weights, then the rows' 1 / sum
-        const int64_t slot0 = (int64_t)ub * p.nsplit;
-        if (tid < PS_ROWS && out_row) {
-          float M = -CUDART_INF_F, L = 0.f;
-          for (int s = 0; s < p.nsplit; ++s) M = fmaxf(M, __ldcg(p.part_ml + ((slot0 + s) * PS_ROWS + rloc) * 2));
-          const float mu = M == -CUDART_INF_F ? 0.f : M;
-          for (int s = 0; s < p.nsplit; ++s) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.part_ml + ((slot0 + s) * PS_ROWS + rloc) * 2));
-            const float f = ex2_approx(ml.x - mu);
-            wgt[s * PS_ROWS + rloc] = f, L = fmaf(ml.y, f, L);
-          }
-          wgt[p.nsplit * PS_ROWS + rloc] = L != 0.f ? 1.f / L : 0.f;
-          if (p.lse) p.lse[((int64_t)b * p.H + head) * p.Nq + tok] = L != 0.f ? M * LN2 + logf(L) : -CUDART_INF_F;
-        }
-        all_sync();
-        for (int i = tid; i < PS_ROWS * (D / 4); i += 32 * PS_SM_WARPS) {
-          const int row = i / (D / 4), c4 = i - row * (D / 4), rr = rb * PS_ROWS + row, t = rr / p.G, h = hk + (rr - t * p.G) * p.Hk;
-          if (t >= p.Nq) break;
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-          for (int s = 0; s < p.nsplit; ++s) {
-            const float f = wgt[s * PS_ROWS + row];
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + ((slot0 + s) * PS_ROWS + row) * D + 4 * c4));
-            acc.x = fmaf(f, x.x, acc.x), acc.y = fmaf(f, x.y, acc.y), acc.z = fmaf(f, x.z, acc.z), acc.w = fmaf(f, x.w, acc.w);
-          }
-          const float f = wgt[p.nsplit * PS_ROWS + row];
-          *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + b * p.so.b + h * p.so.h + (int64_t)t * p.so.n + 4 * c4) =
-              make_uint2(pack2<T>(acc.x * f, acc.y * f), pack2<T>(acc.z * f, acc.w * f));
-        }
-      }
-    }
+    paged_epilogue<T, D>(p.e, tmem + PS_TO, xch, ub, split, b, hk, rb, live ? l_run : 0.f, m_run);
   }
   if (failed) atomicOr(p.status, 1u);
   fence_before_sync();
@@ -585,23 +545,23 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP 
 // ---- host side -----------------------------------------------------------------------------------------
 static int sweep_blocks(const PopeShape& s) { return (int)(((int64_t)s.Nq * (s.H / s.Hk) + PS_ROWS - 1) / PS_ROWS); }
 
-// Key ranges per row block: whole waves of one CTA per SM times a CTA's steps plus what it costs beside them (Q', the epilogue and the merge,
-// about ten steps' time).
+// Key ranges per row block: whole waves of one CTA per SM times a CTA's steps plus what it costs beside them (Q', the epilogue
+// and the merge, about ten steps' time).
 static int sweep_split(const PopeShape& s) {
   const int tiles = (s.Nk + PS_KEYS - 1) / PS_KEYS;
   const int64_t units = (int64_t)s.B * s.Hk * sweep_blocks(s);
   int best = 1;
   int64_t best_cost = INT64_MAX;
-  for (int n = 1; n <= std::min(tiles, PS_MAX_SPLIT); ++n) {
+  for (int n = 1; n <= std::min(tiles, PAGED_MAX_SPLIT); ++n) {
     const int64_t cost = (units * n + 147) / 148 * ((tiles + n - 1) / n + (n > 1 ? 10 : 6));
     if (cost < best_cost) best = n, best_cost = cost;
   }
   return best;
 }
 
-// workspace: [tables][K' images][16-bit V rows][counters][parts][their maxima and sums]
+// workspace: [tables][K' images][16-bit V rows][parts][their maxima and sums]
 struct SweepWs {
-  size_t kimg, vrows, done, part_o, part_ml, total;
+  size_t kimg, vrows, part_o, part_ml, total;
 };
 static SweepWs sweep_ws(const PopeShape& s, int store) {
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
@@ -610,8 +570,7 @@ static SweepWs sweep_ws(const PopeShape& s, int store) {
   SweepWs w;
   w.kimg = trig_tables_bytes(s.Nk, s.r);
   w.vrows = w.kimg + up(units * rows * (s.d + round_up(s.r, 16)) * 2);
-  w.done = w.vrows + (store == POPE_STORE_16 ? 0 : up(units * rows * s.d * 2));
-  w.part_o = w.done + up(blocks * sizeof(unsigned int));
+  w.part_o = w.vrows + (store == POPE_STORE_16 ? 0 : up(units * rows * s.d * 2));
   w.part_ml = w.part_o + up(parts * s.d * sizeof(float));
   w.total = w.part_ml + up(parts * 2 * sizeof(float));
   return w;
@@ -633,19 +592,17 @@ template <typename T, int STORE, int D> static cudaError_t paged_sweep_t(const P
   im.ch = static_cast<const __half*>(tt.ch), im.sh = static_cast<const __half*>(tt.sh);
   im.bias = a.embed.bias, im.bias_sh = a.embed.bias_stride_h;
   im.kimg = base + ws.kimg, im.vrows = base + ws.vrows;
-  im.done = reinterpret_cast<unsigned int*>(base + ws.done), im.ndone = s.B * s.Hk * sweep_blocks(s);
   PagedSweepP p = {};
-  p.H = s.H, p.Hk = s.Hk, p.G = s.H / s.Hk, p.Nq = s.Nq, p.Nk = s.Nk, p.r = s.r, p.RP = RP, p.tiles = tiles;
+  p.Hk = s.Hk, p.G = s.H / s.Hk, p.Nq = s.Nq, p.Nk = s.Nk, p.r = s.r, p.RP = RP, p.tiles = tiles;
   p.nsplit = sweep_split(s), p.blocks = sweep_blocks(s);
   p.page_size = kv.page_size, p.max_pages = kv.max_pages_per_seq, p.num_pages = kv.num_pages;
-  auto wide = [](const void* ptr, const PopeStride3& t) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && t.b % 8 == 0 && t.h % 8 == 0 && t.n % 8 == 0; };
-  p.q_wide = wide(a.q, a.sq);
+  p.q_wide = rows_wide(a.q, a.sq);
   p.scale_log2 = std::abs(a.softmax_scale) * LOG2E, p.q_sign = a.softmax_scale < 0.f ? 0x80008000u : 0u;
   p.page_table = kv.page_table, p.seq_lens = kv.seq_lens, p.counts = a.counts;
-  p.q = a.q, p.o = a.out, p.lse = a.lse, p.sq = Strides(a.sq), p.so = Strides(a.so);
+  p.q = a.q, p.sq = Strides(a.sq);
   p.kimg = im.kimg, p.ch = im.ch, p.sh = im.sh;
-  p.part_o = reinterpret_cast<float*>(base + ws.part_o), p.part_ml = reinterpret_cast<float*>(base + ws.part_ml);
-  p.done = im.done, p.status = im.c.status;
+  p.e = paged_out(a, p.nsplit, reinterpret_cast<float*>(base + ws.part_o), reinterpret_cast<float*>(base + ws.part_ml));
+  p.status = im.c.status;
   CUtensorMap tmap_v;
   const int rows = tiles * IMAGE_ROWS;
   const int64_t page = (int64_t)kv.page_size * s.d;
@@ -661,7 +618,8 @@ template <typename T, int STORE, int D> static cudaError_t paged_sweep_t(const P
   if (s.r > 0 && (e = launch_paged_tables(a.embed, s.Nk, s.r, tt.ch, tt.sh, nullptr, 0, st)) != cudaSuccess) return e;
   const size_t ismem = (size_t)(KD / 8) * CS64 + 2 * (size_t)s.r * sizeof(float);
   if ((e = launch_dependent(paged_image_kernel<T, STORE, D>, dim3((unsigned)((s.Nk + 127) / 128 * 2), (unsigned)(s.B * s.Hk)), dim3(256), ismem, st, im)) != cudaSuccess) return e;
-  return launch_dependent(paged_sweep_kernel<T, D, Q8>, dim3((unsigned)(s.B * s.Hk * p.blocks * p.nsplit)), dim3(PS_THREADS), smem, st, p, tmap_v);
+  e = launch_dependent(paged_sweep_kernel<T, D, Q8>, dim3((unsigned)(s.B * s.Hk * p.blocks * p.nsplit)), dim3(PS_THREADS), smem, st, p, tmap_v);
+  return e != cudaSuccess || p.nsplit == 1 ? e : launch_paged_merge(p.e, s.dtype, s.d, s.B * s.Hk * p.blocks, p.blocks, st);
 }
 template <typename T, int STORE> static cudaError_t paged_sweep_d(const PopePagedAttnArgs& a, cudaStream_t st) {
   const int d = a.shape.d;
@@ -678,7 +636,7 @@ cudaError_t paged_sweep(const PopePagedAttnArgs& a, cudaStream_t st) {
   return a.shape.dtype == POPE_BF16 ? paged_sweep_s<__nv_bfloat16>(a, st) : paged_sweep_s<__half>(a, st);
 }
 
-// ---- which of the two ------------------------------------------------------------------------------------
+// ---- which kernel ----------------------------------------------------------------------------------------
 bool attn_paged_supported(const PopePagedAttnArgs& a) {
   const PopeShape& s = a.shape;
   if (s.dtype != POPE_BF16 && s.dtype != POPE_F16) return false;
@@ -687,11 +645,28 @@ bool attn_paged_supported(const PopePagedAttnArgs& a) {
   return a.cache.kv.page_size % 64 == 0;
 }
 
-// Rows that share a key head, up to which one pass over the keys per block of 32 is taken
-static bool few_rows(const PopeShape& s) { return (int64_t)s.Nq * (s.H / s.Hk) <= 64; }
+enum class Paged { kRows, kStream, kSweep };
+static Paged paged_kernel(const PopeShape& s) {
+  const int64_t rows = (int64_t)s.Nq * (s.H / s.Hk);
+  const char* e = getenv("PAGED_PATH");
+  if (e) return e[0] == '0' ? Paged::kRows : e[0] == '1' ? Paged::kStream : Paged::kSweep;
+  return rows <= 16 ? Paged::kRows : rows <= 256 ? Paged::kStream : Paged::kSweep;
+}
 
-size_t attn_paged_workspace(const PopePagedAttnArgs& a) { return few_rows(a.shape) ? paged_rows_workspace(a) : paged_sweep_workspace(a); }
+size_t attn_paged_workspace(const PopePagedAttnArgs& a) {
+  switch (paged_kernel(a.shape)) {
+    case Paged::kRows: return paged_rows_workspace(a);
+    case Paged::kStream: return paged_stream_workspace(a);
+    default: return paged_sweep_workspace(a);
+  }
+}
 
-cudaError_t attn_paged(const PopePagedAttnArgs& a, cudaStream_t st) { return few_rows(a.shape) ? paged_rows(a, st) : paged_sweep(a, st); }
+cudaError_t attn_paged(const PopePagedAttnArgs& a, cudaStream_t st) {
+  switch (paged_kernel(a.shape)) {
+    case Paged::kRows: return paged_rows(a, st);
+    case Paged::kStream: return paged_stream(a, st);
+    default: return paged_sweep(a, st);
+  }
+}
 
 }  // namespace pope

@@ -1,0 +1,562 @@
+// Attention of a MODERATE number of new tokens per sequence over a paged cache on the Blackwell tensor cores (tcgen05 + TMEM), sm_100a only: the rows
+// of a key head fill one or two blocks of 128, so that writing expanded keys to memory for them (tc_attn_paged.cu) would cost more than they do.
+//
+// One pass over K and V per row block, 64 keys a step, everything else on the chip:
+//   2 loader warps  : K rows with the fp16 cos / sin rows, and V rows (and row scales), each into a ring of stages of its own, by tensor-map copies
+//                     in 128-byte-swizzled rows.  (In one ring a stage stays until its V has been used, and the expanders waited for
+//                     copies a third of the time: 121 us instead of @@ at 64 new tokens of 32 / 8 heads over 32768 keys.)
+//   8 expander warps: K' = [a cos | plain | a sin], a = softplus, out of the stage into one of two operand tiles (the head's phase bias sits in Q');
+//                     of a cache that holds 8 bits also V as 16-bit values
+//   score warp      : S = Q' K'^T, Q' in tensor memory, into one of two buffers
+//   8 softmax warps : two threads per row, online softmax, P over S
+//   PV warp         : O += P V, V from its stage (16 bits) or the expanders' tile (8 bits)
+// The step is bound by instruction issue of the expanders and the softmax (about 60 warp instructions a key at r = 64) next to the 512 bytes
+// of K and V a key at 16 bits.  Small grids are cut along the keys as in tc_attn_paged.cu.
+#include <algorithm>
+#include <type_traits>
+
+#include "kernels.h"
+#include "paged.cuh"
+#include "paged_out.cuh"
+
+namespace pope {
+
+struct PagedStreamP {
+  int Hk, G, Nq, Nk, r, RP, nsplit, blocks, kstages, vstages;
+  int page_size, max_pages, num_pages, q_wide;
+  float scale_log2;          // its magnitude; the sign sits in Q'
+  uint32_t q_sign;
+  const int32_t *page_table, *seq_lens, *counts;
+  const void* q;
+  Strides sq;
+  const __half *ch, *sh;     // fp16 cos / sin, [Nk][r]
+  const float* bias;
+  int64_t bias_sh;
+  PagedOut e;
+  unsigned int* status;
+};
+
+constexpr int SK_KEYS = 64;
+constexpr int SK_EX = PAGED_SM_WARPS, SK_EX_WARPS = 8, SK_EX_THREADS = 32 * SK_EX_WARPS;   // first expander warp
+constexpr int SK_KLOAD = SK_EX + SK_EX_WARPS, SK_VLOAD = SK_KLOAD + 1, SK_S = SK_KLOAD + 2, SK_PV = SK_KLOAD + 3;
+constexpr int SK_THREADS = 32 * (SK_PV + 1);
+constexpr int SK_CS = SK_KEYS * 16 + 16;           // chunk stride of an operand tile: the padding keeps the expanders' stores on distinct banks
+constexpr uint32_t SK_TS = 128, SK_TO = 256;       // first TMEM column of the S / P buffers and of O (Q' starts at 0)
+constexpr int SK_BLOCK = SK_KEYS * 128;            // bytes of 128-byte rows of a step
+constexpr int SK_MAX_STAGES = 4;
+enum {
+  SK_KREADY = 0,    // [2] the expanders: K' (and V at 8 bits) of the step is in its tile
+  SK_KFREE = 2,     // [2] S of the step has completed: the K' tile may be rewritten
+  SK_SFULL = 4,     // [2] the scores are in TMEM
+  SK_PFULL = 6,     // [2] the softmax warps: the probabilities are in TMEM
+  SK_PVDONE = 8,    // [2] O += P V of the step has completed
+  SK_QFULL = 10,
+  SK_ODONE = 11,
+  SK_KFULL = 12,                           // [kstages] K, its phases and scales have landed
+  SK_KEMPTY = SK_KFULL + SK_MAX_STAGES,    // [kstages] the expanders have read them
+  SK_VFULL = SK_KEMPTY + SK_MAX_STAGES,    // [vstages] V has landed
+  SK_VEMPTY = SK_VFULL + SK_MAX_STAGES,    // [vstages] its stage may be refilled: O += P V has completed (16 bits), the expanders have read it (8 bits)
+  SK_COUNT = SK_VEMPTY + SK_MAX_STAGES
+};
+
+template <typename T, int STORE, int D>
+__global__ void __launch_bounds__(SK_THREADS, 1)
+    paged_stream_kernel(PagedStreamP p, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                        const __grid_constant__ CUtensorMap tmap_t, const __grid_constant__ CUtensorMap tmap_ks, const __grid_constant__ CUtensorMap tmap_vs) {
+  constexpr bool Q8 = STORE != POPE_STORE_16;
+  constexpr bool BF = std::is_same_v<T, __nv_bfloat16>;   // its magnitudes come in units of ln 2; fp16 keeps to its own range
+  constexpr int DC = D / 8, KBLK = (D * (Q8 ? 1 : 2) + 127) / 128;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const int r = p.r, RC = r / 8, tblk = (r + 63) / 64, KC = DC + p.RP / 8, KSTEPS = KC / 2;
+  constexpr int trig_at = KBLK * SK_BLOCK, vscale_at = KBLK * SK_BLOCK, vstage = vscale_at + (Q8 ? 1024 : 0);
+  const int scale_at = trig_at + 2 * tblk * SK_BLOCK, kstage = scale_at + (Q8 ? 1024 : 0);
+  uint8_t* vring = smem + p.kstages * kstage;
+  uint8_t* Ks = vring + p.vstages * vstage;                        // [2][KC][SK_CS]
+  uint8_t* Vs = Ks + 2 * KC * SK_CS;                               // 8 bits: [2][DC][SK_CS]
+  float* xch = reinterpret_cast<float*>(Vs + (Q8 ? 2 * DC * SK_CS : 0));   // [2 step parities][2 parts][128 rows] row maxima
+  float* bias_cs = xch + 4 * PAGED_ROWS;                           // [2][r]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(bias_cs + 2 * r);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + SK_COUNT);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (warp == SK_S) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  if (tid == 0) {
+    for (int i = 0; i < SK_COUNT; ++i) {
+      const bool ex = i < SK_KREADY + 2 || (i >= SK_KEMPTY && i < SK_VFULL) || (Q8 && i >= SK_VEMPTY), sm = i == SK_PFULL || i == SK_PFULL + 1 || i == SK_QFULL;
+      mbar_init(&bars[i], ex ? SK_EX_WARPS : sm ? PAGED_SM_WARPS : 1);
+    }
+    mbar_init_fence();
+  }
+  pdl_wait();
+  pdl_trigger();
+  // unit (sequence, key head), row block (late ones, which see more keys, first), key range
+  const int split = blockIdx.x % p.nsplit, ub = blockIdx.x / p.nsplit, u = ub / p.blocks, rb = p.blocks - 1 - ub % p.blocks;
+  const int b = u / p.Hk, hk = u % p.Hk;
+  const int len = max(0, min(p.seq_lens[b], p.Nk)), cnt = p.counts ? max(0, min(p.counts[b], p.Nq)) : p.Nq;
+  const int rows = min(PAGED_ROWS, cnt * p.G - rb * PAGED_ROWS);                       // of this block that are queries
+  const int first_pos = len - cnt + rb * PAGED_ROWS / p.G;                             // position of the first one
+  const int kend = rows > 0 ? max(0, min(len, len - cnt + (rb * PAGED_ROWS + rows - 1) / p.G + 1)) : 0;
+  const int tiles_all = (kend + SK_KEYS - 1) / SK_KEYS;
+  const int t0 = (int)((int64_t)tiles_all * split / p.nsplit), T_tiles = (int)((int64_t)tiles_all * (split + 1) / p.nsplit) - t0;
+  for (int i = tid; i < r; i += SK_THREADS) sincos_reduced(p.bias[hk * p.bias_sh + i], &bias_cs[r + i], &bias_cs[i]);
+  if (RC * 8 < p.RP)   // the zero column behind the sines
+    for (int i = tid; i < 2 * SK_KEYS; i += SK_THREADS)
+      *reinterpret_cast<uint4*>(Ks + (i / SK_KEYS * KC + DC + RC) * SK_CS + i % SK_KEYS * 16) = make_uint4(0, 0, 0, 0);
+  fence_async_smem();
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  bool failed = false;
+
+  if (warp == SK_KLOAD || warp == SK_VLOAD) {
+    const bool is_k = warp == SK_KLOAD;
+    const int stages = is_k ? p.kstages : p.vstages, fulls = is_k ? SK_KFULL : SK_VFULL, empties = is_k ? SK_KEMPTY : SK_VEMPTY;
+    int page = 0;
+    for (int j = 0, s = 0, par = 0; j < T_tiles; ++j) {
+      if ((j & 31) == 0) {   // lane l: the page of step j + l; one outside the pool is never dereferenced (clamped, status bit 1)
+        const int key = (t0 + j + lane) * SK_KEYS, lp = key / p.page_size;
+        page = 0;
+        if (key < kend) {
+          page = lp < p.max_pages ? p.page_table[(int64_t)b * p.max_pages + lp] : -1;
+          if (page < 0 || page >= p.num_pages) page = 0, atomicOr(p.status, 2u);
+        }
+      }
+      const int pg = __shfl_sync(0xffffffffu, page, j & 31);
+      if (lane == 0) {
+        if (j >= stages) failed = !mbar_wait(&bars[empties + s], par ^ 1, WAIT_LIMIT);
+        if (failed) {
+          drain_copies(&bars[fulls], stages, j - stages, j);
+        } else {
+          const int key0 = (t0 + j) * SK_KEYS, row = key0 % p.page_size;
+          uint64_t* bar = &bars[fulls + s];
+          if (is_k) {
+            uint8_t* st = smem + s * kstage;
+            mbar_expect_tx(bar, (uint32_t)(scale_at + (Q8 ? 4 * SK_KEYS : 0)));
+#pragma unroll
+            for (int c = 0; c < KBLK; ++c) tma_load_4d(st + c * SK_BLOCK, &tmap_k, bar, c * 128, row, hk, pg);
+            for (int c = 0; c < tblk; ++c) tma_load_4d(st + trig_at + 2 * c * SK_BLOCK, &tmap_t, bar, c * 64, key0, 0, 0);
+            if constexpr (Q8) tma_load_4d(st + scale_at, &tmap_ks, bar, row, hk, pg, 0);
+          } else {
+            uint8_t* st = vring + s * vstage;
+            mbar_expect_tx(bar, (uint32_t)(vscale_at + (Q8 ? 4 * SK_KEYS : 0)));
+#pragma unroll
+            for (int c = 0; c < KBLK; ++c) tma_load_4d(st + c * SK_BLOCK, &tmap_v, bar, c * 128, row, hk, pg);
+            if constexpr (Q8) tma_load_4d(st + vscale_at, &tmap_vs, bar, row, hk, pg, 0);
+          }
+        }
+      }
+      failed = __shfl_sync(0xffffffffu, (int)failed, 0) != 0;
+      if (failed) break;
+      if (++s == stages) s = 0, par ^= 1;
+    }
+  } else if (warp == SK_S) {
+    if (lane == 0) {
+      const uint32_t idesc = instr_desc(TcFmt<T>::fmt, PAGED_ROWS, SK_KEYS, false, false);
+      const uint32_t ks_addr = smem_u32(Ks);
+      failed = !mbar_wait(&bars[SK_QFULL], 0, WAIT_LIMIT);
+      for (int j = 0; j < T_tiles && !failed; ++j) {
+        const int buf = j & 1;
+        failed = !mbar_wait(&bars[SK_KREADY + buf], (j >> 1) & 1, WAIT_LIMIT);
+        if (j >= 2 && !failed) failed = !mbar_wait(&bars[SK_PVDONE + buf], ((j - 2) >> 1) & 1, WAIT_LIMIT);
+        if (failed) break;
+        fence_after_sync();
+        const uint64_t bd = smem_desc(ks_addr + buf * KC * SK_CS, SK_CS, 128);
+        uint32_t blo = desc_lo(bd), at = tmem;
+#pragma unroll 4
+        for (int ks = 0; ks < KSTEPS; ++ks) {
+          mma_ts_lh(tmem + SK_TS + buf * SK_KEYS, at, blo, desc_hi(bd), idesc, ks > 0 ? 1u : 0u);
+          at += 8, blo += (2 * SK_CS) >> 4;
+        }
+        mma_commit(&bars[SK_SFULL + buf]);
+        mma_commit(&bars[SK_KFREE + buf]);
+      }
+    }
+    __syncwarp();
+  } else if (warp == SK_PV) {
+    if (lane == 0) {
+      const uint32_t idesc = instr_desc(TcFmt<T>::fmt, PAGED_ROWS, D, false, true);
+      for (int j = 0, s = 0, par = 0; j < T_tiles && !failed; ++j) {
+        const int buf = j & 1;
+        // (at 8 bits V is the expanders', and its stage may already be in its next use)
+        if constexpr (!Q8) failed = !mbar_wait(&bars[SK_VFULL + s], par, WAIT_LIMIT);
+        if (!failed) failed = !mbar_wait(&bars[SK_PFULL + buf], (j >> 1) & 1, WAIT_LIMIT);
+        if (failed) break;
+        fence_after_sync();
+        const uint32_t a = tmem + SK_TS + buf * SK_KEYS;
+        // B = V, MN-major.  16 bits: 64-feature blocks 8 KB apart, 8-key groups 1 KB, 16 keys 2 KB, swizzled; 8 bits: 8-feature chunks SK_CS apart,
+        // 8-key groups 128 bytes, 16 keys 256 bytes
+        const uint64_t bd = Q8 ? smem_desc(smem_u32(Vs) + buf * DC * SK_CS, 128, SK_CS) : smem_desc_sw128(smem_u32(vring) + s * vstage, SK_BLOCK, 1024);
+        constexpr uint32_t kstep = (Q8 ? 256 : 2048) >> 4;
+#pragma unroll
+        for (int ks = 0; ks < SK_KEYS / 16; ++ks)   // P of keys [32 t, 32 t + 32) sits in the first 16 columns of part t
+          mma_ts_lh(tmem + SK_TO, a + (ks * 16 / 32) * 32 + (ks * 16 % 32) / 2, desc_lo(bd) + ks * kstep, desc_hi(bd), idesc, (j > 0 || ks > 0) ? 1u : 0u);
+        if (j == T_tiles - 1) mma_commit(&bars[SK_ODONE]);
+        mma_commit(&bars[SK_PVDONE + buf]);
+        if constexpr (!Q8) mma_commit(&bars[SK_VEMPTY + s]);
+        if (++s == p.vstages) s = 0, par ^= 1;
+      }
+    }
+    __syncwarp();
+  } else if (warp >= SK_EX) {
+    // =============================== expanders =====================================================
+    const int et = tid - 32 * SK_EX;
+    // rotated and plain 16-byte columns are dealt out separately: a warp has one kind or the other
+    const int PC = DC - RC;
+    const int rdiv = max(RC, 1), pdiv = max(PC, 1);
+    const int rrow = et / rdiv, rcol = et % rdiv, rrow_step = SK_EX_THREADS / rdiv, rcol_step = SK_EX_THREADS % rdiv;
+    const int prow = et / pdiv, pcol = et % pdiv, prow_step = SK_EX_THREADS / pdiv, pcol_step = SK_EX_THREADS % pdiv;
+    for (int j = 0, s = 0, par = 0, vs = 0, vpar = 0; j < T_tiles; ++j) {   // (vs, vpar: 8 bits)
+      const int buf = j & 1;
+      const uint8_t* st = smem + s * kstage;
+      const float* scl = reinterpret_cast<const float*>(st + scale_at);
+      failed = !mbar_wait(&bars[SK_KFULL + s], par, WAIT_LIMIT);
+      if (j >= 2 && !failed) failed = !mbar_wait(&bars[SK_KFREE + buf], ((j - 2) >> 1) & 1, WAIT_LIMIT);
+      if (failed) break;
+      uint8_t* kt = Ks + buf * KC * SK_CS;
+      auto swizzled = [&](const uint8_t* base, int row, int byte) {   // 16 (or 8) bytes of a 128-byte-swizzled row
+        return base + (byte >> 7) * SK_BLOCK + row * 128 + ((((byte >> 4) & 7) ^ (row & 7)) << 4) + (byte & 15);
+      };
+      using Raw = std::conditional_t<Q8, uint2, uint4>;   // eight features
+      auto raw_of = [&](const uint8_t* base, int row, int c) { return *reinterpret_cast<const Raw*>(swizzled(base, row, c * (Q8 ? 8 : 16))); };
+      auto values = [&](const Raw& w, float scale, float2 (&x)[4]) {
+        if constexpr (Q8) {
+          float lo[4], hi[4];
+          codes_to_f32<STORE>(w.x, lo), codes_to_f32<STORE>(w.y, hi);
+          const float2 f = make_float2(scale, scale);
+          x[0] = mul2(make_float2(lo[0], lo[1]), f), x[1] = mul2(make_float2(lo[2], lo[3]), f);
+          x[2] = mul2(make_float2(hi[0], hi[1]), f), x[3] = mul2(make_float2(hi[2], hi[3]), f);
+        } else {
+          x[0] = unpack2<T>(w.x), x[1] = unpack2<T>(w.y), x[2] = unpack2<T>(w.z), x[3] = unpack2<T>(w.w);
+        }
+      };
+      // two groups of eight at a time: their chains of special functions overlap
+      for (int row = rrow, c = rcol; row < SK_KEYS && RC > 0;) {
+        int rw[2], cl[2];
+        bool on[2];
+        Raw raw[2];
+        uint4 cq[2], sq[2];
+        float f[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          rw[k] = row, cl[k] = c, on[k] = row < SK_KEYS;
+          if (!on[k]) rw[k] = SK_KEYS - 1;
+          raw[k] = raw_of(st, rw[k], cl[k]);
+          const uint8_t* trow = st + trig_at + (cl[k] >> 3) * 2 * SK_BLOCK + rw[k] * 128 + (((cl[k] & 7) ^ (rw[k] & 7)) << 4);
+          cq[k] = *reinterpret_cast<const uint4*>(trow), sq[k] = *reinterpret_cast<const uint4*>(trow + SK_BLOCK);
+          f[k] = Q8 ? scl[rw[k]] : 1.f;
+          row += rrow_step, c += rcol_step;
+          if (c >= rdiv) c -= rdiv, ++row;
+        }
+        float2 a[2][4];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          values(raw[k], f[k], a[k]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 y = mul2(a[k][e], make_float2(LOG2E, LOG2E));
+            const float2 v = add2(make_float2(ex2_approx(-fabsf(y.x)), ex2_approx(-fabsf(y.y))), make_float2(1.f, 1.f));
+            a[k][e] = add2(make_float2(lg2_approx(v.x), lg2_approx(v.y)), make_float2(fmaxf(y.x, 0.f), fmaxf(y.y, 0.f)));
+            if constexpr (!BF) a[k][e] = mul2(a[k][e], make_float2(LN2, LN2));
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t cw[4] = {cq[k].x, cq[k].y, cq[k].z, cq[k].w}, sw[4] = {sq[k].x, sq[k].y, sq[k].z, sq[k].w};
+          uint32_t o1[4], o2[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (!BF) {
+              const uint32_t h = pack2<__half>(a[k][e].x, a[k][e].y);
+              const __half2 c2 = __hmul2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&cw[e]));
+              const __half2 s2 = __hmul2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&sw[e]));
+              o1[e] = *reinterpret_cast<const uint32_t*>(&c2), o2[e] = *reinterpret_cast<const uint32_t*>(&s2);
+            } else {
+              const float2 c2 = mul2(a[k][e], unpack2<__half>(cw[e])), s2 = mul2(a[k][e], unpack2<__half>(sw[e]));
+              o1[e] = pack2<T>(c2.x, c2.y), o2[e] = pack2<T>(s2.x, s2.y);
+            }
+          }
+          if (on[k]) {
+            *reinterpret_cast<uint4*>(kt + cl[k] * SK_CS + rw[k] * 16) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
+            *reinterpret_cast<uint4*>(kt + (DC + cl[k]) * SK_CS + rw[k] * 16) = make_uint4(o2[0], o2[1], o2[2], o2[3]);
+          }
+        }
+      }
+      auto as_16 = [&](const Raw& w, float scale) {
+        if constexpr (Q8) {
+          float2 x[4];
+          values(w, scale, x);
+          return make_uint4(pack2<T>(x[0].x, x[0].y), pack2<T>(x[1].x, x[1].y), pack2<T>(x[2].x, x[2].y), pack2<T>(x[3].x, x[3].y));
+        } else {
+          return w;
+        }
+      };
+      for (int row = prow, c = pcol; row < SK_KEYS && PC > 0;) {
+        *reinterpret_cast<uint4*>(kt + (RC + c) * SK_CS + row * 16) = as_16(raw_of(st, row, RC + c), Q8 ? scl[row] : 1.f);
+        row += prow_step, c += pcol_step;
+        if (c >= pdiv) c -= pdiv, ++row;
+      }
+      fence_async_smem();   // the tile is visible to the tensor core; the stage has been read
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[SK_KEMPTY + s]);
+      if constexpr (Q8) {   // V's values, zeros behind the last key
+        failed = !mbar_wait(&bars[SK_VFULL + vs], vpar, WAIT_LIMIT);
+        if (j >= 2 && !failed) failed = !mbar_wait(&bars[SK_PVDONE + buf], ((j - 2) >> 1) & 1, WAIT_LIMIT);
+        if (failed) break;
+        const int live = kend - (t0 + j) * SK_KEYS;
+        const uint8_t* vst = vring + vs * vstage;
+        uint8_t* vt = Vs + buf * DC * SK_CS;
+        const float* vscl = reinterpret_cast<const float*>(vst + vscale_at);
+        for (int i = et; i < SK_KEYS * DC; i += SK_EX_THREADS) {
+          const int row = i / DC, c = i % DC;
+          *reinterpret_cast<uint4*>(vt + c * SK_CS + row * 16) = row < live ? as_16(raw_of(vst, row, c), vscl[row]) : make_uint4(0, 0, 0, 0);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[SK_VEMPTY + vs]);
+        if (++vs == p.vstages) vs = 0, vpar ^= 1;
+      }
+      if (lane == 0) mbar_arrive(&bars[SK_KREADY + buf]);
+      if (++s == p.kstages) s = 0, par ^= 1;
+    }
+  } else {
+    // =============================== softmax: two threads per query row ==========================
+    const int rloc = tid & 127, part = tid >> 7;
+    const int rho = rb * PAGED_ROWS + rloc, tok = rho / p.G, head = hk + (rho - tok * p.G) * p.Hk, pos = len - cnt + tok;
+    const bool live = rloc < rows && pos >= 0, warp_live = (warp & 3) * 32 < rows;   // (warps without a query only keep the steps' pace)
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const int row_bar = 1 + (warp & 3);   // named barrier of the two warps that share 32 rows
+    auto row_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(row_bar) : "memory"); };
+    {
+      // Q' = [a cos(f - b) | plain | a sin(f - b)], straight into tensor memory; rows that are no queries are zero
+      const T* qrow = static_cast<const T*>(p.q) + b * p.sq.b + head * p.sq.h + (int64_t)tok * p.sq.n;
+      const int64_t trow = (int64_t)pos * r;
+      for (int c = part; c < DC; c += 2) {
+        uint32_t rw[4] = {0, 0, 0, 0};
+        if (live && p.q_wide) {
+          const uint4 raw = *reinterpret_cast<const uint4*>(qrow + c * 8);
+          rw[0] = raw.x, rw[1] = raw.y, rw[2] = raw.z, rw[3] = raw.w;
+        } else if (live) {
+          const uint16_t* q16 = reinterpret_cast<const uint16_t*>(qrow + c * 8);
+          for (int e = 0; e < 4; ++e) rw[e] = q16[2 * e] | (uint32_t)q16[2 * e + 1] << 16;
+        }
+        if (c < RC) {
+          uint4 cq = make_uint4(0, 0, 0, 0), sq = cq;
+          if (live) {
+            cq = *reinterpret_cast<const uint4*>(p.ch + trow + c * 8);
+            sq = *reinterpret_cast<const uint4*>(p.sh + trow + c * 8);
+          }
+          const uint32_t cw[4] = {cq.x, cq.y, cq.z, cq.w}, sw[4] = {sq.x, sq.y, sq.z, sq.w};
+          uint32_t o1[4], o2[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 xv = unpack2<T>(rw[e]), cv = unpack2<__half>(cw[e]), sv = unpack2<__half>(sw[e]);
+            const float2 bc = *reinterpret_cast<const float2*>(bias_cs + c * 8 + 2 * e), bs = *reinterpret_cast<const float2*>(bias_cs + r + c * 8 + 2 * e);
+            const float unit = BF ? LN2 : 1.f;
+            const float a0 = live ? softplus_fast(xv.x) * unit : 0.f, a1 = live ? softplus_fast(xv.y) * unit : 0.f;
+            o1[e] = pack2<T>(a0 * (cv.x * bc.x + sv.x * bs.x), a1 * (cv.y * bc.y + sv.y * bs.y)) ^ p.q_sign;
+            o2[e] = pack2<T>(a0 * (sv.x * bc.x - cv.x * bs.x), a1 * (sv.y * bc.y - cv.y * bs.y)) ^ p.q_sign;
+          }
+          tmem_st4(tmem + lane_base + c * 4, o1[0], o1[1], o1[2], o1[3]);
+          tmem_st4(tmem + lane_base + (DC + c) * 4, o2[0], o2[1], o2[2], o2[3]);
+        } else {
+          tmem_st4(tmem + lane_base + c * 4, rw[0] ^ p.q_sign, rw[1] ^ p.q_sign, rw[2] ^ p.q_sign, rw[3] ^ p.q_sign);
+        }
+      }
+      if (RC * 8 < p.RP && part == 0) tmem_st4(tmem + lane_base + (DC + RC) * 4, 0, 0, 0, 0);
+      tmem_st_wait();
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[SK_QFULL]);
+    }
+    float m_run = -CUDART_INF_F, l_run = 0.f;
+    const int limit = live ? min(pos, kend - 1) : -1;   // last key that this row sees
+
+    for (int j = 0; j < T_tiles; ++j) {
+      const int buf = j & 1, key0 = (t0 + j) * SK_KEYS, n0 = key0 + part * 32;   // first key of this thread's columns
+      if (!failed) failed = !mbar_wait(&bars[SK_SFULL + buf], (j >> 1) & 1, WAIT_LIMIT);
+      fence_after_sync();
+      if (warp_live) {
+        const bool all_vis = key0 + SK_KEYS <= min(kend, first_pos + 1);   // (rows that are no queries are dropped at the end)
+        const int lim = limit - n0;
+        const uint32_t vis = lim >= 31 ? ~0u : (lim < 0 ? 0u : ((2u << lim) - 1u));
+        const uint32_t s_addr = tmem + lane_base + SK_TS + buf * SK_KEYS + part * 32;
+        uint32_t sv[32];
+        tmem_ld32(s_addr, sv);
+        tmem_ld_wait();
+        float m4[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+        if (all_vis) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) m4[(i >> 1) & 3] = max3(m4[(i >> 1) & 3], __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if ((vis >> i) & 1u) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(sv[i]));
+        }
+        float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+        xch[(buf * 2 + part) * PAGED_ROWS + rloc] = mx;
+        row_sync();
+        mx = fmaxf(mx, xch[(buf * 2 + 1 - part) * PAGED_ROWS + rloc]);
+        const float m_new = fmaxf(m_run, mx == -CUDART_INF_F ? mx : mx * p.scale_log2);
+        const bool need = m_new > m_run + 8.f;   // a stale maximum is kept while it is within 2^8 of the true one
+        float alpha = 1.f;
+        if (need) {
+          alpha = ex2_approx(m_run - m_new);
+          l_run *= alpha;
+          m_run = m_new;
+        }
+        if (j > 0 && __any_sync(0xffffffffu, need)) {
+          if (!failed) failed = !mbar_wait(&bars[SK_PVDONE + (1 - buf)], ((j - 1) >> 1) & 1, WAIT_LIMIT);
+          fence_after_sync();
+          const uint32_t o_addr = tmem + lane_base + SK_TO + part * (D / 2);
+#pragma unroll
+          for (int c0 = 0; c0 < D / 2; c0 += 16) {
+            uint32_t ov[16];
+            tmem_ld16(o_addr + c0, ov);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+            tmem_st16(o_addr + c0, ov);
+          }
+          tmem_st_wait();
+        }
+        const float m_use = m_run == -CUDART_INF_F ? 0.f : m_run;
+        float ls2[2] = {0.f, 0.f};
+        uint32_t pk[16];
+        auto exponentials = [&](auto masked) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float p0 = ex2_approx(fmaf(__uint_as_float(sv[2 * i]), p.scale_log2, -m_use));
+            float p1 = ex2_approx(fmaf(__uint_as_float(sv[2 * i + 1]), p.scale_log2, -m_use));
+            if (decltype(masked)::value) {
+              p0 = ((vis >> (2 * i)) & 1u) ? p0 : 0.f;
+              p1 = ((vis >> (2 * i + 1)) & 1u) ? p1 : 0.f;
+            }
+            ls2[i & 1] += p0 + p1;
+            pk[i] = pack2<T>(p0, p1);
+          }
+        };
+        if (all_vis) exponentials(std::false_type());
+        else exponentials(std::true_type());
+        l_run += ls2[0] + ls2[1];
+        tmem_st16(s_addr, pk);
+        tmem_st_wait();
+      }
+      if (!Q8 && key0 + SK_KEYS > kend) {   // rows of V behind the last key may hold anything, and 0 * NaN is NaN (the last step)
+        if (!failed) failed = !mbar_wait(&bars[SK_VFULL + j % p.vstages], (j / p.vstages) & 1, WAIT_LIMIT);
+        const int dead = key0 + SK_KEYS - kend;
+        for (int i = tid; i < dead * KBLK * 8; i += 32 * PAGED_SM_WARPS)
+          *reinterpret_cast<uint4*>(vring + j % p.vstages * vstage + (i / 8 / dead) * SK_BLOCK + (SK_KEYS - dead + i / 8 % dead) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+        fence_async_smem();
+      }
+      fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[SK_PFULL + buf]);
+    }
+    if (T_tiles > 0 && !failed) failed = !mbar_wait(&bars[SK_ODONE], 0, WAIT_LIMIT);
+    paged_epilogue<T, D>(p.e, tmem + SK_TO, xch, ub, split, b, hk, rb, live ? l_run : 0.f, m_run);
+  }
+  if (failed) atomicOr(p.status, 1u);
+  fence_before_sync();
+  __syncthreads();
+  if (warp == SK_S) tmem_dealloc(tmem, 512);
+}
+
+// ---- host side -----------------------------------------------------------------------------------------
+static int stream_blocks(const PopeShape& s) { return (int)(((int64_t)s.Nq * (s.H / s.Hk) + PAGED_ROWS - 1) / PAGED_ROWS); }
+
+// Key ranges per row block: whole waves of one CTA per SM times a CTA's steps plus what it costs beside them (about twelve steps' time).
+static int stream_split(const PopeShape& s) {
+  const int tiles = (s.Nk + SK_KEYS - 1) / SK_KEYS;
+  const int64_t units = (int64_t)s.B * s.Hk * stream_blocks(s);
+  int best = 1;
+  int64_t best_cost = INT64_MAX;
+  for (int n = 1; n <= std::min(tiles, PAGED_MAX_SPLIT); ++n) {
+    const int64_t cost = (units * n + 147) / 148 * ((tiles + n - 1) / n + (n > 1 ? 12 : 8));
+    if (cost < best_cost) best = n, best_cost = cost;
+  }
+  return best;
+}
+
+// workspace: [tables][parts][their maxima and sums]
+struct StreamWs {
+  size_t part_o, part_ml, total;
+};
+static StreamWs stream_ws(const PopeShape& s) {
+  auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+  const size_t blocks = (size_t)s.B * s.Hk * stream_blocks(s), parts = stream_split(s) > 1 ? blocks * stream_split(s) * PAGED_ROWS : 0;
+  StreamWs w;
+  w.part_o = trig_tables_bytes(s.Nk, s.r);
+  w.part_ml = w.part_o + up(parts * s.d * sizeof(float));
+  w.total = w.part_ml + up(parts * 2 * sizeof(float));
+  return w;
+}
+size_t paged_stream_workspace(const PopePagedAttnArgs& a) { return stream_ws(a.shape).total; }
+
+template <typename T, int STORE, int D> static cudaError_t paged_stream_t(const PopePagedAttnArgs& a, cudaStream_t st) {
+  constexpr bool Q8 = STORE != POPE_STORE_16;
+  constexpr int DC = D / 8, KBLK = (D * (Q8 ? 1 : 2) + 127) / 128;
+  const PopeShape& s = a.shape;
+  const PopePagedKV& kv = a.cache.kv;
+  const StreamWs ws = stream_ws(s);
+  uint8_t* base = static_cast<uint8_t*>(a.workspace);
+  const TrigTables tt = trig_tables_at(base, s.Nk, s.r);
+  PagedStreamP p = {};
+  p.Hk = s.Hk, p.G = s.H / s.Hk, p.Nq = s.Nq, p.Nk = s.Nk, p.r = s.r, p.RP = round_up(s.r, 16);
+  p.nsplit = stream_split(s), p.blocks = stream_blocks(s);
+  p.page_size = kv.page_size, p.max_pages = kv.max_pages_per_seq, p.num_pages = kv.num_pages, p.q_wide = rows_wide(a.q, a.sq);
+  p.scale_log2 = std::abs(a.softmax_scale) * LOG2E, p.q_sign = a.softmax_scale < 0.f ? 0x80008000u : 0u;
+  p.page_table = kv.page_table, p.seq_lens = kv.seq_lens, p.counts = a.counts;
+  p.q = a.q, p.sq = Strides(a.sq), p.ch = static_cast<const __half*>(tt.ch), p.sh = static_cast<const __half*>(tt.sh);
+  p.bias = a.embed.bias, p.bias_sh = a.embed.bias_stride_h;
+  p.e = paged_out(a, p.nsplit, reinterpret_cast<float*>(base + ws.part_o), reinterpret_cast<float*>(base + ws.part_ml));
+  p.status = tc_status_ptr();
+  if (!p.status) return cudaErrorInvalidSymbol;
+  CUtensorMap mk, mv, mt, mks, mvs;
+  const int row_bytes = Q8 ? s.d : 2 * s.d;
+  bool ok = make_page_tmap(&mk, kv.k_pages, row_bytes, kv.page_size, s.Hk, kv.num_pages, SK_KEYS, 1) &&
+            make_page_tmap(&mv, kv.v_pages, row_bytes, kv.page_size, s.Hk, kv.num_pages, SK_KEYS, 1);
+  // (the maps of what a call does not have are not used)
+  ok = ok && (s.r > 0 ? make_trig_tmap(&mt, tt.ch, s.Nk, s.r, SK_KEYS) : (mt = mk, true));
+  ok = ok && (Q8 ? make_page_tmap(&mks, a.cache.k_scales, 0, kv.page_size, s.Hk, kv.num_pages, SK_KEYS, 1) &&
+                       make_page_tmap(&mvs, a.cache.v_scales, 0, kv.page_size, s.Hk, kv.num_pages, SK_KEYS, 1)
+                 : (mks = mvs = mk, true));
+  if (!ok) return cudaErrorNotSupported;
+  const size_t kstage = (size_t)(KBLK + 2 * ((s.r + 63) / 64)) * SK_BLOCK + (Q8 ? 1024 : 0), vstage = (size_t)KBLK * SK_BLOCK + (Q8 ? 1024 : 0);
+  const size_t fixed = 1024 + 2 * (size_t)(DC + p.RP / 8) * SK_CS + (Q8 ? 2 * (size_t)DC * SK_CS : 0) + 4 * PAGED_ROWS * 4 + 2 * (size_t)s.r * 4 + SK_COUNT * 8 + 16;
+  // (V of a step is used about two steps after its K: one stage more)
+  for (p.kstages = SK_MAX_STAGES; p.kstages >= 2; --p.kstages) {
+    p.vstages = std::min(p.kstages + 1, SK_MAX_STAGES);
+    if (fixed + p.kstages * kstage + p.vstages * vstage <= (size_t)kMaxDynamicSmem) break;
+  }
+  if (p.kstages < 2) return cudaErrorInvalidValue;
+  // (every CTA allocates all 512 TMEM columns: two must not share an SM)
+  const size_t smem = std::max<size_t>(fixed + p.kstages * kstage + p.vstages * vstage, 120 * 1024);
+  cudaError_t e = ensure_max_smem<paged_stream_kernel<T, STORE, D>>();
+  if (e != cudaSuccess) return e;
+  const unsigned blocks = (unsigned)(s.B * s.Hk * p.blocks);
+  const dim3 grid(blocks * (unsigned)p.nsplit), block(SK_THREADS);
+  if (s.r > 0 && (e = launch_paged_tables(a.embed, s.Nk, s.r, tt.ch, tt.sh, nullptr, 0, st)) != cudaSuccess) return e;
+  e = launch_dependent(paged_stream_kernel<T, STORE, D>, grid, block, smem, st, p, mk, mv, mt, mks, mvs);
+  return e != cudaSuccess || p.nsplit == 1 ? e : launch_paged_merge(p.e, s.dtype, s.d, (int)blocks, p.blocks, st);
+}
+template <typename T, int STORE> static cudaError_t paged_stream_d(const PopePagedAttnArgs& a, cudaStream_t st) {
+  const int d = a.shape.d;
+  return d == 64 ? paged_stream_t<T, STORE, 64>(a, st) : d == 96 ? paged_stream_t<T, STORE, 96>(a, st) : paged_stream_t<T, STORE, 128>(a, st);
+}
+template <typename T> static cudaError_t paged_stream_s(const PopePagedAttnArgs& a, cudaStream_t st) {
+  switch (a.cache.store) {
+    case POPE_STORE_INT8: return paged_stream_d<T, POPE_STORE_INT8>(a, st);
+    case POPE_STORE_E4M3: return paged_stream_d<T, POPE_STORE_E4M3>(a, st);
+    default: return paged_stream_d<T, POPE_STORE_16>(a, st);
+  }
+}
+cudaError_t paged_stream(const PopePagedAttnArgs& a, cudaStream_t st) {
+  return a.shape.dtype == POPE_BF16 ? paged_stream_s<__nv_bfloat16>(a, st) : paged_stream_s<__half>(a, st);
+}
+
+}  // namespace pope
