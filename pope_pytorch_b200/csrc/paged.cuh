@@ -58,6 +58,38 @@ template <int STORE> __device__ __forceinline__ void codes_to_f32(uint32_t w, fl
   }
 }
 
+// Codes of a word times c, for the argument of a softplus.  int8: the byte u = code + 128 in the mantissa of 2^15 makes 2^15 + u;
+// (2^15 + u) c - (2^15 + 128) c is one fused operation, off by the rounding of the constant (2^-9 of a code step,
+// 2^-16 of the row's largest value).
+template <int STORE> __device__ __forceinline__ void codes_times(uint32_t w, float c, float2 (&x)[2]) {
+  if constexpr (STORE == POPE_STORE_INT8) {
+    w ^= 0x80808080u;
+    const float2 cc = make_float2(c, c), off = make_float2(-32896.f * c, -32896.f * c);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      x[i] = fma2(make_float2(__uint_as_float(__byte_perm(w, 0x47000000u, 0x7404 + (i << 5))), __uint_as_float(__byte_perm(w, 0x47000000u, 0x7414 + (i << 5)))), cc, off);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * i)), __NV_E4M3);
+      x[i] = mul2(__half22float2(*reinterpret_cast<const __half2*>(&h)), make_float2(c, c));
+    }
+  }
+}
+
+// softplus(x) / ln 2 = max(y, 0) + log2(1 + t), t = 2^-|y|, y = x log2(e).  The special-function unit, 16 results a clock and SM, sets the pace of the
+// kernels that transform keys on the fly, so only t comes from it: log2(1 + t) = t P(t) with a least-maximum fit of degree 5 over
+// [0, 1], off by 2^-16.8 of its value.
+__device__ __forceinline__ float2 softplus_log2_fma(float2 y) {
+  const float2 t = make_float2(ex2_approx(-fabsf(y.x)), ex2_approx(-fabsf(y.y)));
+  float2 q = fma2(t, make_float2(-0.034435783f, -0.034435783f), make_float2(0.14603262f, 0.14603262f));
+  q = fma2(t, q, make_float2(-0.3030363f, -0.3030363f));
+  q = fma2(t, q, make_float2(0.46917403f, 0.46917403f));
+  q = fma2(t, q, make_float2(-0.72042614f, -0.72042614f));
+  q = fma2(t, q, make_float2(1.4426829f, 1.4426829f));
+  return fma2(t, q, make_float2(fmaxf(y.x, 0.f), fmaxf(y.y, 0.f)));
+}
+
 // fp16 cos / sin tables of a call, [2][n][r]; also zeroes `nzero` counters.  One launch.
 cudaError_t launch_paged_tables(const PopeEmbed& e, int n, int r, void* ch, void* sh, unsigned int* zero, int nzero, cudaStream_t st);
 

@@ -27,18 +27,19 @@ inline bool rows_wide(const void* ptr, const PopeStride3& t) {   // rows on 16-b
   return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && t.b % 8 == 0 && t.h % 8 == 0 && t.n % 8 == 0;
 }
 
-// The softmax warps (threads 0 .. 255), all products of the CTA completed: row tid & 127, half tid >> 7 of its D columns from `tmem_o` on.
-// `l_half`: the row's sum over this thread's keys, 0 for a row that is no query; m: its maximum.  xch: 256 floats of shared memory that nobody reads
-// any more.
-template <typename T, int D>
-__device__ __forceinline__ void paged_epilogue(const PagedOut& e, uint32_t tmem_o, float* xch, int ub, int split, int b, int hk, int rb, float l_half,
-                                               float m) {
+// The softmax warps (threads 0 .. 255), all products of the CTA completed: row tid & 127, half tid >> 7 of its D columns from `tmem_o` on.  TWO: the halves
+// of a row's keys have accumulators of their own, 128 columns apart, and maxima of their own.  `l_half`: the row's sum over this thread's
+// keys, 0 for a row that is no query; m: its maximum.  xch: 512 floats of shared memory that nobody reads any more.
+template <typename T, int D, bool TWO>
+__device__ __forceinline__ void paged_epilogue(const PagedOut& e, uint32_t tmem_o, float* xch, int ub, int split, int b, int hk, int rb, float l_half, float m_half) {
   const int tid = threadIdx.x, rloc = tid & 127, part = tid >> 7;
   auto all_sync = []() { asm volatile("bar.sync 5, %0;" ::"n"(32 * PAGED_SM_WARPS) : "memory"); };
   all_sync();   // (every thread is past its last look at xch)
-  xch[part * PAGED_ROWS + rloc] = l_half;
+  xch[part * PAGED_ROWS + rloc] = m_half, xch[(2 + part) * PAGED_ROWS + rloc] = l_half;
   all_sync();
-  const float l = xch[rloc] + xch[PAGED_ROWS + rloc];
+  const float m0 = xch[rloc], m1 = xch[PAGED_ROWS + rloc], m = fmaxf(m0, m1), mu = m == -CUDART_INF_F ? 0.f : m;
+  const float f0 = TWO ? ex2_approx(m0 - mu) : 1.f, f1 = TWO ? ex2_approx(m1 - mu) : 1.f;   // 0 for a half without visible keys
+  const float l = xch[2 * PAGED_ROWS + rloc] * f0 + xch[3 * PAGED_ROWS + rloc] * f1;
   fence_after_sync();
   const int rho = rb * PAGED_ROWS + rloc, tok = rho / e.G, head = hk + (rho - tok * e.G) * e.Hk;
   const bool whole = e.nsplit == 1, out_row = rho < e.Nq * e.G;   // (padding is written too)
@@ -49,12 +50,18 @@ __device__ __forceinline__ void paged_epilogue(const PagedOut& e, uint32_t tmem_
   float* prow = e.part_o + (slot * PAGED_ROWS + rloc) * D + part * (D / 2);
 #pragma unroll
   for (int c0 = 0; c0 < D / 2; c0 += 16) {
-    uint32_t ov[16];
+    uint32_t ov[16], ov1[16];
     tmem_ld16(o_addr + c0, ov);
+    if constexpr (TWO) tmem_ld16(o_addr + 128 + c0, ov1);
     tmem_ld_wait();
     float x[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = l != 0.f ? __uint_as_float(ov[i]) * inv : 0.f;   // (without a visible key O may hold anything)
+    for (int i = 0; i < 16; ++i) {
+      x[i] = l != 0.f ? __uint_as_float(ov[i]) * inv : 0.f;   // (without a visible key O may hold anything)
+      // (NaN factors stay NaN)
+      if constexpr (TWO)
+        x[i] = l != 0.f ? ((f0 != 0.f ? __uint_as_float(ov[i]) * f0 : 0.f) + (f1 != 0.f ? __uint_as_float(ov1[i]) * f1 : 0.f)) * inv : 0.f;
+    }
     if (out_row && whole) {
 #pragma unroll
       for (int i = 0; i < 16; i += 8)

@@ -2,7 +2,7 @@
 // tokens, the last short piece of a prompt.
 //
 // The query rows that share a key head -- the newest tokens of a sequence times the heads of the group -- are packed into blocks of
-// 8, 16 or 32 (row = token * group + head).  A call then is one pass over K and V, each key transformed once for all rows of the block:
+// 8 or 16 (row = token * group + head).  A call then is one pass over K and V, each key transformed once for all rows of the block:
 //
 //   copies  : tiles of 32 keys (K rows and V rows of one or two key heads, fp16 cos / sin rows, row scales) by tensor-map copies in
 //             128-byte-swizzled rows; the page of a tile comes from the page table.  There is no loading warp: of the warps that share a
@@ -105,23 +105,6 @@ template <int STORE> __device__ __forceinline__ void codes_to_half(uint32_t w, u
     }
   }
 }
-// Codes of a word times c.  int8: the byte u = code + 128 in the mantissa of 2^15 makes 2^15 + u; (2^15 + u) c - (2^15 + 128) c is one fused
-// operation, off by the rounding of the constant (2^-9 of a code step).
-template <int STORE> __device__ __forceinline__ void codes_times(uint32_t w, float c, float2 (&x)[2]) {
-  if constexpr (STORE == POPE_STORE_INT8) {
-    w ^= 0x80808080u;
-    const float2 cc = make_float2(c, c), off = make_float2(-32896.f * c, -32896.f * c);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      x[i] = fma2(make_float2(__uint_as_float(__byte_perm(w, 0x47000000u, 0x7404 + (i << 5))), __uint_as_float(__byte_perm(w, 0x47000000u, 0x7414 + (i << 5)))), cc, off);
-  } else {
-    uint32_t h[2];
-    codes_to_half<STORE>(w, h);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) x[i] = mul2(unpack2<__half>(h[i]), make_float2(c, c));
-  }
-}
-
 // Four codes of each of two keys, first features first -> fp16 pairs (key 0, key 1) of the four features
 template <int STORE> __device__ __forceinline__ void code_pairs(uint32_t a, uint32_t b, uint32_t (&h)[4]) {
   if constexpr (STORE == POPE_STORE_INT8) a ^= 0x80808080u, b ^= 0x80808080u;
@@ -148,7 +131,7 @@ template <int STORE> __device__ __forceinline__ void code_pairs(uint32_t a, uint
 
 constexpr float PR_BIG = 32768.f;   // magnitudes of fp16 operands stay below twice this
 
-// RQ: groups of eight query rows in a block (1, 2, 4); NW: warps
+// RQ: groups of eight query rows in a block (1, 2); NW: warps
 template <typename T, int STORE, int D, int RQ, int NW>
 __global__ void __launch_bounds__(32 * NW, 1)
     paged_rows_kernel(PagedRowsP p, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
@@ -707,14 +690,14 @@ __global__ void __launch_bounds__(32 * NW, 1)
 // ---- host side ---------------------------------------------------------------------------------------
 static int rows_rq(const PopeShape& s) {   // groups of eight rows in a block
   const int64_t rows = (int64_t)s.Nq * (s.H / s.Hk);
-  return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  return rows <= 8 ? 1 : 2;
 }
 static int rows_blocks(const PopeShape& s) {
   const int64_t rows = (int64_t)s.Nq * (s.H / s.Hk);
   return (int)((rows + 8 * rows_rq(s) - 1) / (8 * rows_rq(s)));
 }
 // warps of a CTA: as many as the registers of their outputs (32 per group of eight rows) allow
-constexpr int rows_nw(int rq) { return rq == 4 ? 8 : rq == 2 ? 12 : 16; }
+constexpr int rows_nw(int rq) { return rq == 2 ? 12 : 16; }
 // Key heads of a CTA: they share the copies of the cosines and sines, which at 8 bits are as many bytes as K and V or twice that.
 static int rows_hb(const PopeShape& s, int store) {
   const int pairs = rows_nw(rows_rq(s)) / PR_WPT;
@@ -809,8 +792,7 @@ template <typename T, int STORE, int D, int RQ> static cudaError_t paged_rows_t(
   return cudaGetLastError();
 }
 template <typename T, int STORE, int D> static cudaError_t paged_rows_q(const PopePagedAttnArgs& a, cudaStream_t st) {
-  const int rq = rows_rq(a.shape);
-  return rq == 1 ? paged_rows_t<T, STORE, D, 1>(a, st) : rq == 2 ? paged_rows_t<T, STORE, D, 2>(a, st) : paged_rows_t<T, STORE, D, 4>(a, st);
+  return rows_rq(a.shape) == 1 ? paged_rows_t<T, STORE, D, 1>(a, st) : paged_rows_t<T, STORE, D, 2>(a, st);
 }
 template <typename T, int STORE> static cudaError_t paged_rows_d(const PopePagedAttnArgs& a, cudaStream_t st) {
   const int d = a.shape.d;

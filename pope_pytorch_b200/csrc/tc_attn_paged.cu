@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP 
     }
 
     if (T_tiles > 0 && !failed) failed = !mbar_wait(&bars[PS_ODONE], 0, WAIT_LIMIT);
-    paged_epilogue<T, D>(p.e, tmem + PS_TO, xch, ub, split, b, hk, rb, live ? l_run : 0.f, m_run);
+    paged_epilogue<T, D, false>(p.e, tmem + PS_TO, xch, ub, split, b, hk, rb, live ? l_run : 0.f, m_run);
   }
   if (failed) atomicOr(p.status, 1u);
   fence_before_sync();
@@ -649,7 +649,7 @@ enum class Paged { kRows, kStream, kSweep };
 static Paged paged_kernel(const PopeShape& s) {
   const int64_t rows = (int64_t)s.Nq * (s.H / s.Hk);
   const char* e = getenv("PAGED_PATH");
-  if (e) return e[0] == '0' ? Paged::kRows : e[0] == '1' ? Paged::kStream : Paged::kSweep;
+  if (e) return e[0] == '0' ? (rows > 16 ? Paged::kStream : Paged::kRows) : e[0] == '1' ? Paged::kStream : Paged::kSweep;
   return rows <= 16 ? Paged::kRows : rows <= 256 ? Paged::kStream : Paged::kSweep;
 }
 

@@ -9,7 +9,7 @@
 //                     of a cache that holds 8 bits also V as 16-bit values
 //   score warp      : S = Q' K'^T, Q' in tensor memory, into one of two buffers
 //   8 softmax warps : two threads per row, online softmax, P over S
-//   PV warp         : O += P V, V from its stage (16 bits) or the expanders' tile (8 bits)
+//   PV warp         : O += P V into an accumulator for each of a row's two threads, which so need not agree on a maximum; V from its stage (16 bits) or the expanders' tile (8 bits)
 // The step is bound by instruction issue of the expanders and the softmax (about 60 warp instructions a key at r = 64) next to the 512 bytes
 // of K and V a key at 16 bits.  Small grids are cut along the keys as in tc_attn_paged.cu.
 #include <algorithm>
@@ -41,7 +41,7 @@ constexpr int SK_EX = PAGED_SM_WARPS, SK_EX_WARPS = 8, SK_EX_THREADS = 32 * SK_E
 constexpr int SK_KLOAD = SK_EX + SK_EX_WARPS, SK_VLOAD = SK_KLOAD + 1, SK_S = SK_KLOAD + 2, SK_PV = SK_KLOAD + 3;
 constexpr int SK_THREADS = 32 * (SK_PV + 1);
 constexpr int SK_CS = SK_KEYS * 16 + 16;           // chunk stride of an operand tile: the padding keeps the expanders' stores on distinct banks
-constexpr uint32_t SK_TS = 128, SK_TO = 256;       // first TMEM column of the S / P buffers and of O (Q' starts at 0)
+constexpr uint32_t SK_TS = 128, SK_TO = 256;       // first TMEM column of the S / P buffers and of the two O (Q' starts at 0)
 constexpr int SK_BLOCK = SK_KEYS * 128;            // bytes of 128-byte rows of a step
 constexpr int SK_MAX_STAGES = 4;
 enum {
@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
   uint8_t* vring = smem + p.kstages * kstage;
   uint8_t* Ks = vring + p.vstages * vstage;                        // [2][KC][SK_CS]
   uint8_t* Vs = Ks + 2 * KC * SK_CS;                               // 8 bits: [2][DC][SK_CS]
-  float* xch = reinterpret_cast<float*>(Vs + (Q8 ? 2 * DC * SK_CS : 0));   // [2 step parities][2 parts][128 rows] row maxima
+  float* xch = reinterpret_cast<float*>(Vs + (Q8 ? 2 * DC * SK_CS : 0));   // [2 parts][128 rows] maxima, then sums (epilogue)
   float* bias_cs = xch + 4 * PAGED_ROWS;                           // [2][r]
   uint64_t* bars = reinterpret_cast<uint64_t*>(bias_cs + 2 * r);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + SK_COUNT);
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
         constexpr uint32_t kstep = (Q8 ? 256 : 2048) >> 4;
 #pragma unroll
         for (int ks = 0; ks < SK_KEYS / 16; ++ks)   // P of keys [32 t, 32 t + 32) sits in the first 16 columns of part t
-          mma_ts_lh(tmem + SK_TO, a + (ks * 16 / 32) * 32 + (ks * 16 % 32) / 2, desc_lo(bd) + ks * kstep, desc_hi(bd), idesc, (j > 0 || ks > 0) ? 1u : 0u);
+          mma_ts_lh(tmem + SK_TO + (ks / 2) * 128, a + (ks / 2) * 32 + (ks % 2) * 8, desc_lo(bd) + ks * kstep, desc_hi(bd), idesc, (j > 0 || ks % 2 > 0) ? 1u : 0u);
         if (j == T_tiles - 1) mma_commit(&bars[SK_ODONE]);
         mma_commit(&bars[SK_PVDONE + buf]);
         if constexpr (!Q8) mma_commit(&bars[SK_VEMPTY + s]);
@@ -225,11 +225,9 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
       auto raw_of = [&](const uint8_t* base, int row, int c) { return *reinterpret_cast<const Raw*>(swizzled(base, row, c * (Q8 ? 8 : 16))); };
       auto values = [&](const Raw& w, float scale, float2 (&x)[4]) {
         if constexpr (Q8) {
-          float lo[4], hi[4];
-          codes_to_f32<STORE>(w.x, lo), codes_to_f32<STORE>(w.y, hi);
-          const float2 f = make_float2(scale, scale);
-          x[0] = mul2(make_float2(lo[0], lo[1]), f), x[1] = mul2(make_float2(lo[2], lo[3]), f);
-          x[2] = mul2(make_float2(hi[0], hi[1]), f), x[3] = mul2(make_float2(hi[2], hi[3]), f);
+          float2 y[2];
+          codes_times<STORE>(w.x, scale, y), x[0] = y[0], x[1] = y[1];
+          codes_times<STORE>(w.y, scale, y), x[2] = y[0], x[3] = y[1];
         } else {
           x[0] = unpack2<T>(w.x), x[1] = unpack2<T>(w.y), x[2] = unpack2<T>(w.z), x[3] = unpack2<T>(w.w);
         }
@@ -248,7 +246,7 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
           raw[k] = raw_of(st, rw[k], cl[k]);
           const uint8_t* trow = st + trig_at + (cl[k] >> 3) * 2 * SK_BLOCK + rw[k] * 128 + (((cl[k] & 7) ^ (rw[k] & 7)) << 4);
           cq[k] = *reinterpret_cast<const uint4*>(trow), sq[k] = *reinterpret_cast<const uint4*>(trow + SK_BLOCK);
-          f[k] = Q8 ? scl[rw[k]] : 1.f;
+          f[k] = Q8 ? scl[rw[k]] * LOG2E : 1.f;
           row += rrow_step, c += rcol_step;
           if (c >= rdiv) c -= rdiv, ++row;
         }
@@ -258,9 +256,8 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
           values(raw[k], f[k], a[k]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float2 y = mul2(a[k][e], make_float2(LOG2E, LOG2E));
-            const float2 v = add2(make_float2(ex2_approx(-fabsf(y.x)), ex2_approx(-fabsf(y.y))), make_float2(1.f, 1.f));
-            a[k][e] = add2(make_float2(lg2_approx(v.x), lg2_approx(v.y)), make_float2(fmaxf(y.x, 0.f), fmaxf(y.y, 0.f)));
+            if constexpr (!Q8) a[k][e] = mul2(a[k][e], make_float2(LOG2E, LOG2E));
+            a[k][e] = softplus_log2_fma(a[k][e]);
             if constexpr (!BF) a[k][e] = mul2(a[k][e], make_float2(LN2, LN2));
           }
         }
@@ -287,18 +284,31 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
         }
       }
       auto as_16 = [&](const Raw& w, float scale) {
-        if constexpr (Q8) {
-          float2 x[4];
-          values(w, scale, x);
+        if constexpr (Q8) {   // (value by value: a value that leaves as it is has all of its bits)
+          float lo[4], hi[4];
+          codes_to_f32<STORE>(w.x, lo), codes_to_f32<STORE>(w.y, hi);
+          const float2 f = make_float2(scale, scale);
+          const float2 x[4] = {mul2(make_float2(lo[0], lo[1]), f), mul2(make_float2(lo[2], lo[3]), f), mul2(make_float2(hi[0], hi[1]), f), mul2(make_float2(hi[2], hi[3]), f)};
           return make_uint4(pack2<T>(x[0].x, x[0].y), pack2<T>(x[1].x, x[1].y), pack2<T>(x[2].x, x[2].y), pack2<T>(x[3].x, x[3].y));
         } else {
           return w;
         }
       };
       for (int row = prow, c = pcol; row < SK_KEYS && PC > 0;) {
-        *reinterpret_cast<uint4*>(kt + (RC + c) * SK_CS + row * 16) = as_16(raw_of(st, row, RC + c), Q8 ? scl[row] : 1.f);
-        row += prow_step, c += pcol_step;
-        if (c >= pdiv) c -= pdiv, ++row;
+        int rw[2], cl[2];
+        bool on[2];
+        Raw raw[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          rw[k] = row, cl[k] = RC + c, on[k] = row < SK_KEYS;
+          if (!on[k]) rw[k] = SK_KEYS - 1;
+          raw[k] = raw_of(st, rw[k], cl[k]);
+          row += prow_step, c += pcol_step;
+          if (c >= pdiv) c -= pdiv, ++row;
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (on[k]) *reinterpret_cast<uint4*>(kt + cl[k] * SK_CS + rw[k] * 16) = as_16(raw[k], Q8 ? scl[rw[k]] : 1.f);
       }
       fence_async_smem();   // the tile is visible to the tensor core; the stage has been read
       __syncwarp();
@@ -311,9 +321,14 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
         const uint8_t* vst = vring + vs * vstage;
         uint8_t* vt = Vs + buf * DC * SK_CS;
         const float* vscl = reinterpret_cast<const float*>(vst + vscale_at);
-        for (int i = et; i < SK_KEYS * DC; i += SK_EX_THREADS) {
-          const int row = i / DC, c = i % DC;
-          *reinterpret_cast<uint4*>(vt + c * SK_CS + row * 16) = row < live ? as_16(raw_of(vst, row, c), vscl[row]) : make_uint4(0, 0, 0, 0);
+        constexpr int NV = SK_KEYS * DC / SK_EX_THREADS;
+        Raw raw[NV];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) raw[k] = raw_of(vst, (et + k * SK_EX_THREADS) / DC, (et + k * SK_EX_THREADS) % DC);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          const int row = (et + k * SK_EX_THREADS) / DC, c = (et + k * SK_EX_THREADS) % DC;
+          *reinterpret_cast<uint4*>(vt + c * SK_CS + row * 16) = row < live ? as_16(raw[k], vscl[row]) : make_uint4(0, 0, 0, 0);
         }
         fence_async_smem();
         __syncwarp();
@@ -329,8 +344,6 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
     const int rho = rb * PAGED_ROWS + rloc, tok = rho / p.G, head = hk + (rho - tok * p.G) * p.Hk, pos = len - cnt + tok;
     const bool live = rloc < rows && pos >= 0, warp_live = (warp & 3) * 32 < rows;   // (warps without a query only keep the steps' pace)
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const int row_bar = 1 + (warp & 3);   // named barrier of the two warps that share 32 rows
-    auto row_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(row_bar) : "memory"); };
     {
       // Q' = [a cos(f - b) | plain | a sin(f - b)], straight into tensor memory; rows that are no queries are zero
       const T* qrow = static_cast<const T*>(p.q) + b * p.sq.b + head * p.sq.h + (int64_t)tok * p.sq.n;
@@ -397,10 +410,7 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
           for (int i = 0; i < 32; ++i)
             if ((vis >> i) & 1u) m4[i & 3] = fmaxf(m4[i & 3], __uint_as_float(sv[i]));
         }
-        float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-        xch[(buf * 2 + part) * PAGED_ROWS + rloc] = mx;
-        row_sync();
-        mx = fmaxf(mx, xch[(buf * 2 + 1 - part) * PAGED_ROWS + rloc]);
+        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         const float m_new = fmaxf(m_run, mx == -CUDART_INF_F ? mx : mx * p.scale_log2);
         const bool need = m_new > m_run + 8.f;   // a stale maximum is kept while it is within 2^8 of the true one
         float alpha = 1.f;
@@ -412,9 +422,9 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
         if (j > 0 && __any_sync(0xffffffffu, need)) {
           if (!failed) failed = !mbar_wait(&bars[SK_PVDONE + (1 - buf)], ((j - 1) >> 1) & 1, WAIT_LIMIT);
           fence_after_sync();
-          const uint32_t o_addr = tmem + lane_base + SK_TO + part * (D / 2);
-#pragma unroll
-          for (int c0 = 0; c0 < D / 2; c0 += 16) {
+          const uint32_t o_addr = tmem + lane_base + SK_TO + part * 128;
+#pragma unroll 1
+          for (int c0 = 0; c0 < D; c0 += 16) {
             uint32_t ov[16];
             tmem_ld16(o_addr + c0, ov);
             tmem_ld_wait();
@@ -458,7 +468,7 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
       if (lane == 0) mbar_arrive(&bars[SK_PFULL + buf]);
     }
     if (T_tiles > 0 && !failed) failed = !mbar_wait(&bars[SK_ODONE], 0, WAIT_LIMIT);
-    paged_epilogue<T, D>(p.e, tmem + SK_TO, xch, ub, split, b, hk, rb, live ? l_run : 0.f, m_run);
+    paged_epilogue<T, D, true>(p.e, tmem + SK_TO, xch, ub, split, b, hk, rb, live ? l_run : 0.f, m_run);
   }
   if (failed) atomicOr(p.status, 1u);
   fence_before_sync();
