@@ -170,6 +170,7 @@ __global__ void __launch_bounds__(32 * NW, 1)
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int split = blockIdx.x % p.nsplit, u = blockIdx.x / p.nsplit;
   const int rb = u % p.blocks, bk = u / p.blocks, hk0 = bk % (p.Hk / hb) * hb, b = bk / (p.Hk / hb);
+  if (tid == 32) prefetch_tmap(&tmap_k), prefetch_tmap(&tmap_v), prefetch_tmap(&tmap_t), prefetch_tmap(&tmap_ks), prefetch_tmap(&tmap_vs);
   if (tid == 0) {
     for (int s = 0; s < rings * p.stages; ++s) mbar_init(&full[s], 1), used[s] = 0;
     mbar_init_fence();

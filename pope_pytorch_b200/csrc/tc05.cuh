@@ -108,6 +108,9 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* tmap, ui
       : "memory");
 }
 
+// Fetch a tensor map (a kernel parameter) ahead of its first copy.
+__device__ __forceinline__ void prefetch_tmap(const void* tmap) { asm volatile("prefetch.tensormap [%0];" ::"l"(tmap) : "memory"); }
+
 // Tiled store of a box from this CTA's shared memory (laid out as the tensor map's swizzle mode says) to global
 // memory; parts of the box outside the tensor are not written.  Completion through the bulk async-group of the
 // issuing thread (tma_store_commit / tma_store_wait_read).  Coordinates must not be negative.

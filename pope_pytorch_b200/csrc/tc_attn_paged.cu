@@ -272,6 +272,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP 
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + PS_COUNT);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) prefetch_tmap(&tmap_v);
   if (warp == PS_S) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -496,28 +497,30 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP 
         tmem_st_wait();
       }
       const float m_use = m_run == -CUDART_INF_F ? 0.f : m_run;
-      float ls4[4] = {0.f, 0.f, 0.f, 0.f};
+      float2 ls2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       uint32_t pk[2][16];
+      const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), mu2 = make_float2(-m_use, -m_use);
       auto exponentials = [&](auto masked) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           const uint32_t vq = (uint32_t)(vis >> (32 * q));
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float p0 = ex2_approx(fmaf(__uint_as_float(sv[q][2 * i]), p.scale_log2, -m_use));
-            float p1 = ex2_approx(fmaf(__uint_as_float(sv[q][2 * i + 1]), p.scale_log2, -m_use));
+            float2 x = fma2(make_float2(__uint_as_float(sv[q][2 * i]), __uint_as_float(sv[q][2 * i + 1])), sc2, mu2);
+            x.x = ex2_approx(x.x), x.y = ex2_approx(x.y);
             if (decltype(masked)::value) {
-              p0 = ((vq >> (2 * i)) & 1u) ? p0 : 0.f;
-              p1 = ((vq >> (2 * i + 1)) & 1u) ? p1 : 0.f;
+              x.x = ((vq >> (2 * i)) & 1u) ? x.x : 0.f;
+              x.y = ((vq >> (2 * i + 1)) & 1u) ? x.y : 0.f;
             }
-            ls4[i & 3] += p0 + p1;
-            pk[q][i] = pack2<T>(p0, p1);
+            ls2[i & 1] = add2(ls2[i & 1], x);
+            pk[q][i] = pack2<T>(x.x, x.y);
           }
         }
       };
       if (all_vis) exponentials(std::false_type());
       else exponentials(std::true_type());
-      l_run += (ls4[0] + ls4[1]) + (ls4[2] + ls4[3]);
+      ls2[0] = add2(ls2[0], ls2[1]);
+      l_run += ls2[0].x + ls2[0].y;
 #pragma unroll
       for (int q = 0; q < 2; ++q) tmem_st16(s_addr + q * 16, pk[q]);
       tmem_st_wait();

@@ -80,6 +80,8 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + SK_COUNT);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (warp == SK_KLOAD && lane == 0) prefetch_tmap(&tmap_k), prefetch_tmap(&tmap_t), prefetch_tmap(&tmap_ks);
+  if (warp == SK_VLOAD && lane == 0) prefetch_tmap(&tmap_v), prefetch_tmap(&tmap_vs);
   if (warp == SK_S) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -435,24 +437,26 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
           tmem_st_wait();
         }
         const float m_use = m_run == -CUDART_INF_F ? 0.f : m_run;
-        float ls2[2] = {0.f, 0.f};
+        float2 ls2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         uint32_t pk[16];
+        const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), mu2 = make_float2(-m_use, -m_use);
         auto exponentials = [&](auto masked) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            float p0 = ex2_approx(fmaf(__uint_as_float(sv[2 * i]), p.scale_log2, -m_use));
-            float p1 = ex2_approx(fmaf(__uint_as_float(sv[2 * i + 1]), p.scale_log2, -m_use));
+            float2 x = fma2(make_float2(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1])), sc2, mu2);
+            x.x = ex2_approx(x.x), x.y = ex2_approx(x.y);
             if (decltype(masked)::value) {
-              p0 = ((vis >> (2 * i)) & 1u) ? p0 : 0.f;
-              p1 = ((vis >> (2 * i + 1)) & 1u) ? p1 : 0.f;
+              x.x = ((vis >> (2 * i)) & 1u) ? x.x : 0.f;
+              x.y = ((vis >> (2 * i + 1)) & 1u) ? x.y : 0.f;
             }
-            ls2[i & 1] += p0 + p1;
-            pk[i] = pack2<T>(p0, p1);
+            ls2[i & 1] = add2(ls2[i & 1], x);
+            pk[i] = pack2<T>(x.x, x.y);
           }
         };
         if (all_vis) exponentials(std::false_type());
         else exponentials(std::true_type());
-        l_run += ls2[0] + ls2[1];
+        ls2[0] = add2(ls2[0], ls2[1]);
+        l_run += ls2[0].x + ls2[0].y;
         tmem_st16(s_addr, pk);
         tmem_st_wait();
       }
