@@ -231,6 +231,19 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// One lane of a converged warp.  Products are issued by a whole warp that runs their loop together and branches on this around each group of them:
+// the operands then are uniform registers.  Issued by a thread that has branched off alone, every operand of every product goes
+// through a register move of its own: 125 clocks per product for any N up to 128, against 42 (N = 64) and 73 (N = 128).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok));
+  return ok != 0;
+}
+// a whole warp waits: true when every lane saw the phase
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, uint32_t limit) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, limit)) != 0;
+}
+
 // ---- TMEM <-> registers: each thread moves 32-bit columns of ITS lane (row) -------------------
 // A warp may only touch lanes 32*(warp_id % 4) .. +31; the address carries lane << 16 | column.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {

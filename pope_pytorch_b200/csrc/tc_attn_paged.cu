@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP 
   uint64_t* bars = reinterpret_cast<uint64_t*>(xch + 4 * PS_ROWS);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + PS_COUNT);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   if (tid == 0) prefetch_tmap(&tmap_v);
   if (warp == PS_S) {
     tmem_alloc(tmem_slot, 512);
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP 
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   pdl_wait();
   pdl_trigger();
   // unit (sequence, key head), row block (late ones, which see more keys, first), key range
@@ -345,42 +345,40 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP 
       if (failed) break;
     }
   } else if (warp == PS_S) {
-    if (lane == 0) {
-      const uint32_t idesc = instr_desc(TcFmt<T>::fmt, PS_ROWS, PS_KEYS, false, false);
-      const uint32_t ks_addr = smem_u32(Ks);
-      if (!mbar_wait(&bars[PS_QFULL], 0, WAIT_LIMIT)) failed = true;
-      for (int j = 0; j < T_tiles && !failed; ++j) {
-        const int buf = j & 1;
-        failed = !mbar_wait(&bars[PS_KFULL + buf], (j >> 1) & 1, WAIT_LIMIT);
-        if (j >= 2 && !failed) failed = !mbar_wait(&bars[PS_PVDONE + buf], ((j - 2) >> 1) & 1, WAIT_LIMIT);
-        if (failed) break;
-        fence_after_sync();
-        const uint32_t d = tmem + PS_TS + buf * PS_KEYS;
-        const uint64_t bd = smem_desc(ks_addr + buf * KBUF, CSV, 128);
-        uint32_t blo = desc_lo(bd), at = tmem;
-#pragma unroll 4
-        for (int ks = 0; ks < KSTEPS; ++ks) {
-          mma_ts_lh(d, at, blo, desc_hi(bd), idesc, ks > 0 ? 1u : 0u);
-          at += 8, blo += (2 * CSV) >> 4;
+    const bool leader = elect_one();
+    const uint32_t idesc = instr_desc(TcFmt<T>::fmt, PS_ROWS, PS_KEYS, false, false);
+    const uint64_t bd0 = smem_desc(smem_u32(Ks), CSV, 128);
+    failed = !mbar_wait_warp(&bars[PS_QFULL], 0, WAIT_LIMIT);
+    for (int j = 0; j < T_tiles && !failed; ++j) {
+      const int buf = j & 1;
+      failed = !mbar_wait_warp(&bars[PS_KFULL + buf], (j >> 1) & 1, WAIT_LIMIT);
+      if (j >= 2 && !failed) failed = !mbar_wait_warp(&bars[PS_PVDONE + buf], ((j - 2) >> 1) & 1, WAIT_LIMIT);
+      if (failed) break;
+      fence_after_sync();
+      const uint32_t d = tmem + PS_TS + buf * PS_KEYS, blo = desc_lo(bd0) + buf * (KBUF >> 4);
+      int ks = 0;
+      for (; ks + 4 <= KSTEPS; ks += 4)
+        if (leader) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mma_ts_lh(d, tmem + (ks + i) * 8, blo + (ks + i) * ((2 * CSV) >> 4), desc_hi(bd0), idesc, ks + i > 0 ? 1u : 0u);
         }
-        mma_commit(&bars[PS_SFULL + buf]);
-        mma_commit(&bars[PS_KFREE + buf]);
-      }
+      for (; ks < KSTEPS; ++ks)
+        if (leader) mma_ts_lh(d, tmem + ks * 8, blo + ks * ((2 * CSV) >> 4), desc_hi(bd0), idesc, ks > 0 ? 1u : 0u);
+      if (leader) mma_commit(&bars[PS_SFULL + buf]), mma_commit(&bars[PS_KFREE + buf]);
     }
-    __syncwarp();
   } else if (warp == PS_PV) {
-    if (lane == 0) {
-      const uint32_t idesc = instr_desc(TcFmt<T>::fmt, PS_ROWS, D, false, true);
-      const uint32_t vs_addr = smem_u32(Vs);
-      for (int j = 0; j < T_tiles && !failed; ++j) {
-        const int buf = j & 1;
-        failed = !mbar_wait(&bars[PS_VFULL + buf], (j >> 1) & 1, WAIT_LIMIT);
-        if (!failed) failed = !mbar_wait(&bars[PS_PFULL + buf], (j >> 1) & 1, WAIT_LIMIT);
-        if (failed) break;
-        fence_after_sync();
-        const uint32_t a = tmem + PS_TS + buf * PS_KEYS;
-        // B = V, MN-major: 64-feature blocks 16 KB apart, 8-key groups 1 KB apart, 2 KB per 16 keys
-        const uint64_t bd = smem_desc_sw128(vs_addr + buf * VBUF, PS_KEYS * 128, 1024);
+    const bool leader = elect_one();
+    const uint32_t idesc = instr_desc(TcFmt<T>::fmt, PS_ROWS, D, false, true);
+    for (int j = 0; j < T_tiles && !failed; ++j) {
+      const int buf = j & 1;
+      failed = !mbar_wait_warp(&bars[PS_VFULL + buf], (j >> 1) & 1, WAIT_LIMIT);
+      if (!failed) failed = !mbar_wait_warp(&bars[PS_PFULL + buf], (j >> 1) & 1, WAIT_LIMIT);
+      if (failed) break;
+      fence_after_sync();
+      const uint32_t a = tmem + PS_TS + buf * PS_KEYS;
+      // B = V, MN-major: 64-feature blocks 16 KB apart, 8-key groups 1 KB apart, 2 KB per 16 keys
+      const uint64_t bd = smem_desc_sw128(smem_u32(Vs) + buf * VBUF, PS_KEYS * 128, 1024);
+      if (leader) {
 #pragma unroll
         for (int ks = 0; ks < PS_KEYS / 16; ++ks)   // P of keys [64 t, 64 t + 64) sits in the first 32 columns of part t
           mma_ts_lh(tmem + PS_TO, a + (ks * 16 / 64) * 64 + (ks * 16 % 64) / 2, desc_lo(bd) + ks * (2048 >> 4), desc_hi(bd), idesc, (j > 0 || ks > 0) ? 1u : 0u);
@@ -389,7 +387,6 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP 
         mma_commit(&bars[PS_VFREE + buf]);
       }
     }
-    __syncwarp();
   } else {
     // =============================== softmax: two threads per query row ==========================
     const int rloc = tid & 127, part = tid >> 7;

@@ -40,7 +40,7 @@ constexpr int SK_KEYS = 64;
 constexpr int SK_EX = PAGED_SM_WARPS, SK_EX_WARPS = 8, SK_EX_THREADS = 32 * SK_EX_WARPS;   // first expander warp
 constexpr int SK_KLOAD = SK_EX + SK_EX_WARPS, SK_VLOAD = SK_KLOAD + 1, SK_S = SK_KLOAD + 2, SK_PV = SK_KLOAD + 3;
 constexpr int SK_THREADS = 32 * (SK_PV + 1);
-constexpr int SK_CS = SK_KEYS * 16 + 16;           // chunk stride of an operand tile: the padding keeps the expanders' stores on distinct banks
+constexpr int SK_CS = SK_KEYS * 16;                // chunk stride of an operand tile
 constexpr uint32_t SK_TS = 128, SK_TO = 256;       // first TMEM column of the S / P buffers and of the two O (Q' starts at 0)
 constexpr int SK_BLOCK = SK_KEYS * 128;            // bytes of 128-byte rows of a step
 constexpr int SK_MAX_STAGES = 4;
@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(bias_cs + 2 * r);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + SK_COUNT);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   if (warp == SK_KLOAD && lane == 0) prefetch_tmap(&tmap_k), prefetch_tmap(&tmap_t), prefetch_tmap(&tmap_ks);
   if (warp == SK_VLOAD && lane == 0) prefetch_tmap(&tmap_v), prefetch_tmap(&tmap_vs);
   if (warp == SK_S) {
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   bool failed = false;
 
   if (warp == SK_KLOAD || warp == SK_VLOAD) {
@@ -157,61 +157,60 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
       if (++s == stages) s = 0, par ^= 1;
     }
   } else if (warp == SK_S) {
-    if (lane == 0) {
-      const uint32_t idesc = instr_desc(TcFmt<T>::fmt, PAGED_ROWS, SK_KEYS, false, false);
-      const uint32_t ks_addr = smem_u32(Ks);
-      failed = !mbar_wait(&bars[SK_QFULL], 0, WAIT_LIMIT);
-      for (int j = 0; j < T_tiles && !failed; ++j) {
-        const int buf = j & 1;
-        failed = !mbar_wait(&bars[SK_KREADY + buf], (j >> 1) & 1, WAIT_LIMIT);
-        if (j >= 2 && !failed) failed = !mbar_wait(&bars[SK_PVDONE + buf], ((j - 2) >> 1) & 1, WAIT_LIMIT);
-        if (failed) break;
-        fence_after_sync();
-        const uint64_t bd = smem_desc(ks_addr + buf * KC * SK_CS, SK_CS, 128);
-        uint32_t blo = desc_lo(bd), at = tmem;
-#pragma unroll 4
-        for (int ks = 0; ks < KSTEPS; ++ks) {
-          mma_ts_lh(tmem + SK_TS + buf * SK_KEYS, at, blo, desc_hi(bd), idesc, ks > 0 ? 1u : 0u);
-          at += 8, blo += (2 * SK_CS) >> 4;
+    const bool leader = elect_one();
+    const uint32_t idesc = instr_desc(TcFmt<T>::fmt, PAGED_ROWS, SK_KEYS, false, false);
+    const uint64_t bd0 = smem_desc(smem_u32(Ks), SK_CS, 128);
+    failed = !mbar_wait_warp(&bars[SK_QFULL], 0, WAIT_LIMIT);
+    for (int j = 0; j < T_tiles && !failed; ++j) {
+      const int buf = j & 1;
+      failed = !mbar_wait_warp(&bars[SK_KREADY + buf], (j >> 1) & 1, WAIT_LIMIT);
+      if (j >= 2 && !failed) failed = !mbar_wait_warp(&bars[SK_PVDONE + buf], ((j - 2) >> 1) & 1, WAIT_LIMIT);
+      if (failed) break;
+      fence_after_sync();
+      const uint32_t d = tmem + SK_TS + buf * SK_KEYS, blo = desc_lo(bd0) + buf * ((KC * SK_CS) >> 4);
+      int ks = 0;
+      for (; ks + 4 <= KSTEPS; ks += 4)
+        if (leader) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mma_ts_lh(d, tmem + (ks + i) * 8, blo + (ks + i) * ((2 * SK_CS) >> 4), desc_hi(bd0), idesc, ks + i > 0 ? 1u : 0u);
         }
-        mma_commit(&bars[SK_SFULL + buf]);
-        mma_commit(&bars[SK_KFREE + buf]);
-      }
+      for (; ks < KSTEPS; ++ks)
+        if (leader) mma_ts_lh(d, tmem + ks * 8, blo + ks * ((2 * SK_CS) >> 4), desc_hi(bd0), idesc, ks > 0 ? 1u : 0u);
+      if (leader) mma_commit(&bars[SK_SFULL + buf]), mma_commit(&bars[SK_KFREE + buf]);
     }
-    __syncwarp();
   } else if (warp == SK_PV) {
-    if (lane == 0) {
-      const uint32_t idesc = instr_desc(TcFmt<T>::fmt, PAGED_ROWS, D, false, true);
-      for (int j = 0, s = 0, par = 0; j < T_tiles && !failed; ++j) {
-        const int buf = j & 1;
-        // (at 8 bits V is the expanders', and its stage may already be in its next use)
-        if constexpr (!Q8) failed = !mbar_wait(&bars[SK_VFULL + s], par, WAIT_LIMIT);
-        if (!failed) failed = !mbar_wait(&bars[SK_PFULL + buf], (j >> 1) & 1, WAIT_LIMIT);
-        if (failed) break;
-        fence_after_sync();
-        const uint32_t a = tmem + SK_TS + buf * SK_KEYS;
-        // B = V, MN-major.  16 bits: 64-feature blocks 8 KB apart, 8-key groups 1 KB, 16 keys 2 KB, swizzled; 8 bits: 8-feature chunks SK_CS apart,
-        // 8-key groups 128 bytes, 16 keys 256 bytes
-        const uint64_t bd = Q8 ? smem_desc(smem_u32(Vs) + buf * DC * SK_CS, 128, SK_CS) : smem_desc_sw128(smem_u32(vring) + s * vstage, SK_BLOCK, 1024);
-        constexpr uint32_t kstep = (Q8 ? 256 : 2048) >> 4;
+    const bool leader = elect_one();
+    const uint32_t idesc = instr_desc(TcFmt<T>::fmt, PAGED_ROWS, D, false, true);
+    for (int j = 0, s = 0, par = 0; j < T_tiles && !failed; ++j) {
+      const int buf = j & 1;
+      // (at 8 bits V is the expanders', and its stage may already be in its next use)
+      if constexpr (!Q8) failed = !mbar_wait_warp(&bars[SK_VFULL + s], par, WAIT_LIMIT);
+      if (!failed) failed = !mbar_wait_warp(&bars[SK_PFULL + buf], (j >> 1) & 1, WAIT_LIMIT);
+      if (failed) break;
+      fence_after_sync();
+      const uint32_t a = tmem + SK_TS + buf * SK_KEYS;
+      // B = V, MN-major.  16 bits: 64-feature blocks 8 KB apart, 8-key groups 1 KB, 16 keys 2 KB, swizzled; 8 bits: 8-feature chunks SK_CS apart,
+      // 8-key groups 128 bytes, 16 keys 256 bytes
+      const uint64_t bd = Q8 ? smem_desc(smem_u32(Vs) + buf * DC * SK_CS, 128, SK_CS) : smem_desc_sw128(smem_u32(vring) + s * vstage, SK_BLOCK, 1024);
+      constexpr uint32_t kstep = (Q8 ? 256 : 2048) >> 4;
+      if (leader) {
 #pragma unroll
         for (int ks = 0; ks < SK_KEYS / 16; ++ks)   // P of keys [32 t, 32 t + 32) sits in the first 16 columns of part t
           mma_ts_lh(tmem + SK_TO + (ks / 2) * 128, a + (ks / 2) * 32 + (ks % 2) * 8, desc_lo(bd) + ks * kstep, desc_hi(bd), idesc, (j > 0 || ks % 2 > 0) ? 1u : 0u);
         if (j == T_tiles - 1) mma_commit(&bars[SK_ODONE]);
         mma_commit(&bars[SK_PVDONE + buf]);
         if constexpr (!Q8) mma_commit(&bars[SK_VEMPTY + s]);
-        if (++s == p.vstages) s = 0, par ^= 1;
       }
+      if (++s == p.vstages) s = 0, par ^= 1;
     }
-    __syncwarp();
   } else if (warp >= SK_EX) {
     // =============================== expanders =====================================================
     const int et = tid - 32 * SK_EX;
-    // rotated and plain 16-byte columns are dealt out separately: a warp has one kind or the other
-    const int PC = DC - RC;
-    const int rdiv = max(RC, 1), pdiv = max(PC, 1);
-    const int rrow = et / rdiv, rcol = et % rdiv, rrow_step = SK_EX_THREADS / rdiv, rcol_step = SK_EX_THREADS % rdiv;
-    const int prow = et / pdiv, pcol = et % pdiv, prow_step = SK_EX_THREADS / pdiv, pcol_step = SK_EX_THREADS % pdiv;
+    // A thread keeps its row and takes every fourth 16-byte column: a warp's columns are rotated or plain for all of its lanes, its accesses to the
+    // swizzled stage and to the operand tile fall on distinct banks, and the tile needs no padding.  (With columns along the lanes and a padded
+    // tile, whose 128-byte groups the tensor core then reads in two, shared memory set the pace: a third more bytes.)
+    const int row = et & (SK_KEYS - 1), c_first = et / SK_KEYS;
+    constexpr int CSTEP = SK_EX_THREADS / SK_KEYS;
     for (int j = 0, s = 0, par = 0, vs = 0, vpar = 0; j < T_tiles; ++j) {   // (vs, vpar: 8 bits)
       const int buf = j & 1;
       const uint8_t* st = smem + s * kstage;
@@ -234,28 +233,23 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
           x[0] = unpack2<T>(w.x), x[1] = unpack2<T>(w.y), x[2] = unpack2<T>(w.z), x[3] = unpack2<T>(w.w);
         }
       };
-      // two groups of eight at a time: their chains of special functions overlap
-      for (int row = rrow, c = rcol; row < SK_KEYS && RC > 0;) {
-        int rw[2], cl[2];
-        bool on[2];
+      const float kscale = Q8 ? scl[row] : 1.f;
+      // two columns at a time: their chains of special functions overlap
+      for (int c0 = c_first; c0 < RC; c0 += 2 * CSTEP) {
+        const bool both = c0 + CSTEP < RC;   // (the same for all lanes of the warp)
         Raw raw[2];
         uint4 cq[2], sq[2];
-        float f[2];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          rw[k] = row, cl[k] = c, on[k] = row < SK_KEYS;
-          if (!on[k]) rw[k] = SK_KEYS - 1;
-          raw[k] = raw_of(st, rw[k], cl[k]);
-          const uint8_t* trow = st + trig_at + (cl[k] >> 3) * 2 * SK_BLOCK + rw[k] * 128 + (((cl[k] & 7) ^ (rw[k] & 7)) << 4);
+          const int c = k == 0 || both ? c0 + k * CSTEP : c0;
+          raw[k] = raw_of(st, row, c);
+          const uint8_t* trow = st + trig_at + (c >> 3) * 2 * SK_BLOCK + row * 128 + (((c & 7) ^ (row & 7)) << 4);
           cq[k] = *reinterpret_cast<const uint4*>(trow), sq[k] = *reinterpret_cast<const uint4*>(trow + SK_BLOCK);
-          f[k] = Q8 ? scl[rw[k]] * LOG2E : 1.f;
-          row += rrow_step, c += rcol_step;
-          if (c >= rdiv) c -= rdiv, ++row;
         }
         float2 a[2][4];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          values(raw[k], f[k], a[k]);
+          values(raw[k], kscale * LOG2E, a[k]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             if constexpr (!Q8) a[k][e] = mul2(a[k][e], make_float2(LOG2E, LOG2E));
@@ -279,9 +273,10 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
               o1[e] = pack2<T>(c2.x, c2.y), o2[e] = pack2<T>(s2.x, s2.y);
             }
           }
-          if (on[k]) {
-            *reinterpret_cast<uint4*>(kt + cl[k] * SK_CS + rw[k] * 16) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
-            *reinterpret_cast<uint4*>(kt + (DC + cl[k]) * SK_CS + rw[k] * 16) = make_uint4(o2[0], o2[1], o2[2], o2[3]);
+          if (k == 0 || both) {
+            const int c = c0 + k * CSTEP;
+            *reinterpret_cast<uint4*>(kt + c * SK_CS + row * 16) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
+            *reinterpret_cast<uint4*>(kt + (DC + c) * SK_CS + row * 16) = make_uint4(o2[0], o2[1], o2[2], o2[3]);
           }
         }
       }
@@ -296,22 +291,8 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
           return w;
         }
       };
-      for (int row = prow, c = pcol; row < SK_KEYS && PC > 0;) {
-        int rw[2], cl[2];
-        bool on[2];
-        Raw raw[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          rw[k] = row, cl[k] = RC + c, on[k] = row < SK_KEYS;
-          if (!on[k]) rw[k] = SK_KEYS - 1;
-          raw[k] = raw_of(st, rw[k], cl[k]);
-          row += prow_step, c += pcol_step;
-          if (c >= pdiv) c -= pdiv, ++row;
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-          if (on[k]) *reinterpret_cast<uint4*>(kt + cl[k] * SK_CS + rw[k] * 16) = as_16(raw[k], Q8 ? scl[rw[k]] : 1.f);
-      }
+#pragma unroll 2
+      for (int c = RC + c_first; c < DC; c += CSTEP) *reinterpret_cast<uint4*>(kt + c * SK_CS + row * 16) = as_16(raw_of(st, row, c), kscale);
       fence_async_smem();   // the tile is visible to the tensor core; the stage has been read
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[SK_KEMPTY + s]);
@@ -319,19 +300,13 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
         failed = !mbar_wait(&bars[SK_VFULL + vs], vpar, WAIT_LIMIT);
         if (j >= 2 && !failed) failed = !mbar_wait(&bars[SK_PVDONE + buf], ((j - 2) >> 1) & 1, WAIT_LIMIT);
         if (failed) break;
-        const int live = kend - (t0 + j) * SK_KEYS;
+        const bool live = (t0 + j) * SK_KEYS + row < kend;
         const uint8_t* vst = vring + vs * vstage;
         uint8_t* vt = Vs + buf * DC * SK_CS;
-        const float* vscl = reinterpret_cast<const float*>(vst + vscale_at);
-        constexpr int NV = SK_KEYS * DC / SK_EX_THREADS;
-        Raw raw[NV];
+        const float vscale = reinterpret_cast<const float*>(vst + vscale_at)[row];
 #pragma unroll
-        for (int k = 0; k < NV; ++k) raw[k] = raw_of(vst, (et + k * SK_EX_THREADS) / DC, (et + k * SK_EX_THREADS) % DC);
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          const int row = (et + k * SK_EX_THREADS) / DC, c = (et + k * SK_EX_THREADS) % DC;
-          *reinterpret_cast<uint4*>(vt + c * SK_CS + row * 16) = row < live ? as_16(raw[k], vscl[row]) : make_uint4(0, 0, 0, 0);
-        }
+        for (int c = c_first; c < DC; c += CSTEP)
+          *reinterpret_cast<uint4*>(vt + c * SK_CS + row * 16) = live ? as_16(raw_of(vst, row, c), vscale) : make_uint4(0, 0, 0, 0);
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[SK_VEMPTY + vs]);
