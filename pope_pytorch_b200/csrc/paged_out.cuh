@@ -1,7 +1,9 @@
-// What the two tcgen05 kernels of the paged attention share (sm_100a): 128 packed query rows of a key head (row = token * group + head) whose
-// unnormalised outputs sit in tensor memory leave the CTA, whole or as the part of a key range; a small kernel behind them merges the parts.
+// What the two tcgen05 kernels of the paged attention share (sm_100a): keys and queries are expanded, and 128 packed query rows of a key head (row =
+// token * group + head) whose unnormalised outputs sit in tensor memory leave the CTA, whole or as the part of a key range; a small kernel behind them merges the parts.
 // (Merged by the CTA that finished its row block last, 18 parts of a block took 50 us: one SM does not have the loads in flight.)
 #pragma once
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace pope {
@@ -25,6 +27,104 @@ inline PagedOut paged_out(const PopePagedAttnArgs& a, int nsplit, float* part_o,
 }
 inline bool rows_wide(const void* ptr, const PopeStride3& t) {   // rows on 16-byte boundaries
   return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && t.b % 8 == 0 && t.h % 8 == 0 && t.n % 8 == 0;
+}
+
+// Eight rotated features of keys, x log2(e) -> the words of a cos and of a sin.  bf16: the magnitudes come in units of ln 2 (that factor is the
+// query's) and meet the cosines in fp32, rounded once; fp16 keeps to its own range, magnitude and product are rounded.
+template <typename T> __device__ __forceinline__ void expand8(const float2 (&y)[4], const uint4& cq, const uint4& sq, uint4* oc, uint4* os) {
+  const uint32_t cw[4] = {cq.x, cq.y, cq.z, cq.w}, sw[4] = {sq.x, sq.y, sq.z, sq.w};
+  uint32_t o1[4], o2[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 a = softplus_log2_fma(y[e]);
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      const float2 c2 = mul2(a, unpack2<__half>(cw[e])), s2 = mul2(a, unpack2<__half>(sw[e]));
+      o1[e] = pack2<T>(c2.x, c2.y), o2[e] = pack2<T>(s2.x, s2.y);
+    } else {
+      const float2 m = mul2(a, make_float2(LN2, LN2));
+      const uint32_t h = pack2<__half>(m.x, m.y);
+      const __half2 c2 = __hmul2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&cw[e]));
+      const __half2 s2 = __hmul2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&sw[e]));
+      o1[e] = *reinterpret_cast<const uint32_t*>(&c2), o2[e] = *reinterpret_cast<const uint32_t*>(&s2);
+    }
+  }
+  *oc = make_uint4(o1[0], o1[1], o1[2], o1[3]), *os = make_uint4(o2[0], o2[1], o2[2], o2[3]);
+}
+
+// Eight features as they are: 16-bit words, or codes times the row's scale (value by value: what leaves as a value has all of its bits)
+template <typename T, int STORE> __device__ __forceinline__ uint4 plain8(const std::conditional_t<STORE == POPE_STORE_16, uint4, uint2>& w, float scale) {
+  if constexpr (STORE == POPE_STORE_16) {
+    return w;
+  } else {
+    float lo[4], hi[4];
+    codes_to_f32<STORE>(w.x, lo), codes_to_f32<STORE>(w.y, hi);
+    const float2 f = make_float2(scale, scale);
+    const float2 x[4] = {mul2(make_float2(lo[0], lo[1]), f), mul2(make_float2(lo[2], lo[3]), f), mul2(make_float2(hi[0], hi[1]), f), mul2(make_float2(hi[2], hi[3]), f)};
+    return make_uint4(pack2<T>(x[0].x, x[0].y), pack2<T>(x[1].x, x[1].y), pack2<T>(x[2].x, x[2].y), pack2<T>(x[3].x, x[3].y));
+  }
+}
+// ... and times log2(e) in fp32
+template <typename T, int STORE>
+__device__ __forceinline__ void log2e8(const std::conditional_t<STORE == POPE_STORE_16, uint4, uint2>& w, float scale, float2 (&y)[4]) {
+  if constexpr (STORE == POPE_STORE_16) {
+    const float2 f = make_float2(LOG2E, LOG2E);
+    y[0] = mul2(unpack2<T>(w.x), f), y[1] = mul2(unpack2<T>(w.y), f), y[2] = mul2(unpack2<T>(w.z), f), y[3] = mul2(unpack2<T>(w.w), f);
+  } else {
+    float2 t[2];
+    codes_times<STORE>(w.x, scale * LOG2E, t), y[0] = t[0], y[1] = t[1];
+    codes_times<STORE>(w.y, scale * LOG2E, t), y[2] = t[0], y[3] = t[1];
+  }
+}
+
+// What both need to make Q' = [a cos(f - b) | plain | a sin(f - b)] of a row, straight into tensor memory: lane = row, 4 columns per 8 features.
+struct PagedQ {
+  const void* q;
+  Strides sq;
+  int r, RP, wide;           // RP: r rounded up to 16; wide: rows of q on 16-byte boundaries
+  uint32_t sign;             // the sign of the softmax scale, in both halves of a word
+  const __half *ch, *sh;     // fp16 cos / sin, [Nk][r]
+};
+// A softmax thread's half of the columns of its row; zeros for a row that is no query.  bias_cs: cos, then sin, of the key head's phase offset.
+template <typename T, int D>
+__device__ __forceinline__ void paged_expand_q(const PagedQ& p, uint32_t tmem_row, int part, bool live, int b, int head, int tok, int pos, const float* bias_cs) {
+  constexpr int DC = D / 8;
+  const int r = p.r;
+  const T* qrow = static_cast<const T*>(p.q) + b * p.sq.b + head * p.sq.h + (int64_t)tok * p.sq.n;
+  const int64_t trow = (int64_t)pos * r;
+  for (int c = part; c < DC; c += 2) {
+    uint32_t rw[4] = {0, 0, 0, 0};
+    if (live && p.wide) {
+      const uint4 raw = *reinterpret_cast<const uint4*>(qrow + c * 8);
+      rw[0] = raw.x, rw[1] = raw.y, rw[2] = raw.z, rw[3] = raw.w;
+    } else if (live) {
+      const uint16_t* q16 = reinterpret_cast<const uint16_t*>(qrow + c * 8);
+      for (int e = 0; e < 4; ++e) rw[e] = q16[2 * e] | (uint32_t)q16[2 * e + 1] << 16;
+    }
+    if (c * 8 < r) {
+      uint4 cq = make_uint4(0, 0, 0, 0), sq = cq;
+      if (live) {
+        cq = *reinterpret_cast<const uint4*>(p.ch + trow + c * 8);
+        sq = *reinterpret_cast<const uint4*>(p.sh + trow + c * 8);
+      }
+      const uint32_t cw[4] = {cq.x, cq.y, cq.z, cq.w}, sw[4] = {sq.x, sq.y, sq.z, sq.w};
+      uint32_t o1[4], o2[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 xv = unpack2<T>(rw[e]), cv = unpack2<__half>(cw[e]), sv = unpack2<__half>(sw[e]);
+        const float2 bc = *reinterpret_cast<const float2*>(bias_cs + c * 8 + 2 * e), bs = *reinterpret_cast<const float2*>(bias_cs + r + c * 8 + 2 * e);
+        const float unit = std::is_same_v<T, __nv_bfloat16> ? LN2 : 1.f;
+        const float a0 = live ? softplus_fast(xv.x) * unit : 0.f, a1 = live ? softplus_fast(xv.y) * unit : 0.f;
+        o1[e] = pack2<T>(a0 * (cv.x * bc.x + sv.x * bs.x), a1 * (cv.y * bc.y + sv.y * bs.y)) ^ p.sign;
+        o2[e] = pack2<T>(a0 * (sv.x * bc.x - cv.x * bs.x), a1 * (sv.y * bc.y - cv.y * bs.y)) ^ p.sign;
+      }
+      tmem_st4(tmem_row + c * 4, o1[0], o1[1], o1[2], o1[3]);
+      tmem_st4(tmem_row + (DC + c) * 4, o2[0], o2[1], o2[2], o2[3]);
+    } else {
+      tmem_st4(tmem_row + c * 4, rw[0] ^ p.sign, rw[1] ^ p.sign, rw[2] ^ p.sign, rw[3] ^ p.sign);
+    }
+  }
+  if (r < p.RP && part == 0) tmem_st4(tmem_row + (DC + r / 8) * 4, 0, 0, 0, 0);
+  tmem_st_wait();
 }
 
 // The softmax warps (threads 0 .. 255), all products of the CTA completed: row tid & 127, half tid >> 7 of its D columns from `tmem_o` on.  TWO: the halves
@@ -78,6 +178,13 @@ __device__ __forceinline__ void paged_epilogue(const PagedOut& e, uint32_t tmem_
   }
 }
 
+inline PagedQ paged_q(const PopePagedAttnArgs& a, const TrigTables& tt) {
+  PagedQ q;
+  q.q = a.q, q.sq = Strides(a.sq), q.r = a.shape.r, q.RP = (a.shape.r + 15) / 16 * 16, q.wide = rows_wide(a.q, a.sq);
+  q.sign = a.softmax_scale < 0.f ? 0x80008000u : 0u;
+  q.ch = static_cast<const __half*>(tt.ch), q.sh = static_cast<const __half*>(tt.sh);
+  return q;
+}
 // out and lse from the parts of `blocks` row blocks, behind the kernel that wrote them
 cudaError_t launch_paged_merge(const PagedOut& e, int dtype, int d, int blocks, int blocks_per_unit, cudaStream_t st);
 

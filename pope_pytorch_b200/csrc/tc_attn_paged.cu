@@ -4,8 +4,8 @@
 // The query rows that share a key head are packed, row = token * group + head, and a CTA owns 128 of them: the heads of a group read K and V
 // once.  Three launches:
 //   tables : fp16 cos / sin rows of the positions
-//   images : K' = [a cos | plain | a sin] of every (sequence, key head), read through the page table (8-bit codes are turned into values here),
-//            in 128-row tiles in the order in which the tensor core reads them; every row block sweeps the keys, so they are expanded once.
+//   images : K' = [a cos | plain | a sin] of every (sequence, key head), read through the page table (8-bit codes are turned into values here; the
+//            head's phase bias sits in Q'), in 128-row tiles in the order in which the tensor core reads them; every row block sweeps the keys, so they are expanded once.
 //            Of a cache that holds 8 bits also V, as 16-bit rows.
 //   sweep  : S = Q' K'^T with Q' in tensor memory, online softmax, O += P V with P in tensor memory, 128 keys a step; K' by one bulk copy, V by
 //            tensor-map boxes from the pages.  Small grids are cut along the keys, a fourth launch merges the parts.
@@ -98,8 +98,6 @@ struct PagedImageP {
   PagedPtrs c;
   int B, Nk, r, RP;          // RP: r rounded up to 16, columns r .. of the sines are zero
   const __half *ch, *sh;     // fp16 cos / sin, [Nk][r]
-  const float* bias;
-  int64_t bias_sh;
   uint8_t* kimg;             // [unit][128-row tile][chunk][128 rows][16 B]
   void* vrows;               // 8-bit stores: [unit][rows][D]
   int tiles;                 // 64-row tiles of a unit's image
@@ -120,101 +118,63 @@ __global__ void __launch_bounds__(256, 6) paged_image_kernel(PagedImageP p) {
   __shared__ int64_t row0_s;
   if (tid == 0) row0_s = rows > 0 ? paged_row(p.c, b, hk, key0) : 0;
   const int KC = DC + p.RP / 8;
-  float* bias_c = reinterpret_cast<float*>(stage + KC * CS64);
-  float* bias_s = bias_c + r;
-  for (int i = tid; i < r; i += 256) sincos_reduced(p.bias[hk * p.bias_sh + i], &bias_s[i], &bias_c[i]);
   __syncthreads();
   const int64_t row0 = max(row0_s, (int64_t)0);   // (a page outside the pool: reported, another one read)
   const int c = tid % DC, first = tid / DC;
   const bool active = first < RPP, rotated = c * 8 < r;
-  uint4 raw[NIT];
+  using Raw = std::conditional_t<Q8, uint2, uint4>;   // eight features
+  Raw raw[NIT];
   float scale[NIT];
   auto load = [&](const uint8_t* pool, const float* scales, int base) {
 #pragma unroll
     for (int it = 0; it < NIT; ++it) {
       const int row = first + it * RPP + base;
-      raw[it] = make_uint4(0, 0, 0, 0), scale[it] = 0.f;
+      raw[it] = Raw{}, scale[it] = 0.f;
       if (!active || row >= rows) continue;
-      if constexpr (Q8) {
-        const uint2 x = *reinterpret_cast<const uint2*>(pool + (row0 + row) * D + c * 8);
-        raw[it].x = x.x, raw[it].y = x.y, scale[it] = scales[row0 + row];
-      } else {
-        raw[it] = *reinterpret_cast<const uint4*>(pool + ((row0 + row) * D + c * 8) * 2);
-      }
-    }
-  };
-  auto values = [&](int it, float2 (&x)[4]) {
-    if constexpr (Q8) {
-      float lo[4], hi[4];
-      codes_to_f32<STORE>(raw[it].x, lo), codes_to_f32<STORE>(raw[it].y, hi);
-      const float s = scale[it];
-      x[0] = make_float2(lo[0] * s, lo[1] * s), x[1] = make_float2(lo[2] * s, lo[3] * s);
-      x[2] = make_float2(hi[0] * s, hi[1] * s), x[3] = make_float2(hi[2] * s, hi[3] * s);
-    } else {
-      x[0] = unpack2<T>(raw[it].x), x[1] = unpack2<T>(raw[it].y), x[2] = unpack2<T>(raw[it].z), x[3] = unpack2<T>(raw[it].w);
+      raw[it] = *reinterpret_cast<const Raw*>(pool + ((row0 + row) * D + c * 8) * (Q8 ? 1 : 2));
+      if constexpr (Q8) scale[it] = scales[row0 + row];
     }
   };
 #pragma unroll 1
   for (int base = 0; base < IMAGE_ROWS; base += NIT * RPP) {
-  load(p.c.k, p.c.k_scales, base);
-  if (rotated) {
-    const float *cb = bias_c + c * 8, *sb = bias_s + c * 8;
-    uint4 cq[NIT], sq[NIT];
+    load(p.c.k, p.c.k_scales, base);
+    if (rotated) {
+      uint4 cq[NIT], sq[NIT];
 #pragma unroll
-    for (int it = 0; it < NIT; ++it) {
-      const int row = first + it * RPP + base;
-      cq[it] = sq[it] = make_uint4(0, 0, 0, 0);   // (rows behind the last key become zeros)
-      if (active && row < rows) {
-        cq[it] = *reinterpret_cast<const uint4*>(p.ch + (int64_t)(key0 + row) * r + c * 8);
-        sq[it] = *reinterpret_cast<const uint4*>(p.sh + (int64_t)(key0 + row) * r + c * 8);
+      for (int it = 0; it < NIT; ++it) {
+        const int row = first + it * RPP + base;
+        cq[it] = sq[it] = make_uint4(0, 0, 0, 0);   // (rows behind the last key become zeros)
+        if (active && row < rows) {
+          cq[it] = *reinterpret_cast<const uint4*>(p.ch + (int64_t)(key0 + row) * r + c * 8);
+          sq[it] = *reinterpret_cast<const uint4*>(p.sh + (int64_t)(key0 + row) * r + c * 8);
+        }
+      }
+#pragma unroll
+      for (int it = 0; it < NIT; ++it) {
+        const int row = first + it * RPP + base;
+        if (!active || row >= IMAGE_ROWS) continue;
+        float2 y[4];
+        log2e8<T, STORE>(raw[it], scale[it], y);
+        expand8<T>(y, cq[it], sq[it], reinterpret_cast<uint4*>(stage + c * CS64 + row * 16), reinterpret_cast<uint4*>(stage + (DC + c) * CS64 + row * 16));
+      }
+    } else {
+#pragma unroll
+      for (int it = 0; it < NIT; ++it) {
+        const int row = first + it * RPP + base;
+        if (!active || row >= IMAGE_ROWS) continue;
+        *reinterpret_cast<uint4*>(stage + c * CS64 + row * 16) = plain8<T, STORE>(raw[it], scale[it]);
+        if (c * 8 < p.RP) *reinterpret_cast<uint4*>(stage + (DC + c) * CS64 + row * 16) = make_uint4(0, 0, 0, 0);
       }
     }
+    if constexpr (Q8) {   // V of the same rows, zeros behind the last key
+      load(p.c.v, p.c.v_scales, base);
 #pragma unroll
-    for (int it = 0; it < NIT; ++it) {
-      const int row = first + it * RPP + base;
-      if (!active || row >= IMAGE_ROWS) continue;
-      const uint32_t cw[4] = {cq[it].x, cq[it].y, cq[it].z, cq[it].w}, sw[4] = {sq[it].x, sq[it].y, sq[it].z, sq[it].w};
-      float2 x[4];
-      values(it, x);
-      uint32_t o1[4], o2[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float2 cv = unpack2<__half>(cw[e]), sv = unpack2<__half>(sw[e]);   // cos(f + b), sin(f + b)
-        const float c0 = cv.x * cb[2 * e] - sv.x * sb[2 * e], s0 = sv.x * cb[2 * e] + cv.x * sb[2 * e];
-        const float c1 = cv.y * cb[2 * e + 1] - sv.y * sb[2 * e + 1], s1 = sv.y * cb[2 * e + 1] + cv.y * sb[2 * e + 1];
-        const float a0 = softplus_fast(x[e].x), a1 = softplus_fast(x[e].y);
-        o1[e] = pack2<T>(a0 * c0, a1 * c1), o2[e] = pack2<T>(a0 * s0, a1 * s1);
+      for (int it = 0; it < NIT; ++it) {
+        const int row = first + it * RPP + base;
+        if (!active || row >= IMAGE_ROWS) continue;
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.vrows) + ((int64_t)u * p.tiles * IMAGE_ROWS + key0 + row) * D + c * 8) = plain8<T, STORE>(raw[it], scale[it]);
       }
-      *reinterpret_cast<uint4*>(stage + c * CS64 + row * 16) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
-      *reinterpret_cast<uint4*>(stage + (DC + c) * CS64 + row * 16) = make_uint4(o2[0], o2[1], o2[2], o2[3]);
     }
-  } else {
-#pragma unroll
-    for (int it = 0; it < NIT; ++it) {
-      const int row = first + it * RPP + base;
-      if (!active || row >= IMAGE_ROWS) continue;
-      uint4 o = raw[it];
-      if constexpr (Q8) {
-        float2 x[4];
-        values(it, x);
-        o = make_uint4(pack2<T>(x[0].x, x[0].y), pack2<T>(x[1].x, x[1].y), pack2<T>(x[2].x, x[2].y), pack2<T>(x[3].x, x[3].y));
-      }
-      *reinterpret_cast<uint4*>(stage + c * CS64 + row * 16) = o;
-      if (c * 8 < p.RP) *reinterpret_cast<uint4*>(stage + (DC + c) * CS64 + row * 16) = make_uint4(0, 0, 0, 0);
-    }
-  }
-  if constexpr (Q8) {   // V of the same rows, zeros behind the last key
-    load(p.c.v, p.c.v_scales, base);
-#pragma unroll
-    for (int it = 0; it < NIT; ++it) {
-      const int row = first + it * RPP + base;
-      if (!active || row >= IMAGE_ROWS) continue;
-      float2 x[4];
-      values(it, x);
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.vrows) + ((int64_t)u * p.tiles * IMAGE_ROWS + key0 + row) * D + c * 8) =
-          make_uint4(pack2<T>(x[0].x, x[0].y), pack2<T>(x[1].x, x[1].y), pack2<T>(x[2].x, x[2].y), pack2<T>(x[3].x, x[3].y));
-    }
-  }
   }
   __syncthreads();
   // the image leaves in its own byte order, coalesced: tiles 2 t and 2 t + 1 share a 128-row tile
@@ -228,14 +188,13 @@ __global__ void __launch_bounds__(256, 6) paged_image_kernel(PagedImageP p) {
 // ---- sweep -----------------------------------------------------------------------------------------------
 struct PagedSweepP {
   int Hk, G, Nq, Nk, r, RP, nsplit, blocks, tiles;   // blocks: row blocks per unit; tiles: 64-row tiles of a unit's image
-  int page_size, max_pages, num_pages, q_wide;          // q_wide: rows of q on 16-byte boundaries
+  int page_size, max_pages, num_pages;
   float scale_log2;                                     // its magnitude; the sign sits in Q'
-  uint32_t q_sign;
   const int32_t *page_table, *seq_lens, *counts;
-  const void* q;
-  Strides sq;
+  const float* bias;
+  int64_t bias_sh;
   const uint8_t* kimg;
-  const __half *ch, *sh;
+  PagedQ q;
   PagedOut e;
   unsigned int* status;
 };
@@ -268,7 +227,8 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP 
   uint8_t* Ks = smem;
   uint8_t* Vs = Ks + 2 * KBUF;                                    // (KBUF is a multiple of 4 KB)
   float* xch = reinterpret_cast<float*>(Vs + 2 * VBUF);           // [2 step parities][2 parts][128 rows] row maxima
-  uint64_t* bars = reinterpret_cast<uint64_t*>(xch + 4 * PS_ROWS);
+  float* bias_cs = xch + 4 * PS_ROWS;                             // [2][r]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(bias_cs + 2 * p.r);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + PS_COUNT);
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -395,46 +355,12 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP 
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const int row_bar = 1 + (warp & 3);   // named barrier of the two warps that share 32 rows
     auto row_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(row_bar) : "memory"); };
-    {
-      // Q' = [a cos f | plain | a sin f], expanded here from q and the fp16 tables straight into tensor memory; rows that are no queries are zero
-      constexpr int DC = D >> 3;
-      const T* qrow = static_cast<const T*>(p.q) + b * p.sq.b + head * p.sq.h + (int64_t)tok * p.sq.n;
-      const int64_t trow = (int64_t)pos * p.r;
-      for (int c = part; c < DC; c += 2) {
-        uint32_t rw[4] = {0, 0, 0, 0};
-        if (live && p.q_wide) {
-          const uint4 raw = *reinterpret_cast<const uint4*>(qrow + c * 8);
-          rw[0] = raw.x, rw[1] = raw.y, rw[2] = raw.z, rw[3] = raw.w;
-        } else if (live) {
-          const uint16_t* q16 = reinterpret_cast<const uint16_t*>(qrow + c * 8);
-          for (int e = 0; e < 4; ++e) rw[e] = q16[2 * e] | (uint32_t)q16[2 * e + 1] << 16;
-        }
-        if (c * 8 < p.r) {
-          uint4 cq = make_uint4(0, 0, 0, 0), sq = cq;
-          if (live) {
-            cq = *reinterpret_cast<const uint4*>(p.ch + trow + c * 8);
-            sq = *reinterpret_cast<const uint4*>(p.sh + trow + c * 8);
-          }
-          const uint32_t cw[4] = {cq.x, cq.y, cq.z, cq.w}, sw[4] = {sq.x, sq.y, sq.z, sq.w};
-          uint32_t o1[4], o2[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 xv = unpack2<T>(rw[e]), cv = unpack2<__half>(cw[e]), sv = unpack2<__half>(sw[e]);
-            const float a0 = live ? softplus_fast(xv.x) : 0.f, a1 = live ? softplus_fast(xv.y) : 0.f;
-            o1[e] = pack2<T>(a0 * cv.x, a1 * cv.y) ^ p.q_sign, o2[e] = pack2<T>(a0 * sv.x, a1 * sv.y) ^ p.q_sign;
-          }
-          tmem_st4(tmem + lane_base + c * 4, o1[0], o1[1], o1[2], o1[3]);
-          tmem_st4(tmem + lane_base + (DC + c) * 4, o2[0], o2[1], o2[2], o2[3]);
-        } else {
-          tmem_st4(tmem + lane_base + c * 4, rw[0] ^ p.q_sign, rw[1] ^ p.q_sign, rw[2] ^ p.q_sign, rw[3] ^ p.q_sign);
-          if (c * 8 < p.RP) tmem_st4(tmem + lane_base + (DC + c) * 4, 0, 0, 0, 0);
-        }
-      }
-      tmem_st_wait();
-      fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[PS_QFULL]);
-    }
+    for (int i = tid; i < p.r; i += 32 * PS_SM_WARPS) sincos_reduced(p.bias[hk * p.bias_sh + i], &bias_cs[p.r + i], &bias_cs[i]);
+    asm volatile("bar.sync 5, %0;" ::"n"(32 * PS_SM_WARPS) : "memory");
+    paged_expand_q<T, D>(p.q, tmem + lane_base, part, live, b, head, tok, pos, bias_cs);
+    fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars[PS_QFULL]);
     float m_run = -CUDART_INF_F, l_run = 0.f;
     const int limit = live ? min(pos, kend - 1) : -1;   // last key that this row sees
 
@@ -590,17 +516,15 @@ template <typename T, int STORE, int D> static cudaError_t paged_sweep_t(const P
   if (!im.c.status) return cudaErrorInvalidSymbol;
   im.B = s.B, im.Nk = s.Nk, im.r = s.r, im.RP = RP, im.tiles = tiles;
   im.ch = static_cast<const __half*>(tt.ch), im.sh = static_cast<const __half*>(tt.sh);
-  im.bias = a.embed.bias, im.bias_sh = a.embed.bias_stride_h;
   im.kimg = base + ws.kimg, im.vrows = base + ws.vrows;
   PagedSweepP p = {};
   p.Hk = s.Hk, p.G = s.H / s.Hk, p.Nq = s.Nq, p.Nk = s.Nk, p.r = s.r, p.RP = RP, p.tiles = tiles;
   p.nsplit = sweep_split(s), p.blocks = sweep_blocks(s);
   p.page_size = kv.page_size, p.max_pages = kv.max_pages_per_seq, p.num_pages = kv.num_pages;
-  p.q_wide = rows_wide(a.q, a.sq);
-  p.scale_log2 = std::abs(a.softmax_scale) * LOG2E, p.q_sign = a.softmax_scale < 0.f ? 0x80008000u : 0u;
+  p.scale_log2 = std::abs(a.softmax_scale) * LOG2E;
   p.page_table = kv.page_table, p.seq_lens = kv.seq_lens, p.counts = a.counts;
-  p.q = a.q, p.sq = Strides(a.sq);
-  p.kimg = im.kimg, p.ch = im.ch, p.sh = im.sh;
+  p.bias = a.embed.bias, p.bias_sh = a.embed.bias_stride_h;
+  p.kimg = im.kimg, p.q = paged_q(a, tt);
   p.e = paged_out(a, p.nsplit, reinterpret_cast<float*>(base + ws.part_o), reinterpret_cast<float*>(base + ws.part_ml));
   p.status = im.c.status;
   CUtensorMap tmap_v;
@@ -612,11 +536,11 @@ template <typename T, int STORE, int D> static cudaError_t paged_sweep_t(const P
   if (!ok) return cudaErrorNotSupported;
   const int KD = s.d + RP;
   // (every CTA allocates all 512 TMEM columns: two must not share an SM)
-  const size_t smem = std::max<size_t>(2 * (size_t)PS_KEYS * KD * 2 + 2 * (size_t)((s.d + 63) / 64) * PS_KEYS * 128 + 4 * PS_ROWS * 4 + PS_COUNT * 8 + 16 + 1024, 120 * 1024);
+  const size_t smem = std::max<size_t>(2 * (size_t)PS_KEYS * KD * 2 + 2 * (size_t)((s.d + 63) / 64) * PS_KEYS * 128 + 4 * PS_ROWS * 4 + 2 * (size_t)s.r * 4 + PS_COUNT * 8 + 16 + 1024, 120 * 1024);
   cudaError_t e = ensure_max_smem<paged_sweep_kernel<T, D, Q8>>();
   if (e != cudaSuccess) return e;
   if (s.r > 0 && (e = launch_paged_tables(a.embed, s.Nk, s.r, tt.ch, tt.sh, nullptr, 0, st)) != cudaSuccess) return e;
-  const size_t ismem = (size_t)(KD / 8) * CS64 + 2 * (size_t)s.r * sizeof(float);
+  const size_t ismem = (size_t)(KD / 8) * CS64;
   if ((e = launch_dependent(paged_image_kernel<T, STORE, D>, dim3((unsigned)((s.Nk + 127) / 128 * 2), (unsigned)(s.B * s.Hk)), dim3(256), ismem, st, im)) != cudaSuccess) return e;
   e = launch_dependent(paged_sweep_kernel<T, D, Q8>, dim3((unsigned)(s.B * s.Hk * p.blocks * p.nsplit)), dim3(PS_THREADS), smem, st, p, tmap_v);
   return e != cudaSuccess || p.nsplit == 1 ? e : launch_paged_merge(p.e, s.dtype, s.d, s.B * s.Hk * p.blocks, p.blocks, st);
@@ -645,12 +569,14 @@ bool attn_paged_supported(const PopePagedAttnArgs& a) {
   return a.cache.kv.page_size % 64 == 0;
 }
 
+// By the rows that share a key head.  Up to 16 the keys become product fragments in registers ((8, 32 / 8, 2000, 128), r = 64, us: 16-bit cache 8 rows 23
+// against 31 by the expanders in front of tcgen05, 16 rows 29 / 31, 20 rows 38 / 31; int8 16 rows 32 / 39).  Up to two row blocks they are
+// expanded on the chip, from three on written to memory once ((1, 32 / 8, 32768, 128), r = 64: 256 rows 83 / 98, 384 rows 111 / 109, 512 rows 153 / 128;
+// int8 105 / 114, 146 / 125; int8 with r = 128 and 256 rows 129 / 129).
 enum class Paged { kRows, kStream, kSweep };
 static Paged paged_kernel(const PopeShape& s) {
   const int64_t rows = (int64_t)s.Nq * (s.H / s.Hk);
-  const char* e = getenv("PAGED_PATH");
-  if (e) return e[0] == '0' ? (rows > 16 ? Paged::kStream : Paged::kRows) : e[0] == '1' ? Paged::kStream : Paged::kSweep;
-  return rows <= 16 ? Paged::kRows : rows <= 256 ? Paged::kStream : Paged::kSweep;
+  return rows <= 16 ? Paged::kRows : rows <= 2 * PAGED_ROWS ? Paged::kStream : Paged::kSweep;
 }
 
 size_t attn_paged_workspace(const PopePagedAttnArgs& a) {

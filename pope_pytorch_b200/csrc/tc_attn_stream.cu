@@ -23,15 +23,12 @@ namespace pope {
 
 struct PagedStreamP {
   int Hk, G, Nq, Nk, r, RP, nsplit, blocks, kstages, vstages;
-  int page_size, max_pages, num_pages, q_wide;
+  int page_size, max_pages, num_pages;
   float scale_log2;          // its magnitude; the sign sits in Q'
-  uint32_t q_sign;
   const int32_t *page_table, *seq_lens, *counts;
-  const void* q;
-  Strides sq;
-  const __half *ch, *sh;     // fp16 cos / sin, [Nk][r]
   const float* bias;
   int64_t bias_sh;
+  PagedQ q;
   PagedOut e;
   unsigned int* status;
 };
@@ -64,7 +61,6 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
     paged_stream_kernel(PagedStreamP p, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                         const __grid_constant__ CUtensorMap tmap_t, const __grid_constant__ CUtensorMap tmap_ks, const __grid_constant__ CUtensorMap tmap_vs) {
   constexpr bool Q8 = STORE != POPE_STORE_16;
-  constexpr bool BF = std::is_same_v<T, __nv_bfloat16>;   // its magnitudes come in units of ln 2; fp16 keeps to its own range
   constexpr int DC = D / 8, KBLK = (D * (Q8 ? 1 : 2) + 127) / 128;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -224,15 +220,6 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
       };
       using Raw = std::conditional_t<Q8, uint2, uint4>;   // eight features
       auto raw_of = [&](const uint8_t* base, int row, int c) { return *reinterpret_cast<const Raw*>(swizzled(base, row, c * (Q8 ? 8 : 16))); };
-      auto values = [&](const Raw& w, float scale, float2 (&x)[4]) {
-        if constexpr (Q8) {
-          float2 y[2];
-          codes_times<STORE>(w.x, scale, y), x[0] = y[0], x[1] = y[1];
-          codes_times<STORE>(w.y, scale, y), x[2] = y[0], x[3] = y[1];
-        } else {
-          x[0] = unpack2<T>(w.x), x[1] = unpack2<T>(w.y), x[2] = unpack2<T>(w.z), x[3] = unpack2<T>(w.w);
-        }
-      };
       const float kscale = Q8 ? scl[row] : 1.f;
       // two columns at a time: their chains of special functions overlap
       for (int c0 = c_first; c0 < RC; c0 += 2 * CSTEP) {
@@ -246,53 +233,20 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
           const uint8_t* trow = st + trig_at + (c >> 3) * 2 * SK_BLOCK + row * 128 + (((c & 7) ^ (row & 7)) << 4);
           cq[k] = *reinterpret_cast<const uint4*>(trow), sq[k] = *reinterpret_cast<const uint4*>(trow + SK_BLOCK);
         }
-        float2 a[2][4];
+        float2 y[2][4];
+        uint4 oc[2], os[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) log2e8<T, STORE>(raw[k], kscale, y[k]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) expand8<T>(y[k], cq[k], sq[k], &oc[k], &os[k]);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          values(raw[k], kscale * LOG2E, a[k]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if constexpr (!Q8) a[k][e] = mul2(a[k][e], make_float2(LOG2E, LOG2E));
-            a[k][e] = softplus_log2_fma(a[k][e]);
-            if constexpr (!BF) a[k][e] = mul2(a[k][e], make_float2(LN2, LN2));
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint32_t cw[4] = {cq[k].x, cq[k].y, cq[k].z, cq[k].w}, sw[4] = {sq[k].x, sq[k].y, sq[k].z, sq[k].w};
-          uint32_t o1[4], o2[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if constexpr (!BF) {
-              const uint32_t h = pack2<__half>(a[k][e].x, a[k][e].y);
-              const __half2 c2 = __hmul2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&cw[e]));
-              const __half2 s2 = __hmul2(*reinterpret_cast<const __half2*>(&h), *reinterpret_cast<const __half2*>(&sw[e]));
-              o1[e] = *reinterpret_cast<const uint32_t*>(&c2), o2[e] = *reinterpret_cast<const uint32_t*>(&s2);
-            } else {
-              const float2 c2 = mul2(a[k][e], unpack2<__half>(cw[e])), s2 = mul2(a[k][e], unpack2<__half>(sw[e]));
-              o1[e] = pack2<T>(c2.x, c2.y), o2[e] = pack2<T>(s2.x, s2.y);
-            }
-          }
-          if (k == 0 || both) {
-            const int c = c0 + k * CSTEP;
-            *reinterpret_cast<uint4*>(kt + c * SK_CS + row * 16) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
-            *reinterpret_cast<uint4*>(kt + (DC + c) * SK_CS + row * 16) = make_uint4(o2[0], o2[1], o2[2], o2[3]);
-          }
+          const int c = c0 + k * CSTEP;
+          if (k == 0 || both) *reinterpret_cast<uint4*>(kt + c * SK_CS + row * 16) = oc[k], *reinterpret_cast<uint4*>(kt + (DC + c) * SK_CS + row * 16) = os[k];
         }
       }
-      auto as_16 = [&](const Raw& w, float scale) {
-        if constexpr (Q8) {   // (value by value: a value that leaves as it is has all of its bits)
-          float lo[4], hi[4];
-          codes_to_f32<STORE>(w.x, lo), codes_to_f32<STORE>(w.y, hi);
-          const float2 f = make_float2(scale, scale);
-          const float2 x[4] = {mul2(make_float2(lo[0], lo[1]), f), mul2(make_float2(lo[2], lo[3]), f), mul2(make_float2(hi[0], hi[1]), f), mul2(make_float2(hi[2], hi[3]), f)};
-          return make_uint4(pack2<T>(x[0].x, x[0].y), pack2<T>(x[1].x, x[1].y), pack2<T>(x[2].x, x[2].y), pack2<T>(x[3].x, x[3].y));
-        } else {
-          return w;
-        }
-      };
 #pragma unroll 2
-      for (int c = RC + c_first; c < DC; c += CSTEP) *reinterpret_cast<uint4*>(kt + c * SK_CS + row * 16) = as_16(raw_of(st, row, c), kscale);
+      for (int c = RC + c_first; c < DC; c += CSTEP) *reinterpret_cast<uint4*>(kt + c * SK_CS + row * 16) = plain8<T, STORE>(raw_of(st, row, c), kscale);
       fence_async_smem();   // the tile is visible to the tensor core; the stage has been read
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[SK_KEMPTY + s]);
@@ -306,7 +260,7 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
         const float vscale = reinterpret_cast<const float*>(vst + vscale_at)[row];
 #pragma unroll
         for (int c = c_first; c < DC; c += CSTEP)
-          *reinterpret_cast<uint4*>(vt + c * SK_CS + row * 16) = live ? as_16(raw_of(vst, row, c), vscale) : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(vt + c * SK_CS + row * 16) = live ? plain8<T, STORE>(raw_of(vst, row, c), vscale) : make_uint4(0, 0, 0, 0);
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[SK_VEMPTY + vs]);
@@ -321,48 +275,10 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
     const int rho = rb * PAGED_ROWS + rloc, tok = rho / p.G, head = hk + (rho - tok * p.G) * p.Hk, pos = len - cnt + tok;
     const bool live = rloc < rows && pos >= 0, warp_live = (warp & 3) * 32 < rows;   // (warps without a query only keep the steps' pace)
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    {
-      // Q' = [a cos(f - b) | plain | a sin(f - b)], straight into tensor memory; rows that are no queries are zero
-      const T* qrow = static_cast<const T*>(p.q) + b * p.sq.b + head * p.sq.h + (int64_t)tok * p.sq.n;
-      const int64_t trow = (int64_t)pos * r;
-      for (int c = part; c < DC; c += 2) {
-        uint32_t rw[4] = {0, 0, 0, 0};
-        if (live && p.q_wide) {
-          const uint4 raw = *reinterpret_cast<const uint4*>(qrow + c * 8);
-          rw[0] = raw.x, rw[1] = raw.y, rw[2] = raw.z, rw[3] = raw.w;
-        } else if (live) {
-          const uint16_t* q16 = reinterpret_cast<const uint16_t*>(qrow + c * 8);
-          for (int e = 0; e < 4; ++e) rw[e] = q16[2 * e] | (uint32_t)q16[2 * e + 1] << 16;
-        }
-        if (c < RC) {
-          uint4 cq = make_uint4(0, 0, 0, 0), sq = cq;
-          if (live) {
-            cq = *reinterpret_cast<const uint4*>(p.ch + trow + c * 8);
-            sq = *reinterpret_cast<const uint4*>(p.sh + trow + c * 8);
-          }
-          const uint32_t cw[4] = {cq.x, cq.y, cq.z, cq.w}, sw[4] = {sq.x, sq.y, sq.z, sq.w};
-          uint32_t o1[4], o2[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 xv = unpack2<T>(rw[e]), cv = unpack2<__half>(cw[e]), sv = unpack2<__half>(sw[e]);
-            const float2 bc = *reinterpret_cast<const float2*>(bias_cs + c * 8 + 2 * e), bs = *reinterpret_cast<const float2*>(bias_cs + r + c * 8 + 2 * e);
-            const float unit = BF ? LN2 : 1.f;
-            const float a0 = live ? softplus_fast(xv.x) * unit : 0.f, a1 = live ? softplus_fast(xv.y) * unit : 0.f;
-            o1[e] = pack2<T>(a0 * (cv.x * bc.x + sv.x * bs.x), a1 * (cv.y * bc.y + sv.y * bs.y)) ^ p.q_sign;
-            o2[e] = pack2<T>(a0 * (sv.x * bc.x - cv.x * bs.x), a1 * (sv.y * bc.y - cv.y * bs.y)) ^ p.q_sign;
-          }
-          tmem_st4(tmem + lane_base + c * 4, o1[0], o1[1], o1[2], o1[3]);
-          tmem_st4(tmem + lane_base + (DC + c) * 4, o2[0], o2[1], o2[2], o2[3]);
-        } else {
-          tmem_st4(tmem + lane_base + c * 4, rw[0] ^ p.q_sign, rw[1] ^ p.q_sign, rw[2] ^ p.q_sign, rw[3] ^ p.q_sign);
-        }
-      }
-      if (RC * 8 < p.RP && part == 0) tmem_st4(tmem + lane_base + (DC + RC) * 4, 0, 0, 0, 0);
-      tmem_st_wait();
-      fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[SK_QFULL]);
-    }
+    paged_expand_q<T, D>(p.q, tmem + lane_base, part, live, b, head, tok, pos, bias_cs);
+    fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars[SK_QFULL]);
     float m_run = -CUDART_INF_F, l_run = 0.f;
     const int limit = live ? min(pos, kend - 1) : -1;   // last key that this row sees
 
@@ -497,10 +413,10 @@ template <typename T, int STORE, int D> static cudaError_t paged_stream_t(const 
   PagedStreamP p = {};
   p.Hk = s.Hk, p.G = s.H / s.Hk, p.Nq = s.Nq, p.Nk = s.Nk, p.r = s.r, p.RP = round_up(s.r, 16);
   p.nsplit = stream_split(s), p.blocks = stream_blocks(s);
-  p.page_size = kv.page_size, p.max_pages = kv.max_pages_per_seq, p.num_pages = kv.num_pages, p.q_wide = rows_wide(a.q, a.sq);
-  p.scale_log2 = std::abs(a.softmax_scale) * LOG2E, p.q_sign = a.softmax_scale < 0.f ? 0x80008000u : 0u;
+  p.page_size = kv.page_size, p.max_pages = kv.max_pages_per_seq, p.num_pages = kv.num_pages;
+  p.scale_log2 = std::abs(a.softmax_scale) * LOG2E;
   p.page_table = kv.page_table, p.seq_lens = kv.seq_lens, p.counts = a.counts;
-  p.q = a.q, p.sq = Strides(a.sq), p.ch = static_cast<const __half*>(tt.ch), p.sh = static_cast<const __half*>(tt.sh);
+  p.q = paged_q(a, tt);
   p.bias = a.embed.bias, p.bias_sh = a.embed.bias_stride_h;
   p.e = paged_out(a, p.nsplit, reinterpret_cast<float*>(base + ws.part_o), reinterpret_cast<float*>(base + ws.part_ml));
   p.status = tc_status_ptr();

@@ -26,9 +26,10 @@ def attend(q, k, v, freqs, bias, lens, counts, scale, store=None):
     """q (b, h, n, d) in its type; k, v: lists of (hk, len, d) held values; -> out, lse, worst, rms (fp64, CPU)."""
     dt = q.dtype
     u_out = half_step(dt)
-    u = half_step(dt if store is None else torch.float16)
     b, h, n, d = q.shape
     hk, r = k[0].shape[0], freqs.shape[-1]
+    # the type of the products' operands: that of q, but fp16 for an 8-bit cache and at most 16 rows of a key head
+    u = half_step(torch.float16 if store is not None and n * h // hk <= 16 else dt)
     out = torch.zeros(b, h, n, d, dtype=torch.float64)
     lse = torch.full((b, h, n), -math.inf, dtype=torch.float64)
     worst, rms2 = torch.zeros_like(out), torch.zeros_like(out)
@@ -53,9 +54,11 @@ def attend(q, k, v, freqs, bias, lens, counts, scale, store=None):
                 out[i, head, row], lse[i, head, row] = o, torch.logsumexp(s, 0)
                 worst[i, head, row] = 1.1 * (u_out * o.abs() + 2 * u * (p @ vv.abs()) + (p * ds) @ (vv.abs() + o.abs()))
                 if ds2.max() > 1 / 64:
-                    # scores that are off by an eighth and more: exp(ds) - 1 is no longer ds, and the first order says nothing about the
-                    # 2-norm.  What holds: out is a mean of the rows of v whatever the scores are, so two of them differ by 2 max |v| at most.
-                    rms2[i, head, row] = (2 * vv.abs().max(0).values) ** 2
+                    # scores that are off by an eighth and more: exp(ds) - 1 is no longer ds, and the first order says nothing (where one key
+                    # has all of the weight it gives ds |v| of that key alone, while another key may take its place).  What holds: out is a
+                    # mean of the rows of v whatever the scores are, so two of them differ by 2 max |v| at most, next to the other roundings.
+                    far = 2 * vv.abs().max(0).values
+                    worst[i, head, row], rms2[i, head, row] = 1.1 * (1 + u_out + 2 * u) * far, far ** 2
                     continue
                 rms2[i, head, row] = (u_out * o) ** 2 / 3 + (p * p) @ vv.square() * 2 * u * u / 3 + (p * p * ds2) @ (vv - o).square()
     return out, lse, worst, rms2.sqrt()

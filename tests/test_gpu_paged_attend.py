@@ -49,6 +49,17 @@ CASES = [
     ([385, 200], 70, [70, 41], 6, 2, 96, 96, BF, F8, 192),
     ([100], 40, None, 5, 1, 128, 24, HF, I8, 64),
     ([129], 129, None, 4, 2, 64, 64, BF, F8, 64),
+    # more than 256 rows of a key head
+    ([300, 150], 100, [100, 60], 8, 2, 96, 48, HF, None, 64),
+    ([400], 300, None, 1, 1, 64, 0, BF, None, 64),
+    ([310, 129], 150, [1, 150], 4, 2, 128, 128, BF, None, 128),
+    ([290, 64], 290, None, 2, 2, 64, 24, BF, F8, 64),
+    ([200], 90, None, 6, 2, 96, 8, HF, I8, 192),
+    ([333], 100, None, 4, 1, 128, 64, BF, I8, 256),
+    # 17 to 256 of them
+    ([200, 100], 20, [20, 9], 4, 4, 96, 96, BF, F8, 64),
+    ([500], 64, None, 4, 1, 128, 128, HF, I8, 128),
+    ([70, 65, 64], 18, None, 1, 1, 64, 0, HF, F8, 64),
 ]
 
 
@@ -106,7 +117,7 @@ def test_what_is_not_a_key_never_counts(store):
         fill(c, lens, torch.Generator(device=DEV).manual_seed(8))
     q = torch.randn(2, h, new, d, device=DEV, generator=g).bfloat16()
     emb = table(r, hk, 200, g)
-    for rows in (q, q[:, :, :1], q.repeat(1, 1, 25, 1)):
+    for rows in (q, q[:, :, :1], q.repeat(1, 1, 6, 1), q.repeat(1, 1, 25, 1)):
         got, want = cache.attend(rows, emb), clean.attend(rows, emb)
         assert torch.isfinite(got).all() and torch.equal(got, want)
     cache.append(bad[:, :, :3], bad[:, :, :3])
@@ -117,7 +128,7 @@ def test_what_is_not_a_key_never_counts(store):
 
 
 @pytest.mark.parametrize("store", [None, I8])
-@pytest.mark.parametrize("new", [4, 150])
+@pytest.mark.parametrize("new", [4, 40, 150])
 def test_layouts_and_scales(store, new):
     g = torch.Generator(device=DEV).manual_seed(new)
     h, hk, d, r = 4, 2, 64, 32
@@ -137,7 +148,7 @@ def test_layouts_and_scales(store, new):
 
 
 @pytest.mark.parametrize("store", [None, I8, F8])
-@pytest.mark.parametrize("new", [2, 40])
+@pytest.mark.parametrize("new", [2, 40, 135])
 def test_magnitudes_beyond_fp16(store, new):
     """bf16 keys up to 3e5 against small queries, queries up to 3e5 against small keys, values from 1e-30 to 1e30."""
     g = torch.Generator(device=DEV).manual_seed(new)
@@ -169,7 +180,7 @@ def test_counts_out_of_range_are_clamped_and_no_rows_are_none():
     assert cache.attend(q[:, :, :0], emb).shape == (2, 2, 0, 64)
 
 
-@pytest.mark.parametrize("new", [3, 100])
+@pytest.mark.parametrize("new", [3, 40, 150])
 def test_a_page_outside_the_pool_is_reported_not_read(new):
     g = torch.Generator(device=DEV).manual_seed(2)
     for store in (None, I8):
@@ -188,7 +199,7 @@ def test_a_page_outside_the_pool_is_reported_not_read(new):
         assert torch.equal(cache.attend(q, emb), want) and _native.device_status() == 0
 
 
-@pytest.mark.parametrize("new,store", [(1, I8), (5, None), (90, None), (90, F8)])
+@pytest.mark.parametrize("new,store", [(1, I8), (5, None), (90, None), (90, F8), (140, None), (140, I8)])
 def test_captured_calls_follow_the_cache(new, store):
     """Append and attend in a graph: replays see the lengths and the rows of the moment."""
     g = torch.Generator(device=DEV).manual_seed(3)
@@ -229,7 +240,7 @@ def test_calls_in_a_row_and_on_another_stream_give_the_same():
     cache = make(3, 4, 128, BF, I8, 3000, 256)
     fill(cache, [2900, 1000, 300], g)
     emb = table(64, 4, 3000, g)
-    qs = [torch.randn(3, 8, n, 128, device=DEV, generator=g).bfloat16() for n in (1, 6, 64, 200)]
+    qs = [torch.randn(3, 8, n, 128, device=DEV, generator=g).bfloat16() for n in (1, 6, 64, 200)]   # every kernel, with parts to merge
     want = [cache.attend(q, emb).clone() for q in qs]
     torch.cuda.synchronize()
     for _ in range(20):
@@ -257,7 +268,7 @@ def test_a_pool_whose_offsets_pass_32_bits(store):
         fill(c, [900], torch.Generator(device=DEV).manual_seed(21))
     g = torch.Generator(device=DEV).manual_seed(22)
     emb = table(64, 8, 900, g)
-    for n in (1, 4, 300):
+    for n in (1, 4, 64, 300):
         q = torch.randn(1, 16, n, 128, device=DEV, generator=g).bfloat16()
         assert torch.equal(cache.attend(q, emb), small.attend(q, emb))
     assert all(torch.equal(a, b) for a, b in zip(cache.read(0), small.read(0)))
