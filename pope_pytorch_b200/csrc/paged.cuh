@@ -37,6 +37,29 @@ __device__ __forceinline__ int64_t paged_row(const PagedPtrs& p, int b, int hk, 
   return ((int64_t)pg * p.Hk + hk) * p.page_size + (pos - lp * p.page_size);
 }
 
+// ---- values of keys that a row does not see ----------------------------------------------------------
+// A probability of zero does not keep an infinity or a NaN of v out of a product.  In the steps whose keys some rows see and others do not,
+// such elements are taken out of the tile and given to the rows that see them apart from the products.
+template <typename T> __device__ __forceinline__ bool finite16(uint32_t w) {   // both halves
+  constexpr uint32_t m = TcFmt<T>::fmt == FMT_BF16 ? 0x7f80u : 0x7c00u;
+  return (w & m) != m && (w & m << 16) != m << 16;
+}
+template <typename T> __device__ __forceinline__ uint32_t drop_nonfinite16(uint32_t w) {
+  constexpr uint32_t m = TcFmt<T>::fmt == FMT_BF16 ? 0x7f80u : 0x7c00u;
+  return ((w & m) == m ? 0u : w & 0xffffu) | ((w & m << 16) == m << 16 ? 0u : w & 0xffff0000u);
+}
+// 16 bytes of a tile of v: zeros for a row behind the last key (which may hold anything), else without infinities and NaNs.  True where there were any.
+template <typename T> __device__ __forceinline__ bool clean_v(uint4* at, bool dead) {
+  if (dead) {
+    *at = make_uint4(0, 0, 0, 0);
+    return false;
+  }
+  const uint4 w = *at;
+  if (finite16<T>(w.x) && finite16<T>(w.y) && finite16<T>(w.z) && finite16<T>(w.w)) return false;
+  *at = make_uint4(drop_nonfinite16<T>(w.x), drop_nonfinite16<T>(w.y), drop_nonfinite16<T>(w.z), drop_nonfinite16<T>(w.w));
+  return true;
+}
+
 // ---- 8-bit codes -----------------------------------------------------------------------------------
 constexpr float ROW_LEAST = 1.5046327690525280e-36f;   // 2^-119: M / A of a smaller A would leave the range
 template <int STORE> constexpr float kCodeTop = STORE == POPE_STORE_INT8 ? 127.f : 448.f;

@@ -18,11 +18,12 @@ struct PagedOut {
   Strides so;
   float* lse;                // may be null
   float *part_o, *part_ml;   // [row block][split][128][D], [row block][split][128][max (log2 units), sum]
+  PagedPtrs c;               // the cache, for what clean_v() took out of its tiles
 };
 inline PagedOut paged_out(const PopePagedAttnArgs& a, int nsplit, float* part_o, float* part_ml) {
   PagedOut e;
   e.H = a.shape.H, e.Hk = a.shape.Hk, e.G = a.shape.H / a.shape.Hk, e.Nq = a.shape.Nq, e.nsplit = nsplit;
-  e.o = a.out, e.so = Strides(a.so), e.lse = a.lse, e.part_o = part_o, e.part_ml = part_ml;
+  e.o = a.out, e.so = Strides(a.so), e.lse = a.lse, e.part_o = part_o, e.part_ml = part_ml, e.c = paged_ptrs(a.cache, e.Hk, a.shape.d);
   return e;
 }
 inline bool rows_wide(const void* ptr, const PopeStride3& t) {   // rows on 16-byte boundaries
@@ -127,11 +128,34 @@ __device__ __forceinline__ void paged_expand_q(const PagedQ& p, uint32_t tmem_ro
   tmem_st_wait();
 }
 
+// The infinities and NaNs among the values [c0, c0 + D / 2) of the keys first .. last of a sequence are added to a row's results that this thread has
+// written, whole (out) or as a part.
+template <typename T, int STORE, int D>
+__device__ __forceinline__ void add_nonfinite(const PagedPtrs& c, int b, int hk, int first, int last, int c0, T* out, float* part) {
+#pragma unroll 1
+  for (int key = first; key <= last; ++key) {
+    const int64_t row = paged_row(c, b, hk, key);
+    if (row < 0) continue;
+    const float scale = STORE == POPE_STORE_16 ? 0.f : c.v_scales[row];   // (only a row whose scale is NaN has such values)
+    if (STORE != POPE_STORE_16 && isfinite(scale)) continue;
+    const T* v = reinterpret_cast<const T*>(c.v) + row * D + c0;
+#pragma unroll 1
+    for (int i = 0; i < D / 2; ++i) {
+      const float f = STORE == POPE_STORE_16 ? to_f32<T>(v[i]) : scale;
+      if (isfinite(f)) continue;
+      if (out) out[i] = from_f32<T>(to_f32<T>(out[i]) + f);
+      else part[i] += f;
+    }
+  }
+}
+
 // The softmax warps (threads 0 .. 255), all products of the CTA completed: row tid & 127, half tid >> 7 of its D columns from `tmem_o` on.  TWO: the halves
 // of a row's keys have accumulators of their own, 128 columns apart, and maxima of their own.  `l_half`: the row's sum over this thread's
-// keys, 0 for a row that is no query; m: its maximum.  xch: 512 floats of shared memory that nobody reads any more.
-template <typename T, int D, bool TWO>
-__device__ __forceinline__ void paged_epilogue(const PagedOut& e, uint32_t tmem_o, float* xch, int ub, int split, int b, int hk, int rb, float l_half, float m_half) {
+// keys, 0 for a row that is no query; m: its maximum.  xch: 512 floats of shared memory that nobody reads any more.  *dropped: whether clean_v() took
+// anything out of the tiles from key `first` on; last: the last key of the range that the row sees.
+template <typename T, int STORE, int D, bool TWO>
+__device__ __forceinline__ void paged_epilogue(const PagedOut& e, uint32_t tmem_o, float* xch, int ub, int split, int b, int hk, int rb, float l_half, float m_half,
+                                               const int* dropped, int first, int last) {
   const int tid = threadIdx.x, rloc = tid & 127, part = tid >> 7;
   auto all_sync = []() { asm volatile("bar.sync 5, %0;" ::"n"(32 * PAGED_SM_WARPS) : "memory"); };
   all_sync();   // (every thread is past its last look at xch)
@@ -140,6 +164,7 @@ __device__ __forceinline__ void paged_epilogue(const PagedOut& e, uint32_t tmem_
   const float m0 = xch[rloc], m1 = xch[PAGED_ROWS + rloc], m = fmaxf(m0, m1), mu = m == -CUDART_INF_F ? 0.f : m;
   const float f0 = TWO ? ex2_approx(m0 - mu) : 1.f, f1 = TWO ? ex2_approx(m1 - mu) : 1.f;   // 0 for a half without visible keys
   const float l = xch[2 * PAGED_ROWS + rloc] * f0 + xch[3 * PAGED_ROWS + rloc] * f1;
+  const bool any_dropped = *dropped != 0;
   fence_after_sync();
   const int rho = rb * PAGED_ROWS + rloc, tok = rho / e.G, head = hk + (rho - tok * e.G) * e.Hk;
   const bool whole = e.nsplit == 1, out_row = rho < e.Nq * e.G;   // (padding is written too)
@@ -172,6 +197,7 @@ __device__ __forceinline__ void paged_epilogue(const PagedOut& e, uint32_t tmem_
       for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(prow + c0 + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
     }
   }
+  if (any_dropped && out_row && l != 0.f) add_nonfinite<T, STORE, D>(e.c, b, hk, first, last, part * (D / 2), whole ? orow : nullptr, prow);
   if (part == 0 && out_row) {
     if (!whole) e.part_ml[(slot * PAGED_ROWS + rloc) * 2] = l != 0.f ? m : -CUDART_INF_F, e.part_ml[(slot * PAGED_ROWS + rloc) * 2 + 1] = l;
     else if (e.lse) e.lse[((int64_t)b * e.H + head) * e.Nq + tok] = l != 0.f ? m * LN2 + logf(l) : -CUDART_INF_F;

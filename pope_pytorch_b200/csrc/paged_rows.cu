@@ -495,10 +495,36 @@ __global__ void __launch_bounds__(32 * NW, 1)
     }
     // ---- O^T += V^T P^T ---------------------------------------------------------------------------------
     if constexpr (!Q8) {
-      if (key0 + 16 > ke) {   // rows behind the last key may hold anything, and 0 * NaN is NaN
-        const int dead = min(16, key0 + 16 - ke);
-        for (int i = lane; i < dead * KBLK * 8; i += 32)
-          *reinterpret_cast<uint4*>(vt + (i / 8 / dead) * hb * PR_BLOCK + (sub * 16 + 16 - dead + i / 8 % dead) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+      if (!clean) {
+        bool any = false;
+        auto group = [&](int i) { return reinterpret_cast<uint4*>(vt + (i >> 7) * hb * PR_BLOCK + (sub * 16 + (i >> 3 & 15)) * 128) + (i & 7); };
+        for (int i = lane; i < KBLK * 128; i += 32) {   // (looked at first: the values go to the rows before they go)
+          const uint4 x = *group(i);
+          any |= key0 + (i >> 3 & 15) < ke && !(finite16<T>(x.x) && finite16<T>(x.y) && finite16<T>(x.z) && finite16<T>(x.w));
+        }
+        if (__any_sync(0xffffffffu, any)) {
+#pragma unroll 1
+          for (int k = 0; k < min(16, ke - key0); ++k) {
+            const int vrow = sub * 16 + k;
+#pragma unroll
+            for (int m = 0; m < RQ; ++m)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float lo = __shfl_sync(0xffffffffu, sco[m][e], (k & 7) * 4 + t), hi = __shfl_sync(0xffffffffu, sco[m][2 + e], (k & 7) * 4 + t);
+                const bool seen = (k < 8 ? lo : hi) != -CUDART_INF_F;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                  for (int f = 0; f < 2; ++f) {   // feature 16 n + g + 8 f
+                    const int ch = 2 * n + f;
+                    const float x = to_f32<T>(*reinterpret_cast<const T*>(vt + (ch >> 3) * hb * PR_BLOCK + vrow * 128 + (((ch & 7) ^ (vrow & 7)) << 4) + g * 2));
+                    if (seen && !isfinite(x)) o[m][n][2 * f + e] += x;
+                  }
+              }
+          }
+          __syncwarp();
+        }
+        for (int i = lane; i < KBLK * 128; i += 32) clean_v<T>(group(i), key0 + (i >> 3 & 15) >= ke);
         __syncwarp();
       }
       const int row = sub * 16 + (lane & 7) + ((lane >> 4) << 3);

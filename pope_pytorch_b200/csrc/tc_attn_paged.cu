@@ -112,14 +112,15 @@ __global__ void __launch_bounds__(256, 6) paged_image_kernel(PagedImageP p) {
   const int tid = threadIdx.x, tile = blockIdx.x, u = blockIdx.y, b = u / p.c.Hk, hk = u % p.c.Hk, r = p.r;
   pdl_wait();
   pdl_trigger();
-  const int len = max(0, min(p.c.seq_lens[b], p.Nk)), key0 = tile * IMAGE_ROWS;
+  // (the page is read beside the length, not behind it)
+  const int key0 = tile * IMAGE_ROWS, lp = key0 / p.c.page_size, pg = lp < p.c.max_pages ? p.c.page_table[(int64_t)b * p.c.max_pages + lp] : -1;
+  const int len = max(0, min(p.c.seq_lens[b], p.Nk));
   if (key0 >= (len + 127) / 128 * 128) return;   // (tiles come in pairs)
   const int rows = max(0, min(IMAGE_ROWS, len - key0));
-  __shared__ int64_t row0_s;
-  if (tid == 0) row0_s = rows > 0 ? paged_row(p.c, b, hk, key0) : 0;
+  const bool there = pg >= 0 && pg < p.c.num_pages;   // a page outside the pool: reported, another one read
+  if (rows > 0 && !there && tid == 0) atomicOr(p.c.status, 2u);
+  const int64_t row0 = ((int64_t)(there ? pg : 0) * p.c.Hk + hk) * p.c.page_size + key0 % p.c.page_size;
   const int KC = DC + p.RP / 8;
-  __syncthreads();
-  const int64_t row0 = max(row0_s, (int64_t)0);   // (a page outside the pool: reported, another one read)
   const int c = tid % DC, first = tid / DC;
   const bool active = first < RPP, rotated = c * 8 < r;
   using Raw = std::conditional_t<Q8, uint2, uint4>;   // eight features
@@ -209,7 +210,7 @@ enum {
   PS_KFREE = 2,    // [2] S of the tile has completed
   PS_PVDONE = 4,   // [2] O += P V of the tile has completed: S / P buffer free
   PS_SFULL = 6,    // [2] the scores are in TMEM
-  PS_PFULL = 8,    // [2] the probabilities are in TMEM (and V's rows behind the last key are zero)
+  PS_PFULL = 8,    // [2] the probabilities are in TMEM (and V is fit for them, clean_v())
   PS_QFULL = 10,
   PS_ODONE = 11,
   PS_VFULL = 12,   // [2] V tile landed
@@ -217,10 +218,11 @@ enum {
   PS_COUNT = 16
 };
 
-template <typename T, int D, bool Q8>
+template <typename T, int STORE, int D>
 __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP p, const __grid_constant__ CUtensorMap tmap_v) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  constexpr bool Q8 = STORE != POPE_STORE_16;
   constexpr int VB = (D + 63) / 64, VBUF = VB * PS_KEYS * 128;   // V stage: [64-feature block][128 keys][128 B], swizzled
   constexpr int CSV = PS_KEYS * 16;
   const int KD = D + p.RP, KSTEPS = KD >> 4, KBUF = PS_KEYS * KD * 2;
@@ -230,6 +232,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP 
   float* bias_cs = xch + 4 * PS_ROWS;                             // [2][r]
   uint64_t* bars = reinterpret_cast<uint64_t*>(bias_cs + 2 * p.r);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + PS_COUNT);
+  int* dropped = reinterpret_cast<int*>(tmem_slot + 1);            // whether clean_v() took anything out
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   if (tid == 0) prefetch_tmap(&tmap_v);
@@ -240,6 +243,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP 
   if (tid == 0) {
     for (int i = 0; i < PS_COUNT; ++i) mbar_init(&bars[i], i == PS_PFULL || i == PS_PFULL + 1 || i == PS_QFULL ? PS_SM_WARPS : 1);
     mbar_init_fence();
+    *dropped = 0;
   }
   fence_before_sync();
   __syncthreads();
@@ -447,11 +451,12 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP 
 #pragma unroll
       for (int q = 0; q < 2; ++q) tmem_st16(s_addr + q * 16, pk[q]);
       tmem_st_wait();
-      if (!Q8 && key0 + PS_KEYS > kend) {   // rows behind the last key may hold anything, and 0 * NaN is NaN
+      if (!all_vis) {
         if (!failed) failed = !mbar_wait(&bars[PS_VFULL + buf], (j >> 1) & 1, WAIT_LIMIT);
-        const int dead = key0 + PS_KEYS - kend;
-        for (int i = tid; i < dead * VB * 8; i += 32 * PS_SM_WARPS)
-          *reinterpret_cast<uint4*>(Vs + buf * VBUF + (i / 8 / dead) * (PS_KEYS * 128) + (PS_KEYS - dead + i / 8 % dead) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+        bool any = false;
+        for (int i = tid; i < VBUF / 16; i += 32 * PS_SM_WARPS)
+          any |= clean_v<T>(reinterpret_cast<uint4*>(Vs + buf * VBUF) + i, key0 + (i >> 3 & (PS_KEYS - 1)) >= kend);
+        if (any) *dropped = 1;
         fence_async_smem();
       }
       fence_before_sync();
@@ -460,7 +465,8 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP 
     }
 
     if (T_tiles > 0 && !failed) failed = !mbar_wait(&bars[PS_ODONE], 0, WAIT_LIMIT);
-    paged_epilogue<T, D, false>(p.e, tmem + PS_TO, xch, ub, split, b, hk, rb, live ? l_run : 0.f, m_run);
+    paged_epilogue<T, STORE, D, false>(p.e, tmem + PS_TO, xch, ub, split, b, hk, rb, live ? l_run : 0.f, m_run, dropped,
+                                       max(t0, max(0, min(kend, first_pos + 1)) / PS_KEYS) * PS_KEYS, min(limit, (t0 + T_tiles) * PS_KEYS - 1));
   }
   if (failed) atomicOr(p.status, 1u);
   fence_before_sync();
@@ -537,12 +543,12 @@ template <typename T, int STORE, int D> static cudaError_t paged_sweep_t(const P
   const int KD = s.d + RP;
   // (every CTA allocates all 512 TMEM columns: two must not share an SM)
   const size_t smem = std::max<size_t>(2 * (size_t)PS_KEYS * KD * 2 + 2 * (size_t)((s.d + 63) / 64) * PS_KEYS * 128 + 4 * PS_ROWS * 4 + 2 * (size_t)s.r * 4 + PS_COUNT * 8 + 16 + 1024, 120 * 1024);
-  cudaError_t e = ensure_max_smem<paged_sweep_kernel<T, D, Q8>>();
+  cudaError_t e = ensure_max_smem<paged_sweep_kernel<T, STORE, D>>();
   if (e != cudaSuccess) return e;
   if (s.r > 0 && (e = launch_paged_tables(a.embed, s.Nk, s.r, tt.ch, tt.sh, nullptr, 0, st)) != cudaSuccess) return e;
   const size_t ismem = (size_t)(KD / 8) * CS64;
   if ((e = launch_dependent(paged_image_kernel<T, STORE, D>, dim3((unsigned)((s.Nk + 127) / 128 * 2), (unsigned)(s.B * s.Hk)), dim3(256), ismem, st, im)) != cudaSuccess) return e;
-  e = launch_dependent(paged_sweep_kernel<T, D, Q8>, dim3((unsigned)(s.B * s.Hk * p.blocks * p.nsplit)), dim3(PS_THREADS), smem, st, p, tmap_v);
+  e = launch_dependent(paged_sweep_kernel<T, STORE, D>, dim3((unsigned)(s.B * s.Hk * p.blocks * p.nsplit)), dim3(PS_THREADS), smem, st, p, tmap_v);
   return e != cudaSuccess || p.nsplit == 1 ? e : launch_paged_merge(p.e, s.dtype, s.d, s.B * s.Hk * p.blocks, p.blocks, st);
 }
 template <typename T, int STORE> static cudaError_t paged_sweep_d(const PopePagedAttnArgs& a, cudaStream_t st) {

@@ -74,6 +74,7 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
   float* bias_cs = xch + 4 * PAGED_ROWS;                           // [2][r]
   uint64_t* bars = reinterpret_cast<uint64_t*>(bias_cs + 2 * r);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + SK_COUNT);
+  int* dropped = reinterpret_cast<int*>(tmem_slot + 1);             // whether clean_v() took anything out
 
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   if (warp == SK_KLOAD && lane == 0) prefetch_tmap(&tmap_k), prefetch_tmap(&tmap_t), prefetch_tmap(&tmap_ks);
@@ -88,6 +89,7 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
       mbar_init(&bars[i], ex ? SK_EX_WARPS : sm ? PAGED_SM_WARPS : 1);
     }
     mbar_init_fence();
+    *dropped = 0;
   }
   pdl_wait();
   pdl_trigger();
@@ -286,8 +288,8 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
       const int buf = j & 1, key0 = (t0 + j) * SK_KEYS, n0 = key0 + part * 32;   // first key of this thread's columns
       if (!failed) failed = !mbar_wait(&bars[SK_SFULL + buf], (j >> 1) & 1, WAIT_LIMIT);
       fence_after_sync();
+      const bool all_vis = key0 + SK_KEYS <= min(kend, first_pos + 1);   // (rows that are no queries are dropped at the end)
       if (warp_live) {
-        const bool all_vis = key0 + SK_KEYS <= min(kend, first_pos + 1);   // (rows that are no queries are dropped at the end)
         const int lim = limit - n0;
         const uint32_t vis = lim >= 31 ? ~0u : (lim < 0 ? 0u : ((2u << lim) - 1u));
         const uint32_t s_addr = tmem + lane_base + SK_TS + buf * SK_KEYS + part * 32;
@@ -351,11 +353,13 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
         tmem_st16(s_addr, pk);
         tmem_st_wait();
       }
-      if (!Q8 && key0 + SK_KEYS > kend) {   // rows of V behind the last key may hold anything, and 0 * NaN is NaN (the last step)
-        if (!failed) failed = !mbar_wait(&bars[SK_VFULL + j % p.vstages], (j / p.vstages) & 1, WAIT_LIMIT);
-        const int dead = key0 + SK_KEYS - kend;
-        for (int i = tid; i < dead * KBLK * 8; i += 32 * PAGED_SM_WARPS)
-          *reinterpret_cast<uint4*>(vring + j % p.vstages * vstage + (i / 8 / dead) * SK_BLOCK + (SK_KEYS - dead + i / 8 % dead) * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+      if (!all_vis) {   // (the same for all threads of these warps)
+        uint4* vt = reinterpret_cast<uint4*>(Q8 ? Vs + buf * DC * SK_CS : vring + j % p.vstages * vstage);
+        if (!Q8 && !failed) failed = !mbar_wait(&bars[SK_VFULL + j % p.vstages], (j / p.vstages) & 1, WAIT_LIMIT);
+        bool any = false;
+        for (int i = tid; i < (Q8 ? DC * SK_CS : KBLK * SK_BLOCK) / 16; i += 32 * PAGED_SM_WARPS)
+          any |= clean_v<T>(vt + i, key0 + (Q8 ? i & (SK_KEYS - 1) : i >> 3 & (SK_KEYS - 1)) >= kend);
+        if (any) *dropped = 1;
         fence_async_smem();
       }
       fence_before_sync();
@@ -363,7 +367,8 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
       if (lane == 0) mbar_arrive(&bars[SK_PFULL + buf]);
     }
     if (T_tiles > 0 && !failed) failed = !mbar_wait(&bars[SK_ODONE], 0, WAIT_LIMIT);
-    paged_epilogue<T, D, true>(p.e, tmem + SK_TO, xch, ub, split, b, hk, rb, live ? l_run : 0.f, m_run);
+    paged_epilogue<T, STORE, D, true>(p.e, tmem + SK_TO, xch, ub, split, b, hk, rb, live ? l_run : 0.f, m_run, dropped,
+                                      max(t0, max(0, min(kend, first_pos + 1)) / SK_KEYS) * SK_KEYS, min(limit, (t0 + T_tiles) * SK_KEYS - 1));
   }
   if (failed) atomicOr(p.status, 1u);
   fence_before_sync();

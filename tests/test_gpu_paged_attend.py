@@ -127,6 +127,40 @@ def test_what_is_not_a_key_never_counts(store):
     assert torch.equal(cache.attend(q, emb), clean.attend(q, emb))
 
 
+@pytest.mark.parametrize("store", [None, I8, F8])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("new", [3, 30, 200])
+def test_later_tokens_do_not_reach_earlier_rows(store, dtype, new):
+    """Infinities and NaN in k and v of a token: the rows before it are untouched, to the bit; it and the rows behind it are not finite."""
+    g = torch.Generator(device=DEV).manual_seed(new)
+    h, hk, d, r, n = 4, 2, 128, 64, 333
+    k, v = (torch.randn(1, hk, n, d, device=DEV, generator=g).to(dtype) for _ in range(2))
+    q = torch.randn(1, h, new, d, device=DEV, generator=g).to(dtype)
+    emb = table(r, hk, n, g)
+
+    def run(k, v):
+        cache = make(1, hk, d, dtype, store, n, seed=1)
+        cache.append(k, v)
+        return cache.attend(q, emb)
+
+    want = run(k, v)
+    bad = n - 1 - new // 3          # seen by the last rows alone
+    first = new - 1 - new // 3
+    for what, value in (("k", math.nan), ("v", math.nan), ("v", math.inf), ("v", -math.inf)):
+        kk, vv = k.clone(), v.clone()
+        (kk if what == "k" else vv)[:, 1, bad, 5 if what == "v" else slice(None)] = value
+        got = run(kk, vv)
+        assert torch.equal(got[:, :, :first], want[:, :, :first])
+        assert torch.equal(got[:, 0::2], want[:, 0::2])                 # the other key head's
+        hit = got[:, 1::2, first:]
+        if store is not None or what == "k":                            # an 8-bit row with such a value is NaN as a whole
+            assert hit.isnan().all()
+        else:
+            assert (hit[..., 5].isnan().all() if math.isnan(value) else (hit[..., 5] == value).all())
+            rest = torch.arange(d, device=DEV) != 5
+            assert torch.equal(hit[..., rest], want[:, 1::2, first:][..., rest])
+
+
 @pytest.mark.parametrize("store", [None, I8])
 @pytest.mark.parametrize("new", [4, 40, 150])
 def test_layouts_and_scales(store, new):
