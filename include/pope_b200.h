@@ -333,7 +333,7 @@ typedef struct PopeKvReadArgs {
 /* Attention of the newest tokens of every sequence over everything the cache holds for it.  Row i < counts[b] of q (B, H, Nq, d)
  * is the query of position seq_lens[b] - counts[b] + i and sees the keys up to that position; counts (device, may be NULL = Nq
  * everywhere) is clamped to [0, Nq].  Rows behind the count, and rows whose position is negative, give out = 0, lse = -inf.
- * shape.Nk = an upper bound of every seq_lens[b], as for PopePagedDecodeArgs; shape.Nq may exceed it.  dtype is that of q and
+ * shape.Nk = an upper bound of every seq_lens[b], as for PopePagedDecodeArgs, at most 2^24; shape.Nq may exceed it.  dtype is that of q and
  * out and, with POPE_STORE_16, of the pages.  lse (B, H, Nq) fp32 may be NULL.  Workspace: pope_b200_workspace_bytes(
  * POPE_OP_ATTN_PAGED, &args). */
 typedef struct PopePagedAttnArgs {

@@ -33,8 +33,9 @@
 namespace pope {
 
 struct PagedRowsP {
-  int H, Hk, G, Nq, Nk, r, nsplit, stages, blocks, hb;   // G: query heads per key head; stages: of one tile ring; blocks: row blocks per
-  int page_size, max_pages, num_pages, npg_smem;         // (sequence, key head); hb: key heads that a CTA takes
+  int H, Hk, G, Nq, Nk, r, nsplit, blocks, hb;           // G: query heads per key head; blocks: row blocks per (sequence, key head); hb: key heads
+  int rings, stages;                                     // that a CTA takes; rings: tiles in work at a time, each with a ring of stages
+  int page_size, max_pages, num_pages, npg_smem;
   float scale_log2;
   const int32_t *page_table, *seq_lens, *counts;
   const float *freqs, *bias;
@@ -49,7 +50,7 @@ struct PagedRowsP {
 
 constexpr int PR_TILE = 32;              // keys of a tile
 constexpr int PR_WPT = PR_TILE / 16;     // warps that share a tile of one key head
-constexpr int PR_MAX_SPLIT = 64;
+constexpr int PR_MAX_SPLIT = 64, PR_MAX_PAGES = 4096;
 constexpr int PR_BLOCK = PR_TILE * 128;  // bytes of 128-byte rows of a tile
 
 template <typename TM> __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(32 * NW, 1)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int r = p.r, tblk = (r + 63) / 64, RP = (r + FPI - 1) / FPI * FPI, hb = p.hb;
-  const int rings = NW / (PR_WPT * hb);                                // tiles in work at a time, a ring of stages for each
+  const int rings = p.rings;   // at most NW / (PR_WPT * hb): where shared memory holds fewer tiles some warps have none
   const int v_at = hb * KBLK * PR_BLOCK, trig_at = 2 * v_at, scale_at = trig_at + 2 * tblk * PR_BLOCK;
   const int stage_bytes = scale_at + (Q8 ? 1024 : 0);   // [K block][head], [V block][head], [trig block][cos, sin], [k, v][head] scales
   const int pitch = (DP + RP) * 2 + ((DP + RP) % 64 == 0 ? 64 : 0);   // an odd multiple of 64 bytes: eight rows x 64 bytes on distinct banks
@@ -296,7 +297,7 @@ __global__ void __launch_bounds__(32 * NW, 1)
   bool failed = false;
   int s = 0;
   uint32_t par = 0;
-  for (int jt = rg; jt < T_tiles; jt += rings) {
+  for (int jt = rg; rg < rings && jt < T_tiles; jt += rings) {
     const int key0 = kb + jt * PR_TILE + sub * 16;   // first key of this warp
     const int at = rg * p.stages + s;
     uint8_t* st = smem + (size_t)at * stage_bytes;
@@ -725,20 +726,23 @@ static int rows_blocks(const PopeShape& s) {
 }
 // warps of a CTA: as many as the registers of their outputs (32 per group of eight rows) allow
 constexpr int rows_nw(int rq) { return rq == 2 ? 12 : 16; }
-// Key heads of a CTA: they share the copies of the cosines and sines, which at 8 bits are as many bytes as K and V or twice that.
+// Key heads of a CTA: they share the copies of the cosines and sines, which at 8 bits are as many bytes as K and V or twice that, and the larger boxes
+// need fewer copies.  At 16 bits two for up to 8 rows ((8, 32 / 8, 16384, 128): r = 64 118 us against 133, r = 128 148 / 179), but one for 16
+// rows, where the second head's outputs cost more at the end of short ranges (2000 keys 35 / 30 us) than it saves on long ones (152 / 165).
 static int rows_hb(const PopeShape& s, int store) {
   const int pairs = rows_nw(rows_rq(s)) / PR_WPT;
-  if (store == POPE_STORE_16) return 1;
-  return s.Hk % 4 == 0 && pairs % 4 == 0 ? 4 : s.Hk % 2 == 0 && pairs % 2 == 0 ? 2 : 1;
+  const int most = store != POPE_STORE_16 ? 4 : rows_rq(s) == 1 ? 2 : 1;
+  return most >= 4 && s.Hk % 4 == 0 && pairs % 4 == 0 ? 4 : most >= 2 && s.Hk % 2 == 0 ? 2 : 1;
 }
 
 // Key ranges per unit: whole waves of one CTA per SM times a CTA's tiles plus what it costs beside them.
-static int rows_split(const PopeShape& s, int store) {
+static int rows_split(const PopeShape& s, int store, int page_size) {
   const int tiles = (s.Nk + PR_TILE - 1) / PR_TILE;
+  const int least = std::max(1, (int)(((int64_t)s.Nk / page_size + PR_MAX_PAGES - 1) / PR_MAX_PAGES));   // (a CTA keeps the pages of its range)
   const int64_t units = (int64_t)s.B * s.Hk / rows_hb(s, store) * rows_blocks(s);
-  int best = 1;
+  int best = least;
   int64_t best_cost = INT64_MAX;
-  for (int n = 1; n <= std::min(tiles, PR_MAX_SPLIT); ++n) {
+  for (int n = least; n <= std::min(tiles, PR_MAX_SPLIT); ++n) {
     const int64_t cost = (units * n + 147) / 148 * ((tiles + n - 1) / n + 8);
     if (cost < best_cost) best = n, best_cost = cost;
   }
@@ -749,9 +753,9 @@ static int rows_split(const PopeShape& s, int store) {
 struct RowsWs {
   size_t part_o, part_ml, table, total;
 };
-static RowsWs rows_ws(const PopeShape& s, int store) {
+static RowsWs rows_ws(const PopeShape& s, int store, int page_size) {
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
-  const size_t units = (size_t)s.B * s.Hk * rows_blocks(s), slots = units * rows_split(s, store) * 8 * rows_rq(s);
+  const size_t units = (size_t)s.B * s.Hk * rows_blocks(s), slots = units * rows_split(s, store, page_size) * 8 * rows_rq(s);
   RowsWs w;
   w.part_o = up(units * sizeof(unsigned int));
   w.part_ml = w.part_o + up(slots * s.d * sizeof(float));
@@ -759,19 +763,19 @@ static RowsWs rows_ws(const PopeShape& s, int store) {
   w.total = w.table + up((size_t)s.Nk * s.r * 4);
   return w;
 }
-size_t paged_rows_workspace(const PopePagedAttnArgs& a) { return rows_ws(a.shape, a.cache.store).total; }
+size_t paged_rows_workspace(const PopePagedAttnArgs& a) { return rows_ws(a.shape, a.cache.store, a.cache.kv.page_size).total; }
 
 template <typename T, int STORE, int D, int RQ> static cudaError_t paged_rows_t(const PopePagedAttnArgs& a, cudaStream_t st) {
   constexpr bool Q8 = STORE != POPE_STORE_16;
   constexpr int NW = rows_nw(RQ), RB = 8 * RQ, FPI = Q8 ? 64 : 32, DP = (D + FPI - 1) / FPI * FPI, KBLK = (D * (Q8 ? 1 : 2) + 127) / 128;
   const PopeShape& s = a.shape;
   const PopePagedKV& kv = a.cache.kv;
-  const RowsWs ws = rows_ws(s, STORE);
+  const RowsWs ws = rows_ws(s, STORE, kv.page_size);
   uint8_t* base = static_cast<uint8_t*>(a.workspace);
   __half* table = reinterpret_cast<__half*>(base + ws.table);
   PagedRowsP p = {};
   p.H = s.H, p.Hk = s.Hk, p.G = s.H / s.Hk, p.Nq = s.Nq, p.Nk = s.Nk, p.r = s.r;
-  p.nsplit = rows_split(s, STORE), p.blocks = rows_blocks(s), p.hb = rows_hb(s, STORE);
+  p.nsplit = rows_split(s, STORE, kv.page_size), p.blocks = rows_blocks(s), p.hb = rows_hb(s, STORE);
   p.page_size = kv.page_size, p.max_pages = kv.max_pages_per_seq, p.num_pages = kv.num_pages;
   const int tiles = (s.Nk + PR_TILE - 1) / PR_TILE;
   p.npg_smem = (int)((int64_t)((tiles + p.nsplit - 1) / p.nsplit) * PR_TILE / kv.page_size) + 2;
@@ -795,14 +799,15 @@ template <typename T, int STORE, int D, int RQ> static cudaError_t paged_rows_t(
                  : (mks = mvs = mk, true));
   if (!ok) return cudaErrorNotSupported;
 
-  const int tblk = (s.r + 63) / 64, RP = (s.r + FPI - 1) / FPI * FPI, rings = NW / (PR_WPT * p.hb);
+  const int tblk = (s.r + 63) / 64, RP = (s.r + FPI - 1) / FPI * FPI, most = NW / (PR_WPT * p.hb);
   const size_t stage = (size_t)(p.hb * 2 * KBLK + 2 * tblk) * PR_BLOCK + (Q8 ? 1024 : 0), red = (size_t)NW * RB * D * 4;
   const size_t pitch = (DP + RP) * 2 + ((DP + RP) % 64 == 0 ? 64 : 0);
-  const size_t fixed = 1024 + p.hb * RB * pitch + (size_t)NW * RB * 8 + p.hb * RB * 4 + RB * 4 + p.hb * 2 * (size_t)s.r * 4 + rings * 4 * 12 + 16 +
+  const size_t fixed = 1024 + p.hb * RB * pitch + (size_t)NW * RB * 8 + p.hb * RB * 4 + RB * 4 + p.hb * 2 * (size_t)s.r * 4 + most * 4 * 12 + 16 +
                        (size_t)p.npg_smem * 4;
-  p.stages = (int)std::min<size_t>(4, (kMaxDynamicSmem - fixed) / (stage * rings));
-  if (fixed > (size_t)kMaxDynamicSmem || p.stages < 1) return cudaErrorInvalidValue;
-  const size_t smem = fixed + std::max(rings * p.stages * stage, red);
+  if (fixed + stage > (size_t)kMaxDynamicSmem) return cudaErrorInvalidValue;
+  const int tiles_smem = (int)((kMaxDynamicSmem - fixed) / stage);
+  p.rings = std::min(most, tiles_smem), p.stages = std::min(4, tiles_smem / p.rings);
+  const size_t smem = fixed + std::max(p.rings * p.stages * stage, red);
   if (smem > (size_t)kMaxDynamicSmem) return cudaErrorInvalidValue;
   const auto kernel = paged_rows_kernel<T, STORE, D, RQ, NW>;
   cudaError_t e;

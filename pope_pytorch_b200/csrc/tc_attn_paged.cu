@@ -572,7 +572,7 @@ bool attn_paged_supported(const PopePagedAttnArgs& a) {
   if (s.dtype != POPE_BF16 && s.dtype != POPE_F16) return false;
   if (s.d != 64 && s.d != 96 && s.d != 128) return false;
   if (s.r % 8 != 0 || (s.r > 0 && (a.embed.sf.b != 0 || a.embed.sf.h != 0))) return false;
-  return a.cache.kv.page_size % 64 == 0;
+  return a.cache.kv.page_size >= 64 && a.cache.kv.page_size % 64 == 0 && s.Nk <= 1 << 24;
 }
 
 // By the rows that share a key head.  Up to 16 the keys become product fragments in registers ((8, 32 / 8, 2000, 128), r = 64, us: 16-bit cache 8 rows 23

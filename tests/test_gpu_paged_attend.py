@@ -199,7 +199,7 @@ def test_magnitudes_beyond_fp16(store, new):
         qq = (q * dq).bfloat16()
         vals = held(cache)
         ref = R.attend(qq, [x[0] for x in vals], [x[1] for x in vals], emb[0], emb[1], [n], [new], 0.125, store)
-        got = cache.attend(qq, emb).double().cpu() / dv
+        got = cache.attend(qq, emb).double() / dv
         R.check(got, ref[0] / dv, ref[2] / dv, ref[3] / dv)
 
 
@@ -306,6 +306,51 @@ def test_a_pool_whose_offsets_pass_32_bits(store):
         q = torch.randn(1, 16, n, 128, device=DEV, generator=g).bfloat16()
         assert torch.equal(cache.attend(q, emb), small.attend(q, emb))
     assert all(torch.equal(a, b) for a, b in zip(cache.read(0), small.read(0)))
+
+
+@pytest.mark.parametrize("d", [64, 96, 128])
+@pytest.mark.parametrize("store", [None, I8, F8])
+def test_every_width_of_rotation_and_number_of_heads(d, store):
+    """Every r, with numbers of key heads and rows that give every split of work over warps, CTAs and kernels: each has to fit the SM."""
+    g = torch.Generator(device=DEV).manual_seed(d)
+    for at, r in enumerate(range(0, d + 1, 8)):
+        dtype = (BF, HF)[at % 2]
+        for hk, h, new in ((1, 1, 1), (2, 2, 8), (4, 16, 1), (3, 3, 11), (4, 8, 8), (2, 4, 19), (1, 2, 131)):
+            lens = [70, 131 + new]
+            cache = make(2, hk, d, dtype, store, 280, 64, seed=r)
+            fill(cache, lens, g)
+            q = torch.randn(2, h, new, d, device=DEV, generator=g).to(dtype)
+            emb = table(r, hk, 280, g)
+            vals = held(cache)
+            want = R.attend(q, [x[0] for x in vals], [x[1] for x in vals], emb[0], emb[1], lens, [new] * 2, d ** -0.5, store)
+            R.check(cache.attend(q, emb), want[0], want[2], want[3])
+    assert _native.device_status() == 0
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_drawn_shapes(seed):
+    """Sizes of all kinds: long and ragged caches, chunks from one token to hundreds, every kernel and every cut along the keys."""
+    import random
+    rng = random.Random(seed)
+    d = rng.choice([64, 96, 128])
+    r = rng.choice([d, d // 2, d // 4 // 8 * 8])
+    hk = rng.choice([1, 2, 3, 4, 8])
+    h = hk * rng.choice([1, 2, 4, 5])
+    b, dtype, store, page = rng.choice([1, 2, 5]), rng.choice([BF, HF]), rng.choice([None, I8, F8]), rng.choice([64, 128, 192, 256])
+    lens = [round(math.exp(rng.uniform(0, math.log(9000)))) for _ in range(b)]
+    new = min(max(lens), rng.choice([1, 2, 3, 7, 16, 33, 64, 100, 257]))
+    counts = [rng.randint(0, new) for _ in lens] if rng.random() < 0.5 else None
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    cache = make(b, hk, d, dtype, store, max(lens) + 5, page, seed)
+    fill(cache, lens, g)
+    q = torch.randn(b, h, new, d, device=DEV, generator=g).to(dtype)
+    emb = table(r, hk, max(lens), g)
+    given = None if counts is None else torch.tensor(counts, dtype=torch.int32, device=DEV)
+    out, lse = cache.attend(q, emb, counts=given, return_lse=True)
+    vals = held(cache)
+    want = R.attend(q, [x[0] for x in vals], [x[1] for x in vals], emb[0], emb[1], lens, counts or [new] * b, d ** -0.5, store)
+    R.check(out, want[0], want[2], want[3], lse, want[1])
+    assert _native.device_status() == 0
 
 
 def test_against_the_attention_over_contiguous_keys():
