@@ -45,6 +45,11 @@ int dtype_of(const Tensor& t) {
 // (batch, head, row) strides of a (b, h, n, x) tensor or, with seq_first, of a (b, n, h, x) one; the innermost stride is 1
 PopeStride3 s3(const Tensor& t, bool seq_first = false) { return {t.stride(0), t.stride(seq_first ? 2 : 1), t.stride(seq_first ? 1 : 2)}; }
 
+// the same for calls that look at the alignment of rows: an axis of one element has no stride that counts (a transposed vector has 1 there)
+PopeStride3 s3_used(const Tensor& t) {
+  return {t.size(0) > 1 ? t.stride(0) : 0, t.size(1) > 1 ? t.stride(1) : 0, t.size(2) > 1 ? t.stride(2) : 0};
+}
+
 Tensor inner_contig(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 
 Tensor fp32_rows(const Tensor& t) { return inner_contig(t.scalar_type() == at::kFloat ? t : t.to(at::kFloat)); }
@@ -512,8 +517,9 @@ void kv_append(const Pages& p, const Tensor& k_, const Tensor& v_, int64_t row) 
   const auto fill = [&](auto& a) {
     a.struct_bytes = sizeof(a), a.dtype = dtype_of(k), a.B = one ? 1 : (int32_t)k.size(0), a.Hk = (int32_t)k.size(h), a.d = (int32_t)k.size(h + 2);
     a.n_new = (int32_t)k.size(h + 1), a.advance = 1;
-    a.k = k.const_data_ptr(), a.sk = {one ? 0 : k.stride(0), k.stride(h), k.stride(h + 1)};
-    a.v = v.const_data_ptr(), a.sv = {one ? 0 : v.stride(0), v.stride(h), v.stride(h + 1)};
+    const auto stride = [](const Tensor& t, int64_t axis) { return t.size(axis) > 1 ? t.stride(axis) : 0; };   // (as s3_used())
+    a.k = k.const_data_ptr(), a.sk = {one ? 0 : stride(k, 0), stride(k, h), stride(k, h + 1)};
+    a.v = v.const_data_ptr(), a.sv = {one ? 0 : stride(v, 0), stride(v, h), stride(v, h + 1)};
   };
   if (p.store() != POPE_STORE_16) {
     PopeKvWriteArgs a = {};
@@ -579,7 +585,7 @@ std::tuple<Tensor, optional<Tensor>> kv_attend(const Pages& p, const Tensor& q_,
   a.shape = {(int32_t)q.size(0), (int32_t)q.size(1), (int32_t)p.k.size(1), (int32_t)q.size(2), (int32_t)nk, (int32_t)q.size(3), r, dtype_of(q)};
   a.embed = embed_of(freqs, bias, r), a.cache = p.held();
   if (counts) a.counts = counts->const_data_ptr<int32_t>();
-  a.q = q.const_data_ptr(), a.sq = s3(q), a.out = out.mutable_data_ptr(), a.so = s3(out);
+  a.q = q.const_data_ptr(), a.sq = s3_used(q), a.out = out.mutable_data_ptr(), a.so = s3_used(out);
   if (lse) a.lse = lse->mutable_data_ptr<float>();
   const Tensor ws = workspace(POPE_OP_ATTN_PAGED, a, q);
   check(pope_b200_attn_paged(&a, stream_of(q)), "pope_b200_attn_paged");

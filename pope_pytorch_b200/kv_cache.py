@@ -231,6 +231,8 @@ class PagedKVCache:
         if self.store is None:
             out, lse = N._ops().kv_decode(self._pages(), q, freqs, bias, scale, nk)
         else:
+            if r % 8 != 0 or r > self.head_dim:
+                raise ValueError("over 8 bits the rotated features must be a multiple of 8, up to head_dim")
             out, lse = N._ops().kv_attend(self._pages(), q, freqs, bias, None, scale, nk, return_lse)
             lse = lse[..., 0] if return_lse else None
         return (out, lse) if return_lse else out
@@ -241,8 +243,8 @@ class PagedKVCache:
         row i stands at position ``len - n + i`` and sees the keys up to its own.  ``counts``, an int32 tensor (batch,) on the
         cache's device, gives sequences fewer new tokens than n: row i < counts[b] then stands at ``len - counts[b] + i`` and the
         rows behind are padding (counts outside [0, n] are clamped).  Padding, and rows at negative positions, give zeros (lse -inf).
-        pos_emb: (freqs, bias) with at least ``max_len`` rows of freqs.  Returns out (batch, heads, n, head_dim) in q's dtype and
-        layout (and lse (batch, heads, n) on request)."""
+        pos_emb: (freqs, bias) with at least ``max_len`` rows of freqs, the rotated features a multiple of 8.  Returns out
+        (batch, heads, n, head_dim) in q's dtype and layout (and lse (batch, heads, n) on request)."""
         freqs, bias = pos_emb
         if q.ndim != 4 or q.shape[0] != self.batch or q.shape[3] != self.head_dim or q.shape[1] == 0 or q.shape[1] % self.kv_heads != 0:
             raise ValueError("q must be (batch, heads, n, head_dim) with heads a multiple of kv_heads")
@@ -251,6 +253,8 @@ class PagedKVCache:
         r, nk = freqs.shape[-1], max(self.max_len, 1)
         if freqs.ndim != 2:
             raise ValueError("the paged attention takes a (positions, rotate_dim) table")
+        if r % 8 != 0 or r > self.head_dim:
+            raise ValueError("the rotated features must be a multiple of 8, up to head_dim")
         if r > 0 and freqs.shape[0] < nk:
             raise ValueError("freqs must cover every cached position")
         if counts is not None:

@@ -308,6 +308,60 @@ def test_a_pool_whose_offsets_pass_32_bits(store):
     assert all(torch.equal(a, b) for a, b in zip(cache.read(0), small.read(0)))
 
 
+@pytest.mark.parametrize("store", [None, I8])
+def test_transposed_vectors(store):
+    """One token whose features were the last axis but one: the strides of axes of one element say nothing."""
+    g = torch.Generator(device=DEV).manual_seed(4)
+    cache, other = make(1, 2, 64, BF, store, 100), make(1, 2, 64, BF, store, 100)
+    col = lambda h: torch.randn(1, h, 64, 1, device=DEV, generator=g).bfloat16().transpose(2, 3)
+    for _ in range(3):
+        k, v = col(2), col(2)
+        assert k.stride(2) == 1
+        cache.append(k, v)
+        other.append_to(0, k[0].clone(memory_format=torch.contiguous_format), v[0].clone(memory_format=torch.contiguous_format))
+    for a, b in zip(cache.gather(0), other.gather(0)):
+        assert torch.equal(a, b)
+    emb, q = table(32, 2, 100, g), col(4)
+    want = other.attend(q.clone(memory_format=torch.contiguous_format), emb)
+    assert torch.equal(cache.attend(q, emb), want)
+    vals = held(cache)
+    ref = R.attend(q, [x[0] for x in vals], [x[1] for x in vals], emb[0], emb[1], [3], [1], 0.125, store)
+    R.check(want, ref[0], ref[2], ref[3])
+
+
+@pytest.mark.parametrize("store", [None, F8])
+def test_refusals(store):
+    g = torch.Generator(device=DEV).manual_seed(2)
+    cache = make(2, 2, 64, BF, store, 100)
+    fill(cache, [40, 60], g)
+    q = torch.randn(2, 4, 3, 64, device=DEV, generator=g).bfloat16()
+    freqs, bias = table(32, 2, 100, g)
+    before = [cache.lens, cache.page_table.clone(), cache.seq_lens.clone()]
+    for err, qq, emb, more in (
+            (TypeError, q.half(), (freqs, bias), {}),
+            (TypeError, q.cpu(), (freqs, bias), {}),
+            (ValueError, q[:, :3], (freqs, bias), {}),
+            (ValueError, q[:1], (freqs, bias), {}),
+            (ValueError, q, (freqs[None], bias), {}),
+            (ValueError, q, (freqs[:59], bias), {}),
+            (ValueError, q, (freqs, bias[:1]), {}),
+            (ValueError, q, (freqs[:, :12], bias), {}),          # not a multiple of eight
+            (ValueError, q, (torch.cat([freqs] * 3, -1), bias), {}),
+            ((TypeError, ValueError, RuntimeError), q, (freqs.cpu(), bias), {}),
+            ((TypeError, ValueError, RuntimeError), q, (freqs, bias.cpu()), {}),
+            (TypeError, q, (freqs, bias), dict(counts=torch.zeros(2, dtype=torch.int64, device=DEV))),
+            (TypeError, q, (freqs, bias), dict(counts=torch.zeros(2, dtype=torch.int32))),
+            (ValueError, q, (freqs, bias), dict(counts=torch.zeros(3, dtype=torch.int32, device=DEV)))):
+        with pytest.raises(err):
+            cache.attend(qq, emb, **more)
+    with pytest.raises(TypeError):
+        cache.append(q[:, :2], q[:, :2].float())
+    with pytest.raises(IndexError):
+        cache.read(0, 0, 41)
+    assert cache.lens == before[0] and torch.equal(cache.page_table, before[1]) and torch.equal(cache.seq_lens, before[2])
+    assert _native.device_status() == 0
+
+
 @pytest.mark.parametrize("d", [64, 96, 128])
 @pytest.mark.parametrize("store", [None, I8, F8])
 def test_every_width_of_rotation_and_number_of_heads(d, store):
