@@ -85,7 +85,7 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // the address of *p in the shared memory of CTA `rank` of this cluster, and a load from such an address
-__device__ __forceinline__ uint32_t dsmem_map(const float* p, uint32_t rank) {
+__device__ __forceinline__ uint32_t dsmem_map(const void* p, uint32_t rank) {
   uint32_t a;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   return a;
@@ -94,6 +94,11 @@ __device__ __forceinline__ float dsmem_ld(uint32_t a) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
   return v;
+}
+// `bytes` of this CTA's shared memory to an address of another's (both on 16 bytes), counted on a barrier there
+__device__ __forceinline__ void bulk_copy_to_peer(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "r"(smem_u32(src)), "r"(bytes), "r"(bar)
+               : "memory");
 }
 __device__ __forceinline__ float dsmem_ld(const float* p, uint32_t rank) { return dsmem_ld(dsmem_map(p, rank)); }
 
@@ -229,6 +234,11 @@ __device__ __forceinline__ uint32_t desc_hi(uint64_t d) { return static_cast<uin
 // mbarrier arrives once every MMA issued so far by this thread has completed
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// the same barrier of both CTAs of a pair gets an arrival
+__device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
 }
 
 // One lane of a converged warp.  Products are issued by a whole warp that runs their loop together and branches on this around each group of them:

@@ -4,14 +4,20 @@
 // One pass over K and V per row block, 64 keys a step, everything else on the chip:
 //   2 loader warps  : K rows with the fp16 cos / sin rows, and V rows (and row scales), each into a ring of stages of its own, by tensor-map copies
 //                     in 128-byte-swizzled rows.  (In one ring a stage stays until its V has been used, and the expanders waited for
-//                     copies a third of the time: 121 us instead of @@ at 64 new tokens of 32 / 8 heads over 32768 keys.)
+//                     copies a third of the time: 121 us instead of 106 at 64 new tokens of 32 / 8 heads over 32768 keys, when that was changed.)
 //   8 expander warps: K' = [a cos | plain | a sin], a = softplus, out of the stage into one of two operand tiles (the head's phase bias sits in Q');
-//                     of a cache that holds 8 bits also V as 16-bit values
+//                     of a cache that holds 8 bits also V as 16-bit values.  Four of them take the even steps, four the odd ones: the waits
+//                     and arrivals of a step, about 500 clocks, are then behind the other group's work.
 //   score warp      : S = Q' K'^T, Q' in tensor memory, into one of two buffers
 //   8 softmax warps : two threads per row, online softmax, P over S
 //   PV warp         : O += P V into an accumulator for each of a row's two threads, which so need not agree on a maximum; V from its stage (16 bits) or the expanders' tile (8 bits)
-// The step is bound by instruction issue of the expanders and the softmax (about 60 warp instructions a key at r = 64) next to the 512 bytes
-// of K and V a key at 16 bits.  Small grids are cut along the keys as in tc_attn_paged.cu.
+// Where a key head has two row blocks, a cluster of two CTAs takes them, step by step over the same keys: each expands half of a step's keys and
+// sends its part of the operand tile to the other's shared memory.  64 new tokens of 32 / 8 heads over 32768 keys, us, each CTA for itself / pairs:
+// r = 64 82 / 77, r = 128 99 / 92; int8 112 / 103, 139 / 120.  (Pairs with all expanders on every step: 83, 90, 114, 130.)
+// What bounds a step (1.8K clocks at 64 keys): the chain through one of the two score buffers -- S 600, softmax 1200, P V 500, with 250 to 300 for
+// each hand-over -- which only two steps overlap; tensor memory has no room for a third next to Q' and two outputs at d = 128.  The
+// special functions (770), the matrix instructions (800) and the 512 bytes of K and V a key at 16 bits are below that.  Small grids are cut
+// along the keys as in tc_attn_paged.cu.
 #include <algorithm>
 #include <type_traits>
 
@@ -34,7 +40,7 @@ struct PagedStreamP {
 };
 
 constexpr int SK_KEYS = 64;
-constexpr int SK_EX = PAGED_SM_WARPS, SK_EX_WARPS = 8, SK_EX_THREADS = 32 * SK_EX_WARPS;   // first expander warp
+constexpr int SK_EX = PAGED_SM_WARPS, SK_EX_WARPS = 8, SK_EX_GROUP = SK_EX_WARPS / 2;   // first expander warp; groups of warps take the steps in turn
 constexpr int SK_KLOAD = SK_EX + SK_EX_WARPS, SK_VLOAD = SK_KLOAD + 1, SK_S = SK_KLOAD + 2, SK_PV = SK_KLOAD + 3;
 constexpr int SK_THREADS = 32 * (SK_PV + 1);
 constexpr int SK_CS = SK_KEYS * 16;                // chunk stride of an operand tile
@@ -53,20 +59,24 @@ enum {
   SK_KEMPTY = SK_KFULL + SK_MAX_STAGES,    // [kstages] the expanders have read them
   SK_VFULL = SK_KEMPTY + SK_MAX_STAGES,    // [vstages] V has landed
   SK_VEMPTY = SK_VFULL + SK_MAX_STAGES,    // [vstages] its stage may be refilled: O += P V has completed (16 bits), the expanders have read it (8 bits)
-  SK_COUNT = SK_VEMPTY + SK_MAX_STAGES
+  SK_VTFREE = SK_VEMPTY + SK_MAX_STAGES,  // [2] pairs at 8 bits: O += P V of the step has completed in both CTAs
+  SK_COUNT = SK_VTFREE + 2
 };
 
-template <typename T, int STORE, int D>
+// PAIR: a cluster of two CTAs has the two row blocks of a key head; each expands half of a step's keys for both
+template <typename T, int STORE, int D, bool PAIR>
 __global__ void __launch_bounds__(SK_THREADS, 1)
     paged_stream_kernel(PagedStreamP p, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
                         const __grid_constant__ CUtensorMap tmap_t, const __grid_constant__ CUtensorMap tmap_ks, const __grid_constant__ CUtensorMap tmap_vs) {
   constexpr bool Q8 = STORE != POPE_STORE_16;
   constexpr int DC = D / 8, KBLK = (D * (Q8 ? 1 : 2) + 127) / 128;
+  constexpr int KROWS = PAIR ? SK_KEYS / 2 : SK_KEYS, VROWS = PAIR && Q8 ? SK_KEYS / 2 : SK_KEYS;   // keys of a step whose K, V this CTA loads
+  constexpr int KBYTES = KROWS * 128, VBYTES = VROWS * 128;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int r = p.r, RC = r / 8, tblk = (r + 63) / 64, KC = DC + p.RP / 8, KSTEPS = KC / 2;
-  constexpr int trig_at = KBLK * SK_BLOCK, vscale_at = KBLK * SK_BLOCK, vstage = vscale_at + (Q8 ? 1024 : 0);
-  const int scale_at = trig_at + 2 * tblk * SK_BLOCK, kstage = scale_at + (Q8 ? 1024 : 0);
+  constexpr int trig_at = KBLK * KBYTES, vscale_at = KBLK * VBYTES, vstage = vscale_at + (Q8 ? 1024 : 0);
+  const int scale_at = trig_at + 2 * tblk * KBYTES, kstage = scale_at + (Q8 ? 1024 : 0);
   uint8_t* vring = smem + p.kstages * kstage;
   uint8_t* Ks = vring + p.vstages * vstage;                        // [2][KC][SK_CS]
   uint8_t* Vs = Ks + 2 * KC * SK_CS;                               // 8 bits: [2][DC][SK_CS]
@@ -85,8 +95,9 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
   }
   if (tid == 0) {
     for (int i = 0; i < SK_COUNT; ++i) {
-      const bool ex = i < SK_KREADY + 2 || (i >= SK_KEMPTY && i < SK_VFULL) || (Q8 && i >= SK_VEMPTY), sm = i == SK_PFULL || i == SK_PFULL + 1 || i == SK_QFULL;
-      mbar_init(&bars[i], ex ? SK_EX_WARPS : sm ? PAGED_SM_WARPS : 1);
+      const bool ex = i < SK_KREADY + 2 || (i >= SK_KEMPTY && i < SK_VFULL) || (Q8 && i >= SK_VEMPTY && i < SK_VTFREE), sm = i == SK_PFULL || i == SK_PFULL + 1 || i == SK_QFULL;
+      const bool two = PAIR && (i == SK_KFREE || i == SK_KFREE + 1 || i >= SK_VTFREE);
+      mbar_init(&bars[i], ex ? SK_EX_GROUP : sm ? PAGED_SM_WARPS : two ? 2 : 1);
     }
     mbar_init_fence();
     *dropped = 0;
@@ -94,12 +105,14 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
   pdl_wait();
   pdl_trigger();
   // unit (sequence, key head), row block (late ones, which see more keys, first), key range
-  const int split = blockIdx.x % p.nsplit, ub = blockIdx.x / p.nsplit, u = ub / p.blocks, rb = p.blocks - 1 - ub % p.blocks;
+  const int rank = PAIR ? blockIdx.x & 1 : 0, at = PAIR ? blockIdx.x >> 1 : blockIdx.x;
+  const int split = at % p.nsplit, ub = PAIR ? at / p.nsplit * 2 + rank : at / p.nsplit, u = ub / p.blocks, rb = p.blocks - 1 - ub % p.blocks;
   const int b = u / p.Hk, hk = u % p.Hk;
   const int len = max(0, min(p.seq_lens[b], p.Nk)), cnt = p.counts ? max(0, min(p.counts[b], p.Nq)) : p.Nq;
   const int rows = min(PAGED_ROWS, cnt * p.G - rb * PAGED_ROWS);                       // of this block that are queries
   const int first_pos = len - cnt + rb * PAGED_ROWS / p.G;                             // position of the first one
-  const int kend = rows > 0 ? max(0, min(len, len - cnt + (rb * PAGED_ROWS + rows - 1) / p.G + 1)) : 0;
+  // keys that the last one sees (of a pair: the last row of both blocks, so that they take the same steps)
+  const int kend = PAIR ? (cnt > 0 ? len : 0) : rows > 0 ? max(0, min(len, len - cnt + (rb * PAGED_ROWS + rows - 1) / p.G + 1)) : 0;
   const int tiles_all = (kend + SK_KEYS - 1) / SK_KEYS;
   const int t0 = (int)((int64_t)tiles_all * split / p.nsplit), T_tiles = (int)((int64_t)tiles_all * (split + 1) / p.nsplit) - t0;
   for (int i = tid; i < r; i += SK_THREADS) sincos_reduced(p.bias[hk * p.bias_sh + i], &bias_cs[r + i], &bias_cs[i]);
@@ -108,7 +121,8 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
       *reinterpret_cast<uint4*>(Ks + (i / SK_KEYS * KC + DC + RC) * SK_CS + i % SK_KEYS * 16) = make_uint4(0, 0, 0, 0);
   fence_async_smem();
   fence_before_sync();
-  __syncthreads();
+  if constexpr (PAIR) __syncwarp(), cluster_sync();   // (the other CTA's barriers are there)
+  else __syncthreads();
   fence_after_sync();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   bool failed = false;
@@ -132,20 +146,20 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
         if (failed) {
           drain_copies(&bars[fulls], stages, j - stages, j);
         } else {
-          const int key0 = (t0 + j) * SK_KEYS, row = key0 % p.page_size;
+          const int key0 = (t0 + j) * SK_KEYS + (is_k || Q8 ? rank * KROWS : 0), row = key0 % p.page_size;
           uint64_t* bar = &bars[fulls + s];
           if (is_k) {
             uint8_t* st = smem + s * kstage;
-            mbar_expect_tx(bar, (uint32_t)(scale_at + (Q8 ? 4 * SK_KEYS : 0)));
+            mbar_expect_tx(bar, (uint32_t)(scale_at + (Q8 ? 4 * KROWS : 0)));
 #pragma unroll
-            for (int c = 0; c < KBLK; ++c) tma_load_4d(st + c * SK_BLOCK, &tmap_k, bar, c * 128, row, hk, pg);
-            for (int c = 0; c < tblk; ++c) tma_load_4d(st + trig_at + 2 * c * SK_BLOCK, &tmap_t, bar, c * 64, key0, 0, 0);
+            for (int c = 0; c < KBLK; ++c) tma_load_4d(st + c * KBYTES, &tmap_k, bar, c * 128, row, hk, pg);
+            for (int c = 0; c < tblk; ++c) tma_load_4d(st + trig_at + 2 * c * KBYTES, &tmap_t, bar, c * 64, key0, 0, 0);
             if constexpr (Q8) tma_load_4d(st + scale_at, &tmap_ks, bar, row, hk, pg, 0);
           } else {
             uint8_t* st = vring + s * vstage;
-            mbar_expect_tx(bar, (uint32_t)(vscale_at + (Q8 ? 4 * SK_KEYS : 0)));
+            mbar_expect_tx(bar, (uint32_t)(vscale_at + (Q8 ? 4 * VROWS : 0)));
 #pragma unroll
-            for (int c = 0; c < KBLK; ++c) tma_load_4d(st + c * SK_BLOCK, &tmap_v, bar, c * 128, row, hk, pg);
+            for (int c = 0; c < KBLK; ++c) tma_load_4d(st + c * VBYTES, &tmap_v, bar, c * 128, row, hk, pg);
             if constexpr (Q8) tma_load_4d(st + vscale_at, &tmap_vs, bar, row, hk, pg, 0);
           }
         }
@@ -174,7 +188,7 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
         }
       for (; ks < KSTEPS; ++ks)
         if (leader) mma_ts_lh(d, tmem + ks * 8, blo + ks * ((2 * SK_CS) >> 4), desc_hi(bd0), idesc, ks > 0 ? 1u : 0u);
-      if (leader) mma_commit(&bars[SK_SFULL + buf]), mma_commit(&bars[SK_KFREE + buf]);
+      if (leader) mma_commit(&bars[SK_SFULL + buf]), PAIR ? mma_commit_pair(&bars[SK_KFREE + buf]) : mma_commit(&bars[SK_KFREE + buf]);
     }
   } else if (warp == SK_PV) {
     const bool leader = elect_one();
@@ -198,18 +212,32 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
         if (j == T_tiles - 1) mma_commit(&bars[SK_ODONE]);
         mma_commit(&bars[SK_PVDONE + buf]);
         if constexpr (!Q8) mma_commit(&bars[SK_VEMPTY + s]);
+        if constexpr (Q8 && PAIR) mma_commit_pair(&bars[SK_VTFREE + buf]);
       }
       if (++s == p.vstages) s = 0, par ^= 1;
     }
   } else if (warp >= SK_EX) {
     // =============================== expanders =====================================================
-    const int et = tid - 32 * SK_EX;
+    const int group = (warp - SK_EX) / SK_EX_GROUP, et = tid - 32 * (SK_EX + group * SK_EX_GROUP);
     // A thread keeps its row and takes every fourth 16-byte column: a warp's columns are rotated or plain for all of its lanes, its accesses to the
     // swizzled stage and to the operand tile fall on distinct banks, and the tile needs no padding.  (With columns along the lanes and a padded
     // tile, whose 128-byte groups the tensor core then reads in two, shared memory set the pace: a third more bytes.)
-    const int row = et & (SK_KEYS - 1), c_first = et / SK_KEYS;
-    constexpr int CSTEP = SK_EX_THREADS / SK_KEYS;
-    for (int j = 0, s = 0, par = 0, vs = 0, vpar = 0; j < T_tiles; ++j) {   // (vs, vpar: 8 bits)
+    const int row = et & (KROWS - 1), c_first = et / KROWS;
+    constexpr int CSTEP = 32 * SK_EX_GROUP / KROWS;
+    const int trow0 = rank * KROWS + row;   // of the operand tile
+    // Of a pair: a warp has 32 rows of every fourth column, 512 bytes each in either tile, which it sends over when it is done with them.  The
+    // tile's barrier counts them: a step is ready when this CTA's warps have arrived and the other's bytes are there.
+    const uint32_t sent = PAIR ? (DC + RC + (Q8 ? DC : 0)) * KROWS * 16 : 0;
+    auto send = [&](uint8_t* tile, int buf, int columns) {   // columns c_first, c_first + CSTEP, .. of the first `columns`
+      if constexpr (PAIR) {
+        const int c = c_first + lane * CSTEP;
+        if (c < columns) {
+          uint8_t* from = tile + c * SK_CS + rank * KROWS * 16;
+          bulk_copy_to_peer(dsmem_map(from, rank ^ 1), from, KROWS * 16, dsmem_map(&bars[SK_KREADY + buf], rank ^ 1));
+        }
+      }
+    };
+    for (int j = group, s = group, par = 0, vs = group, vpar = 0; j < T_tiles; j += 2) {   // (rings of at least two stages; vs, vpar: 8 bits)
       const int buf = j & 1;
       const uint8_t* st = smem + s * kstage;
       const float* scl = reinterpret_cast<const float*>(st + scale_at);
@@ -218,7 +246,7 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
       if (failed) break;
       uint8_t* kt = Ks + buf * KC * SK_CS;
       auto swizzled = [&](const uint8_t* base, int row, int byte) {   // 16 (or 8) bytes of a 128-byte-swizzled row
-        return base + (byte >> 7) * SK_BLOCK + row * 128 + ((((byte >> 4) & 7) ^ (row & 7)) << 4) + (byte & 15);
+        return base + (byte >> 7) * KBYTES + row * 128 + ((((byte >> 4) & 7) ^ (row & 7)) << 4) + (byte & 15);
       };
       using Raw = std::conditional_t<Q8, uint2, uint4>;   // eight features
       auto raw_of = [&](const uint8_t* base, int row, int c) { return *reinterpret_cast<const Raw*>(swizzled(base, row, c * (Q8 ? 8 : 16))); };
@@ -232,8 +260,8 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
         for (int k = 0; k < 2; ++k) {
           const int c = k == 0 || both ? c0 + k * CSTEP : c0;
           raw[k] = raw_of(st, row, c);
-          const uint8_t* trow = st + trig_at + (c >> 3) * 2 * SK_BLOCK + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-          cq[k] = *reinterpret_cast<const uint4*>(trow), sq[k] = *reinterpret_cast<const uint4*>(trow + SK_BLOCK);
+          const uint8_t* trow = st + trig_at + (c >> 3) * 2 * KBYTES + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+          cq[k] = *reinterpret_cast<const uint4*>(trow), sq[k] = *reinterpret_cast<const uint4*>(trow + KBYTES);
         }
         float2 y[2][4];
         uint4 oc[2], os[2];
@@ -244,32 +272,38 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int c = c0 + k * CSTEP;
-          if (k == 0 || both) *reinterpret_cast<uint4*>(kt + c * SK_CS + row * 16) = oc[k], *reinterpret_cast<uint4*>(kt + (DC + c) * SK_CS + row * 16) = os[k];
+          if (k == 0 || both) *reinterpret_cast<uint4*>(kt + c * SK_CS + trow0 * 16) = oc[k], *reinterpret_cast<uint4*>(kt + (DC + c) * SK_CS + trow0 * 16) = os[k];
         }
       }
 #pragma unroll 2
-      for (int c = RC + c_first; c < DC; c += CSTEP) *reinterpret_cast<uint4*>(kt + c * SK_CS + row * 16) = plain8<T, STORE>(raw_of(st, row, c), kscale);
+      for (int c = RC + (PAIR ? (c_first - RC) & (CSTEP - 1) : c_first); c < DC; c += CSTEP)   // (a pair's columns are those that the warp sends)
+        *reinterpret_cast<uint4*>(kt + c * SK_CS + trow0 * 16) = plain8<T, STORE>(raw_of(st, row, c), kscale);
       fence_async_smem();   // the tile is visible to the tensor core; the stage has been read
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[SK_KEMPTY + s]);
+      send(kt, buf, DC), send(kt + DC * SK_CS, buf, RC);
       if constexpr (Q8) {   // V's values, zeros behind the last key
         failed = !mbar_wait(&bars[SK_VFULL + vs], vpar, WAIT_LIMIT);
-        if (j >= 2 && !failed) failed = !mbar_wait(&bars[SK_PVDONE + buf], ((j - 2) >> 1) & 1, WAIT_LIMIT);
+        if (j >= 2 && !failed) failed = !mbar_wait(&bars[(PAIR ? SK_VTFREE : SK_PVDONE) + buf], ((j - 2) >> 1) & 1, WAIT_LIMIT);
         if (failed) break;
-        const bool live = (t0 + j) * SK_KEYS + row < kend;
+        const bool live = (t0 + j) * SK_KEYS + trow0 < kend;
         const uint8_t* vst = vring + vs * vstage;
         uint8_t* vt = Vs + buf * DC * SK_CS;
         const float vscale = reinterpret_cast<const float*>(vst + vscale_at)[row];
 #pragma unroll
         for (int c = c_first; c < DC; c += CSTEP)
-          *reinterpret_cast<uint4*>(vt + c * SK_CS + row * 16) = live ? plain8<T, STORE>(raw_of(vst, row, c), vscale) : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(vt + c * SK_CS + trow0 * 16) = live ? plain8<T, STORE>(raw_of(vst, row, c), vscale) : make_uint4(0, 0, 0, 0);
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[SK_VEMPTY + vs]);
-        if (++vs == p.vstages) vs = 0, vpar ^= 1;
+        send(vt, buf, DC);
+        if ((vs += 2) >= p.vstages) vs -= p.vstages, vpar ^= 1;
       }
-      if (lane == 0) mbar_arrive(&bars[SK_KREADY + buf]);
-      if (++s == p.kstages) s = 0, par ^= 1;
+      if (lane == 0) {
+        if (PAIR && c_first == 0) mbar_expect_tx(&bars[SK_KREADY + buf], sent);
+        else mbar_arrive(&bars[SK_KREADY + buf]);
+      }
+      if ((s += 2) >= p.kstages) s -= p.kstages, par ^= 1;
     }
   } else {
     // =============================== softmax: two threads per query row ==========================
@@ -356,6 +390,7 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
       if (!all_vis) {   // (the same for all threads of these warps)
         uint4* vt = reinterpret_cast<uint4*>(Q8 ? Vs + buf * DC * SK_CS : vring + j % p.vstages * vstage);
         if (!Q8 && !failed) failed = !mbar_wait(&bars[SK_VFULL + j % p.vstages], (j / p.vstages) & 1, WAIT_LIMIT);
+        if (Q8 && PAIR && !failed) failed = !mbar_wait(&bars[SK_KREADY + buf], (j >> 1) & 1, WAIT_LIMIT);   // (V of the other CTA's keys)
         bool any = false;
         for (int i = tid; i < (Q8 ? DC * SK_CS : KBLK * SK_BLOCK) / 16; i += 32 * PAGED_SM_WARPS)
           any |= clean_v<T>(vt + i, key0 + (Q8 ? i & (SK_KEYS - 1) : i >> 3 & (SK_KEYS - 1)) >= kend);
@@ -372,7 +407,8 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
   }
   if (failed) atomicOr(p.status, 1u);
   fence_before_sync();
-  __syncthreads();
+  if constexpr (PAIR) __syncwarp(), cluster_sync();   // (nobody leaves while the other may still send)
+  else __syncthreads();
   if (warp == SK_S) tmem_dealloc(tmem, 512);
 }
 
@@ -407,8 +443,9 @@ static StreamWs stream_ws(const PopeShape& s) {
 }
 size_t paged_stream_workspace(const PopePagedAttnArgs& a) { return stream_ws(a.shape).total; }
 
-template <typename T, int STORE, int D> static cudaError_t paged_stream_t(const PopePagedAttnArgs& a, cudaStream_t st) {
+template <typename T, int STORE, int D, bool PAIR> static cudaError_t paged_stream_t(const PopePagedAttnArgs& a, cudaStream_t st) {
   constexpr bool Q8 = STORE != POPE_STORE_16;
+  constexpr int KROWS = PAIR ? SK_KEYS / 2 : SK_KEYS, VROWS = PAIR && Q8 ? SK_KEYS / 2 : SK_KEYS;
   constexpr int DC = D / 8, KBLK = (D * (Q8 ? 1 : 2) + 127) / 128;
   const PopeShape& s = a.shape;
   const PopePagedKV& kv = a.cache.kv;
@@ -428,15 +465,15 @@ template <typename T, int STORE, int D> static cudaError_t paged_stream_t(const 
   if (!p.status) return cudaErrorInvalidSymbol;
   CUtensorMap mk, mv, mt, mks, mvs;
   const int row_bytes = Q8 ? s.d : 2 * s.d;
-  bool ok = make_page_tmap(&mk, kv.k_pages, row_bytes, kv.page_size, s.Hk, kv.num_pages, SK_KEYS, 1) &&
-            make_page_tmap(&mv, kv.v_pages, row_bytes, kv.page_size, s.Hk, kv.num_pages, SK_KEYS, 1);
+  bool ok = make_page_tmap(&mk, kv.k_pages, row_bytes, kv.page_size, s.Hk, kv.num_pages, KROWS, 1) &&
+            make_page_tmap(&mv, kv.v_pages, row_bytes, kv.page_size, s.Hk, kv.num_pages, VROWS, 1);
   // (the maps of what a call does not have are not used)
-  ok = ok && (s.r > 0 ? make_trig_tmap(&mt, tt.ch, s.Nk, s.r, SK_KEYS) : (mt = mk, true));
-  ok = ok && (Q8 ? make_page_tmap(&mks, a.cache.k_scales, 0, kv.page_size, s.Hk, kv.num_pages, SK_KEYS, 1) &&
-                       make_page_tmap(&mvs, a.cache.v_scales, 0, kv.page_size, s.Hk, kv.num_pages, SK_KEYS, 1)
+  ok = ok && (s.r > 0 ? make_trig_tmap(&mt, tt.ch, s.Nk, s.r, KROWS) : (mt = mk, true));
+  ok = ok && (Q8 ? make_page_tmap(&mks, a.cache.k_scales, 0, kv.page_size, s.Hk, kv.num_pages, KROWS, 1) &&
+                       make_page_tmap(&mvs, a.cache.v_scales, 0, kv.page_size, s.Hk, kv.num_pages, VROWS, 1)
                  : (mks = mvs = mk, true));
   if (!ok) return cudaErrorNotSupported;
-  const size_t kstage = (size_t)(KBLK + 2 * ((s.r + 63) / 64)) * SK_BLOCK + (Q8 ? 1024 : 0), vstage = (size_t)KBLK * SK_BLOCK + (Q8 ? 1024 : 0);
+  const size_t kstage = (size_t)(KBLK + 2 * ((s.r + 63) / 64)) * KROWS * 128 + (Q8 ? 1024 : 0), vstage = (size_t)KBLK * VROWS * 128 + (Q8 ? 1024 : 0);
   const size_t fixed = 1024 + 2 * (size_t)(DC + p.RP / 8) * SK_CS + (Q8 ? 2 * (size_t)DC * SK_CS : 0) + 4 * PAGED_ROWS * 4 + 2 * (size_t)s.r * 4 + SK_COUNT * 8 + 16;
   // (V of a step is used about two steps after its K: one stage more)
   for (p.kstages = SK_MAX_STAGES; p.kstages >= 2; --p.kstages) {
@@ -446,17 +483,21 @@ template <typename T, int STORE, int D> static cudaError_t paged_stream_t(const 
   if (p.kstages < 2) return cudaErrorInvalidValue;
   // (every CTA allocates all 512 TMEM columns: two must not share an SM)
   const size_t smem = std::max<size_t>(fixed + p.kstages * kstage + p.vstages * vstage, 120 * 1024);
-  cudaError_t e = ensure_max_smem<paged_stream_kernel<T, STORE, D>>();
+  cudaError_t e = ensure_max_smem<paged_stream_kernel<T, STORE, D, PAIR>>();
   if (e != cudaSuccess) return e;
   const unsigned blocks = (unsigned)(s.B * s.Hk * p.blocks);
   const dim3 grid(blocks * (unsigned)p.nsplit), block(SK_THREADS);
   if (s.r > 0 && (e = launch_paged_tables(a.embed, s.Nk, s.r, tt.ch, tt.sh, nullptr, 0, st)) != cudaSuccess) return e;
-  e = launch_dependent(paged_stream_kernel<T, STORE, D>, grid, block, smem, st, p, mk, mv, mt, mks, mvs);
+  e = PAIR ? launch_clusters(paged_stream_kernel<T, STORE, D, PAIR>, 2, grid, block, smem, st, true, p, mk, mv, mt, mks, mvs)
+           : launch_dependent(paged_stream_kernel<T, STORE, D, PAIR>, grid, block, smem, st, p, mk, mv, mt, mks, mvs);
   return e != cudaSuccess || p.nsplit == 1 ? e : launch_paged_merge(p.e, s.dtype, s.d, (int)blocks, p.blocks, st);
+}
+template <typename T, int STORE, int D> static cudaError_t paged_stream_p(const PopePagedAttnArgs& a, cudaStream_t st) {
+  return stream_blocks(a.shape) == 2 ? paged_stream_t<T, STORE, D, true>(a, st) : paged_stream_t<T, STORE, D, false>(a, st);
 }
 template <typename T, int STORE> static cudaError_t paged_stream_d(const PopePagedAttnArgs& a, cudaStream_t st) {
   const int d = a.shape.d;
-  return d == 64 ? paged_stream_t<T, STORE, 64>(a, st) : d == 96 ? paged_stream_t<T, STORE, 96>(a, st) : paged_stream_t<T, STORE, 128>(a, st);
+  return d == 64 ? paged_stream_p<T, STORE, 64>(a, st) : d == 96 ? paged_stream_p<T, STORE, 96>(a, st) : paged_stream_p<T, STORE, 128>(a, st);
 }
 template <typename T> static cudaError_t paged_stream_s(const PopePagedAttnArgs& a, cudaStream_t st) {
   switch (a.cache.store) {
