@@ -334,8 +334,8 @@ typedef struct PopeKvReadArgs {
  * is the query of position seq_lens[b] - counts[b] + i and sees the keys up to that position; counts (device, may be NULL = Nq
  * everywhere) is clamped to [0, Nq].  Rows behind the count, and rows whose position is negative, give out = 0, lse = -inf.
  * shape.Nk = an upper bound of every seq_lens[b], as for PopePagedDecodeArgs, at most 2^24; shape.Nq may exceed it.  dtype is that of q and
- * out and, with POPE_STORE_16, of the pages.  lse (B, H, Nq) fp32 may be NULL.  Workspace: pope_b200_workspace_bytes(
- * POPE_OP_ATTN_PAGED, &args). */
+ * out and, with POPE_STORE_16, of the pages.  lse (B, H, Nq) fp32 may be NULL.  out has its rows on 16-byte boundaries, freqs
+ * one table for all.  Workspace: pope_b200_workspace_bytes(POPE_OP_ATTN_PAGED, &args), on 256 bytes. */
 typedef struct PopePagedAttnArgs {
   uint32_t struct_bytes;
   float softmax_scale;
@@ -388,8 +388,8 @@ POPE_API int pope_b200_abi_version(void);
 POPE_API const char* pope_b200_status_str(int status);
 
 /* Name of the kernel family the last successful call ON THIS THREAD dispatched to: "tcgen05" (tensor
- * cores), "decode_stream" / "decode_stream_paged" (one 16-bit query row, streamed keys), "kv_append", "simt"
- * (the exact-arithmetic kernels).  Diagnostic only. */
+ * cores), "decode_stream" / "decode_stream_paged" (one 16-bit query row, streamed keys), "kv_append",
+ * "kv_write", "kv_read", "attn_paged" (the paged cache), "simt" (the exact-arithmetic kernels).  Diagnostic only. */
 POPE_API const char* pope_b200_last_path(void);
 
 /* Sticky device-side status of the tensor-core kernels on the current device: 0 = healthy,
