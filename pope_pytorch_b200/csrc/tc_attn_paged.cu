@@ -478,7 +478,8 @@ __global__ void __launch_bounds__(PS_THREADS, 1) paged_sweep_kernel(PagedSweepP 
 static int sweep_blocks(const PopeShape& s) { return (int)(((int64_t)s.Nq * (s.H / s.Hk) + PS_ROWS - 1) / PS_ROWS); }
 
 // Key ranges per row block: whole waves of one CTA per SM times a CTA's steps plus what it costs beside them (Q', the epilogue
-// and the merge, about ten steps' time).
+// and the merge, about ten steps' time).  The first cut has to promise a sixteenth: parts are written and read again (2048 tokens of
+// 32 / 8 heads over 16384 keys, whose halves promise 3 %: 615 us whole, 640 cut).
 static int sweep_split(const PopeShape& s) {
   const int tiles = (s.Nk + PS_KEYS - 1) / PS_KEYS;
   const int64_t units = (int64_t)s.B * s.Hk * sweep_blocks(s);
@@ -486,7 +487,7 @@ static int sweep_split(const PopeShape& s) {
   int64_t best_cost = INT64_MAX;
   for (int n = 1; n <= std::min(tiles, PAGED_MAX_SPLIT); ++n) {
     const int64_t cost = (units * n + 147) / 148 * ((tiles + n - 1) / n + (n > 1 ? 10 : 6));
-    if (cost < best_cost) best = n, best_cost = cost;
+    if (cost < (n > 1 && best == 1 ? best_cost - best_cost / 16 : best_cost)) best = n, best_cost = cost;
   }
   return best;
 }
@@ -579,14 +580,20 @@ bool attn_paged_supported(const PopePagedAttnArgs& a) {
 // against 31 by the expanders in front of tcgen05, 16 rows 29 / 31, 20 rows 38 / 31; int8 16 rows 32 / 39).  Up to two row blocks they are
 // expanded on the chip, from three on written to memory once ((1, 32 / 8, 32768, 128), r = 64: 256 rows 77 / 98, 384 rows 111 / 109, 512 rows 153 / 128;
 // int8 103 / 114, 146 / 125; int8 with r = 128 and 256 rows 120 / 129).
+// The images are up to 1.5 times (16 bits) or 2.4 times (8 bits, r = 64) what the cache holds, and every sequence's has the room of the longest one:
+// beyond 8 GB of them the keys are expanded on the chip for each row block, whatever their number.
+constexpr size_t IMAGES_MOST = (size_t)8 << 30;
 enum class Paged { kRows, kStream, kSweep };
-static Paged paged_kernel(const PopeShape& s) {
+static Paged paged_kernel(const PopePagedAttnArgs& a) {
+  const PopeShape& s = a.shape;
   const int64_t rows = (int64_t)s.Nq * (s.H / s.Hk);
-  return rows <= 16 ? Paged::kRows : rows <= 2 * PAGED_ROWS ? Paged::kStream : Paged::kSweep;
+  if (rows <= 16) return Paged::kRows;
+  const SweepWs ws = sweep_ws(s, a.cache.store);
+  return rows <= 2 * PAGED_ROWS || ws.part_o - ws.kimg > IMAGES_MOST ? Paged::kStream : Paged::kSweep;
 }
 
 size_t attn_paged_workspace(const PopePagedAttnArgs& a) {
-  switch (paged_kernel(a.shape)) {
+  switch (paged_kernel(a)) {
     case Paged::kRows: return paged_rows_workspace(a);
     case Paged::kStream: return paged_stream_workspace(a);
     default: return paged_sweep_workspace(a);
@@ -594,7 +601,7 @@ size_t attn_paged_workspace(const PopePagedAttnArgs& a) {
 }
 
 cudaError_t attn_paged(const PopePagedAttnArgs& a, cudaStream_t st) {
-  switch (paged_kernel(a.shape)) {
+  switch (paged_kernel(a)) {
     case Paged::kRows: return paged_rows(a, st);
     case Paged::kStream: return paged_stream(a, st);
     default: return paged_sweep(a, st);

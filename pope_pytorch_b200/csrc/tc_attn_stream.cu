@@ -415,7 +415,8 @@ __global__ void __launch_bounds__(SK_THREADS, 1)
 // ---- host side -----------------------------------------------------------------------------------------
 static int stream_blocks(const PopeShape& s) { return (int)(((int64_t)s.Nq * (s.H / s.Hk) + PAGED_ROWS - 1) / PAGED_ROWS); }
 
-// Key ranges per row block: whole waves of one CTA per SM times a CTA's steps plus what it costs beside them (about twelve steps' time).
+// Key ranges per row block: whole waves of one CTA per SM times a CTA's steps plus what it costs beside them (about twelve steps' time; the first
+// cut has to promise a sixteenth, as in tc_attn_paged.cu).
 static int stream_split(const PopeShape& s) {
   const int tiles = (s.Nk + SK_KEYS - 1) / SK_KEYS;
   const int64_t units = (int64_t)s.B * s.Hk * stream_blocks(s);
@@ -423,7 +424,7 @@ static int stream_split(const PopeShape& s) {
   int64_t best_cost = INT64_MAX;
   for (int n = 1; n <= std::min(tiles, PAGED_MAX_SPLIT); ++n) {
     const int64_t cost = (units * n + 147) / 148 * ((tiles + n - 1) / n + (n > 1 ? 12 : 8));
-    if (cost < best_cost) best = n, best_cost = cost;
+    if (cost < (n > 1 && best == 1 ? best_cost - best_cost / 16 : best_cost)) best = n, best_cost = cost;
   }
   return best;
 }

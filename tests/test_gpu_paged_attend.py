@@ -407,6 +407,24 @@ def test_drawn_shapes(seed):
     assert _native.device_status() == 0
 
 
+@pytest.mark.parametrize("store", [None, I8])
+def test_one_long_sequence_among_many(store):
+    """Forty sequences, one of 110000 keys: more than 8 GB of expanded keys, were each given the room of the longest."""
+    g = torch.Generator(device=DEV).manual_seed(9)
+    b, hk, d, r, new, n = 40, 8, 64, 64, 300, 110000
+    lens = [n if i == 7 else 305 + i for i in range(b)]
+    cache = PagedKVCache(b, hk, d, num_pages=-(-n // 256) + 2 * b, page_size=256, max_seq_len=n, dtype=BF, store=store)
+    fill(cache, lens, g)
+    q = torch.randn(b, hk, new, d, device=DEV, generator=g).bfloat16()
+    emb = table(r, hk, n, g)
+    got = cache.attend(q, emb)
+    for i in (0, 7, 39):
+        k, v = (x.float() for x in cache.gather(i)) if store is None else (c * s[..., None] for c, s in stored(cache, i))
+        want = R.attend(q[i:i + 1, :, -40:], [k], [v], emb[0], emb[1], [lens[i]], [40], d ** -0.5)
+        R.check(got[i:i + 1, :, -40:], want[0], want[2], want[3])
+    assert _native.device_status() == 0
+
+
 def test_against_the_attention_over_contiguous_keys():
     """Every position of a prompt at once: the causal forward over the same keys."""
     g = torch.Generator(device=DEV).manual_seed(31)

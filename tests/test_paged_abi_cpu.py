@@ -129,3 +129,10 @@ def test_attention(lib, ptr):
         assert call(lib, name, a) == MISALIGNED
     a = make_attn(ptr, dict(d=80))
     assert lib.pope_b200_workspace_bytes(N.OP_ATTN_PAGED, C.addressof(a)) == 0
+
+
+def test_images_of_a_large_cache_stay_out_of_the_workspace(lib, ptr):
+    """Sixty-four sequences of up to 131072 keys: expanded keys of all of them would be 27 GB and more."""
+    for kind in (N.STORE_16, N.STORE_INT8):
+        a = make_attn(ptr, dict(B=64, H=8, Hk=8, Nq=2048, Nk=131072), cache=store(ptr, store=kind, most=512))
+        assert 0 < lib.pope_b200_workspace_bytes(N.OP_ATTN_PAGED, C.addressof(a)) < 1 << 30
