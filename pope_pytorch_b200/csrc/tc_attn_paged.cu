@@ -1,5 +1,5 @@
 // Attention of a chunk of new tokens over a paged cache on the Blackwell tensor cores (tcgen05 + TMEM), sm_100a only: for chunks whose rows per
-// key head are many (paged_rows.cu takes the others).
+// key head are many (paged_rows.cu and tc_attn_stream.cu take the others; the choice is made here).
 //
 // The query rows that share a key head are packed, row = token * group + head, and a CTA owns 128 of them: the heads of a group read K and V
 // once.  Three launches:

@@ -1,5 +1,6 @@
 // Attention of a MODERATE number of new tokens per sequence over a paged cache on the Blackwell tensor cores (tcgen05 + TMEM), sm_100a only: the rows
-// of a key head fill one or two blocks of 128, so that writing expanded keys to memory for them (tc_attn_paged.cu) would cost more than they do.
+// of a key head fill one or two blocks of 128, so that writing expanded keys to memory for them (tc_attn_paged.cu) would cost more than they do
+// (or any number of blocks, where the memory that takes is not to be had).
 //
 // One pass over K and V per row block, 64 keys a step, everything else on the chip:
 //   2 loader warps  : K rows with the fp16 cos / sin rows, and V rows (and row scales), each into a ring of stages of its own, by tensor-map copies
