@@ -90,8 +90,9 @@ __device__ __forceinline__ void write_rows(const KvWriteP& p, int b, int len, in
   }
 }
 
+// (five CTAs per SM: four waited for memory, 50 us against 47 for 32768 tokens of 8 key heads of 128)
 template <typename T, int STORE, int D>
-__global__ void __launch_bounds__(256) kv_write_kernel(KvWriteP p) {
+__global__ void __launch_bounds__(256, 5) kv_write_kernel(KvWriteP p) {
   constexpr int LPR = D == 64 ? 8 : 16;
   const int group = threadIdx.x / LPR, lane = threadIdx.x % LPR, b = blockIdx.z;
   pdl_wait();
